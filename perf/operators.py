@@ -125,7 +125,7 @@ def prepare(case, seed):
         import numpy as np
 
         def arr(t, dtype=np.float32):
-            return None if t is None else cb.DeviceArray(tuple(t.shape), dtype, _ptr=t.data_ptr(), _owner=t)
+            return None if not isinstance(t, torch.Tensor) else cb.DeviceArray(tuple(t.shape), dtype, _ptr=t.data_ptr(), _owner=t)
 
         s["dev"] = {key: arr(s.get(key)) for key in ("g", "out", "w", "m", "x", "bias", "values")}
         if "packed" in s:
