@@ -21,6 +21,28 @@ int sm_count();
 // slot 1: matmul workspace.
 ctk_status device_scratch(int slot, size_t bytes, void** out);
 
+// Scratch for one call: allocated from the device's pool and given back in the order of `stream`, so calls on
+// different streams never share it, and a call that is being captured records its own allocation in the graph.
+ctk_status stream_alloc(size_t bytes, void* stream, void** out);
+struct StreamScratch {
+    void* p = nullptr;
+    void* stream = nullptr;
+    ctk_status get(size_t bytes, void* st) { stream = st; return stream_alloc(bytes, st, &p); }
+    StreamScratch() = default;
+    ~StreamScratch() { if (p && cudaFreeAsync(p, reinterpret_cast<cudaStream_t>(stream)) != cudaSuccess) (void)cudaGetLastError(); }
+    StreamScratch(const StreamScratch&) = delete;
+    StreamScratch& operator=(const StreamScratch&) = delete;
+};
+
+inline bool aligned_to(const void* p, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+// Whether two [rows, cols] fp32 arrays of row pitch lda / ldb share a byte between their first and last element.
+inline bool spans_overlap(const void* a, int64_t rows_a, int64_t cols_a, int64_t lda, const void* b, int64_t rows_b, int64_t cols_b, int64_t ldb) {
+    if (rows_a <= 0 || cols_a <= 0 || rows_b <= 0 || cols_b <= 0) return false;
+    const uintptr_t a0 = reinterpret_cast<uintptr_t>(a), b0 = reinterpret_cast<uintptr_t>(b);
+    const uintptr_t a1 = a0 + 4 * static_cast<uintptr_t>((rows_a - 1) * lda + cols_a), b1 = b0 + 4 * static_cast<uintptr_t>((rows_b - 1) * ldb + cols_b);
+    return a0 < b1 && b0 < a1;
+}
+
 inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s); }
 
 // NVTX range around the host side of an entry point (header-only NVTX: a no-op costing a few

@@ -83,6 +83,14 @@ static ctk_status ensure_pool() {
     return CTK_OK;
 }
 
+ctk_status stream_alloc(size_t bytes, void* stream, void** out) {
+    *out = nullptr;
+    ctk_status st = ensure_pool();
+    if (st) return st;
+    CTK_CUDA(cudaMallocAsync(out, bytes, reinterpret_cast<cudaStream_t>(stream)));
+    return CTK_OK;
+}
+
 }  // namespace ctk
 
 using namespace ctk;

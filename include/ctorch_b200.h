@@ -396,6 +396,63 @@ ctk_status ctk_matmul_profile_read(int64_t* launches, double* total_ms, double* 
 ctk_status ctk_matmul_status(int* status);
 
 /* ------------------------------------------------------------------------------------------- */
+/* Orthogonalised updates (no counterpart in the reference, whose only update is SGD).          */
+/* ------------------------------------------------------------------------------------------- */
+/* out = NS(g), the matrix with g's singular vectors and singular values brought near 1 by `steps`
+ * Newton-Schulz steps:  X = g / (|g|_F + eps), then  X <- a X + (b A + c A A) X,  A = X X^T
+ * (A = X^T X and X on the left where rows > cols), (a, b, c) = (3.4445, -4.7750, 2.0315).
+ * g is [rows, cols] with row pitch ldg >= cols, out with row pitch ldo >= cols (elements; any 4-byte
+ * aligned pointers); out == g with the same pitch is allowed, other overlaps are not.  fp32-level accuracy: the products
+ * take both operands as 22-bit fixed-precision pairs of fp16 and are summed in fp32 with rounding.  A
+ * non-finite element of g makes every element of out NaN; g == 0 gives 0.  The same bits from call to call.
+ * workspace: ctk_orthogonalize_workspace_bytes(rows, cols) bytes of device memory, 256-byte aligned, that
+ * no other running call uses, or NULL: taken from the device's pool for the duration of the call, in
+ * stream order (also while the stream is being captured).
+ * CTK_ERR_INVALID: negative extents, pitch below cols, steps outside [1, 64], eps not positive and finite,
+ * null or misaligned pointers.  CTK_ERR_LIMIT: more than 2^30 elements. */
+size_t ctk_orthogonalize_workspace_bytes(int64_t rows, int64_t cols);
+ctk_status ctk_orthogonalize_f32(const float* g, int64_t ldg, float* out, int64_t ldo, int64_t rows, int64_t cols,
+                                 int steps, float eps, void* workspace, void* stream);
+/* One orthogonalised step of a weight matrix, next to ctk_sgd_update_f32:
+ *   momentum <- mu momentum + g;  u = nesterov ? g + mu momentum : momentum;
+ *   p <- (1 - lr weight_decay) p - lr scale NS(u),
+ * p and momentum updated in place, g read only; pitches, NS, workspace and errors as above.  The three
+ * arrays must not overlap.  A non-finite element of u makes p NaN, as any update with it would in the end. */
+ctk_status ctk_muon_update_f32(float* p, int64_t ldp, const float* g, int64_t ldg, float* momentum, int64_t ldm,
+                               int64_t rows, int64_t cols, float lr, float mu, int nesterov, float weight_decay,
+                               float scale, int steps, float eps, void* workspace, void* stream);
+/* Device status word of these kernels' bounded waits: 0 = none ran out.  Synchronises the device. */
+ctk_status ctk_orthogonalize_status(int* status);
+
+/* ------------------------------------------------------------------------------------------- */
+/* 4-bit weights (no counterpart in the reference).                                             */
+/* A [k, n] weight W of y = x W as 4-bit codes with a scale per group of `group` (32, 64 or 128)  */
+/* consecutive k of one column:  W[l, j] = (code - zero) * scale.                               */
+/*   packed  n rows of kw = ceil(k / group) * group / 8 32-bit words: column j's codes, eight     */
+/*           consecutive k per word, code 2p of the eight in bits [4p, 4p+4), code 2p+1 in bits   */
+/*           [16+4p, 20+4p); 16-byte aligned.  Codes past k are written as the zero point and    */
+/*           never enter a result.                                                               */
+/*   scales  [n, ceil(k / group)] fp32;  zeros  the same shape in bytes (0..15), or NULL: zero = 8. */
+/* ------------------------------------------------------------------------------------------- */
+size_t ctk_w4_packed_bytes(int64_t k, int64_t n, int group);
+/* Quantises w [k, n] (row pitch ldw).  zeros == NULL: symmetric, scale = max|w| / 7 of the group, code =
+ * round(w / scale) + 8.  Otherwise scale = (max(w, 0) - min(w, 0)) / 15, zero = round(-min(w, 0) / scale), code =
+ * round(w / scale) + zero clamped to [0, 15].  Scales are rounded to the nearest fp32 number, quotients exactly
+ * (ties to even).  A group of zeros gets scale 0; a group with a non-finite weight gets scale NaN. */
+ctk_status ctk_w4_quantize_f32(const float* w, int64_t ldw, int64_t k, int64_t n, int group, uint32_t* packed,
+                               float* scales, uint8_t* zeros, void* stream);
+/* The values a 4-bit weight stands for, w [k, n] with row pitch ldw. */
+ctk_status ctk_w4_dequantize_f32(const uint32_t* packed, const float* scales, const uint8_t* zeros, int64_t k, int64_t n,
+                                 int group, float* w, int64_t ldw, void* stream);
+/* y = [relu](x W + bias): x [m, k] with row pitch ldx, y [m, n] with row pitch ldy, bias n floats or NULL.
+ * Made for few rows (the weight's bytes are the bound up to about 8 rows); any m is taken.  fp32-level accuracy:
+ * codes are exact in the products, x enters with its 24 bits, sums are fp32 per group and across groups, in
+ * an order that depends on the sizes only.  x must not overlap y. */
+ctk_status ctk_w4_matmul_f32(const float* x, int64_t ldx, const uint32_t* packed, const float* scales, const uint8_t* zeros,
+                             const float* bias, int relu, float* y, int64_t ldy, int64_t m, int64_t k, int64_t n,
+                             int group, void* stream);
+
+/* ------------------------------------------------------------------------------------------- */
 /* Data-parallel gradient exchange (no counterpart in the reference, which is single-process):  */
 /* one NCCL communicator per process, fp32 sum.                                                  */
 /* ------------------------------------------------------------------------------------------- */
