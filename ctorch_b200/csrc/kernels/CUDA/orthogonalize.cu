@@ -1,14 +1,33 @@
 // Orthogonalised updates: NS(G) by Newton-Schulz steps, and the weight update built on it.
 //
 //   X0 = G / (|G|_F + eps);  X <- a X + (b A + c A A) X,  A = X X^T (the short side's Gram matrix)
+//
+// Two passes over U (momentum update + norm, then scaling) and three products a step:
+//   GRAM   A = X X^T       symmetric: one triangle of tiles, each written to its mirror place too
+//   POLY   B = b A + c A A symmetric, the polynomial in the epilogue
+//   APPLY  X = a X + B X   (X B where rows > cols); the last one writes the result, or the weights of an update
+// The products run on the tensor cores at fp32 accuracy: every matrix is held as hi + lo, two fp16 numbers
+// (22 bits), and hi hi + hi lo + lo hi are three kind::f16 products into one accumulator -- 1.5 units of TF32-rate
+// work per fp32 product where a TF32 split costs 2 or 3, for the same 4 bytes per element.  fp16's range is no
+// obstacle here: the singular values of X never pass 1.21 (the step's polynomial maps [0, 1.21] into itself), so
+// |X| <= 1.21, |A| <= 1.46 and |B| <= 2.81 element by element, and a fixed power of two puts them high in fp16's range
+// (2^15, 2^15, 2^14); elements 2^-24 below the largest keep 11 bits or more between hi and lo.
+// The tensor core truncates as it adds into its fp32 accumulator, so an accumulator holds CHUNK_KB * 64 terms
+// at a time; the epilogue warps add those up in registers with rounding.
 #include <math.h>
 
-#include "common.cuh"
+#include <mutex>
+
+#include "tcgen05.cuh"
 
 namespace {
 using namespace ctk;
 
+__device__ int g_ns_status = 0;  // first bounded wait that ran out: (role << 8) | barrier, else 0
+
 constexpr float kA = 3.4445f, kB = -4.7750f, kC = 2.0315f;
+// Powers of two by which X, A (= X X^T) and B (= b A + c A A) are held.
+constexpr float kScaleX = 32768.0f;
 constexpr int PREP_THREADS = 256;
 
 struct Source {
@@ -23,62 +42,128 @@ struct Source {
 
 // ---- pass 1: momentum update and the Frobenius norm ------------------------------------------------------
 // |U|_F^2 as a double per CTA (one double multiply-add per element neither overflows nor loses small
-// elements); the partial sums are added in CTA order by whoever needs the norm.
-__global__ void __launch_bounds__(PREP_THREADS) prep_norm_kernel(Source S, double* __restrict__ partial) {
-    const int64_t total = S.rows * S.cols;
-    double acc = 0.0;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * PREP_THREADS + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * PREP_THREADS) {
-        const int64_t r = i / S.cols, c = i - r * S.cols;
-        float u = S.g[r * S.ldg + c];
-        if (S.momentum) {
-            float* mp = S.momentum + r * S.ldm + c;
-            const float m = fmaf(S.mu, *mp, u);
-            *mp = m;
-            u = S.nesterov ? fmaf(S.mu, m, u) : m;
-        }
-        acc = fma(static_cast<double>(u), static_cast<double>(u), acc);
-    }
+// elements); the partial sums are added in a fixed order by whoever needs the norm.  V elements per access (4 where
+// every pitch and pointer allows it).  Bound by the bytes of G and M.
+template <int V>
+struct Vec;
+template <>
+struct Vec<1> { float v[1]; };
+template <>
+struct __align__(16) Vec<4> { float v[4]; };
+
+template <int V>
+__device__ __forceinline__ Vec<V> load_vec(const float* p) { return *reinterpret_cast<const Vec<V>*>(p); }
+
+__device__ __forceinline__ double block_sum(double acc) {
     __shared__ double sums[PREP_THREADS / 32];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
     if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = acc;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        double t = 0.0;
-        for (int w = 0; w < PREP_THREADS / 32; ++w) t += sums[w];
-        partial[blockIdx.x] = t;
-    }
+    double t = 0.0;
+#pragma unroll
+    for (int w = 0; w < PREP_THREADS / 32; ++w) t += sums[w];
+    return t;
 }
 
-// ---- pass 2: Y = U / (|U|_F + eps) -----------------------------------------------------------------------
-__global__ void __launch_bounds__(PREP_THREADS) prep_scale_kernel(Source S, const double* __restrict__ partial, int parts, float eps, float* __restrict__ y) {
-    __shared__ float inv_s;
-    if (threadIdx.x == 0) {
-        double t = 0.0;
-        for (int i = 0; i < parts; ++i) t += partial[i];
-        inv_s = isfinite(t) ? static_cast<float>(1.0 / (sqrt(t) + static_cast<double>(eps))) : __int_as_float(0x7fc00000);
-    }
-    __syncthreads();
-    const float inv = inv_s;
-    const int64_t total = S.rows * S.cols;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * PREP_THREADS + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * PREP_THREADS) {
-        const int64_t r = i / S.cols, c = i - r * S.cols;
-        float u = S.g[r * S.ldg + c];
-        if (S.momentum) {
-            const float m = S.momentum[r * S.ldm + c];
-            u = S.nesterov ? fmaf(S.mu, m, u) : m;
+template <int V, bool MOMENTUM>
+__global__ void __launch_bounds__(PREP_THREADS) prep_norm_kernel(Source S, double* __restrict__ partial) {
+    const uint32_t per_row = static_cast<uint32_t>(S.cols / V), total = static_cast<uint32_t>(S.rows) * per_row;
+    double acc = 0.0;
+    for (uint32_t i = blockIdx.x * PREP_THREADS + threadIdx.x; i < total; i += gridDim.x * PREP_THREADS) {
+        const uint32_t r = i / per_row, c = (i - r * per_row) * V;
+        Vec<V> u = load_vec<V>(S.g + r * S.ldg + c);
+        if (MOMENTUM) {
+            float* mp = S.momentum + r * S.ldm + c;
+            Vec<V> m = load_vec<V>(mp);
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                m.v[e] = fmaf(S.mu, m.v[e], u.v[e]);
+                u.v[e] = S.nesterov ? fmaf(S.mu, m.v[e], u.v[e]) : m.v[e];
+            }
+            *reinterpret_cast<Vec<V>*>(mp) = m;
         }
-        y[i] = u * inv;
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc = fma(static_cast<double>(u.v[e]), static_cast<double>(u.v[e]), acc);
     }
+    const double t = block_sum(acc);
+    if (threadIdx.x == 0) partial[blockIdx.x] = t;
 }
 
-__global__ void __launch_bounds__(PREP_THREADS) poly_kernel(float* __restrict__ a, const float* __restrict__ a2, int64_t n) {
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * PREP_THREADS + threadIdx.x;
-    if (i < n) a[i] = fmaf(kB, a[i], kC * a2[i]);
+// ---- pass 2: X0 as hi + lo, and the steps' coefficients --------------------------------------------------
+// With n = |U|_F and T = n + eps, X0 = U / T.  Where eps is not small beside n, X0 is small as a whole and
+// would sink in fp16's range; it is held as Y = X0 2^e instead, e >= 0 such that |Y|_F lies in (1/4, 1].  A step on Y is
+// Y <- f (a Y + (b 4^-e A_Y + c 16^-e A_Y A_Y) Y) with f = 1/4 and e <- e - 2 as long as e > 0 (the step multiplies by
+// less than 4), all exact powers of two.  coef[4 s ..] = {b 4^-e, c 16^-e, f, -} of step s; the last step's f undoes 2^e.
+struct Normaliser {
+    float p2, rest;  // Y = (U * p2) * rest * kScaleX
+    int e;
+};
+__device__ __forceinline__ Normaliser normaliser(double sumsq, float eps) {
+    Normaliser N;
+    if (!(sumsq < 1.7e308)) return Normaliser{__int_as_float(0x7fc00000), 1.0f, 0};  // a non-finite element: NaN everywhere
+    const double n = sqrt(sumsq), t = n + static_cast<double>(eps);
+    int en = 0, et = 0;
+    (void)frexp(n, &en);
+    const double mt = frexp(t, &et);
+    if (n == 0.0 || en < -126) en = n == 0.0 ? et : -126;  // (2^-en stays a normal number)
+    const int gap = et - en;
+    N.e = gap > 1 ? gap - 1 : 0;
+    N.p2 = static_cast<float>(ldexp(1.0, -en));
+    N.rest = static_cast<float>(gap >= 1 ? 0.5 / mt : 1.0 / mt);
+    return N;
 }
-__global__ void __launch_bounds__(PREP_THREADS) combine_kernel(float* __restrict__ x, const float* __restrict__ bx, int64_t n) {
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * PREP_THREADS + threadIdx.x;
-    if (i < n) x[i] = fmaf(kA, x[i], bx[i]);
+
+__device__ __forceinline__ void split_half(float x, __half& hi, __half& lo) {
+    hi = __float2half_rn(x);
+    lo = __float2half_rn(x - __half2float(hi));
+}
+
+// One matrix as hi and lo arrays: [outer, pitch] each, lo behind hi.
+struct Pair {
+    __half* hi;
+    int64_t pitch;
+    int64_t lo;  // elements from hi to lo
+};
+
+template <int V, bool MOMENTUM>
+__global__ void __launch_bounds__(PREP_THREADS) prep_split_kernel(Source S, const double* __restrict__ partial, int parts, float eps, int steps,
+                                                                  Pair X, float* __restrict__ coef) {
+    double acc = 0.0;
+    for (int i = threadIdx.x; i < parts; i += PREP_THREADS) acc += partial[i];
+    const Normaliser N = normaliser(block_sum(acc), eps);
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        int e = N.e;
+        for (int s = 0; s < steps; ++s) {
+            const int drop = e < 2 ? e : 2;
+            coef[4 * s] = ldexpf(kB, -2 * e);
+            coef[4 * s + 1] = ldexpf(kC, -4 * e);
+            coef[4 * s + 2] = s + 1 == steps ? ldexpf(1.0f, -e) : ldexpf(1.0f, -drop);
+            coef[4 * s + 3] = 0.0f;
+            e -= drop;
+        }
+    }
+    const uint32_t per_row = static_cast<uint32_t>(S.cols / V), total = static_cast<uint32_t>(S.rows) * per_row;
+    for (uint32_t i = blockIdx.x * PREP_THREADS + threadIdx.x; i < total; i += gridDim.x * PREP_THREADS) {
+        const uint32_t r = i / per_row, c = (i - r * per_row) * V;
+        Vec<V> u = load_vec<V>(S.g + r * S.ldg + c);
+        if (MOMENTUM) {
+            const Vec<V> m = load_vec<V>(S.momentum + r * S.ldm + c);
+#pragma unroll
+            for (int e = 0; e < V; ++e) u.v[e] = S.nesterov ? fmaf(S.mu, m.v[e], u.v[e]) : m.v[e];
+        }
+        __half hi[V], lo[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) split_half((u.v[e] * N.p2) * (N.rest * kScaleX), hi[e], lo[e]);
+        __half* dst = X.hi + r * X.pitch + c;
+        if (V == 4) {
+            *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(hi);
+            *reinterpret_cast<uint2*>(dst + X.lo) = *reinterpret_cast<const uint2*>(lo);
+        } else {
+            dst[0] = hi[0];
+            dst[X.lo] = lo[0];
+        }
+    }
 }
 
 // ---- where the result goes -------------------------------------------------------------------------------
@@ -87,33 +172,447 @@ struct Sink {
     int64_t ldo;
     int update;  // 0: out = o;  1: out = keep * out - step * o
     float keep, step;
+    int vec;     // 16-byte accesses are possible
 };
-__global__ void __launch_bounds__(PREP_THREADS) sink_kernel(Sink K, const float* __restrict__ x, int64_t rows, int64_t cols) {
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * PREP_THREADS + threadIdx.x;
-    if (i >= rows * cols) return;
-    float* o = K.out + (i / cols) * K.ldo + i % cols;
-    *o = K.update ? fmaf(-K.step, x[i], K.keep * *o) : x[i];
+__device__ __forceinline__ float sink_value(const Sink& K, float o, float old) { return K.update ? fmaf(-K.step, o, K.keep * old) : o; }
+
+// ---- the products ----------------------------------------------------------------------------------------
+enum { GRAM = 0, POLY = 1, APPLY = 2 };
+constexpr int BM = 128, BK = 64;
+constexpr int THREADS = 320;      // warp 0 loads, warp 1 multiplies, warps 2-9 take the accumulators
+constexpr int EPI_WARPS = 8;
+constexpr int STAGE_BYTES = 4 * BM * BK * 2;  // [A hi | lo][B hi | lo], 128 rows of each per CTA
+constexpr int STAGES = 3;
+constexpr int CHUNK_KB = 2;       // k-blocks summed in TMEM before they move to registers
+constexpr int OUT_PITCH = 33;
+constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_WARPS * 32 * OUT_PITCH * 4 + 1024;
+
+struct Params {
+    int m, n;                 // extents of the product's result
+    int tiles_m, tiles_n, units, num_kb;
+    Pair src;                 // POLY: A; APPLY: X before the step
+    Pair dst;                 // GRAM: A; POLY: B; APPLY: X after the step (unless last)
+    const float* coef;        // this step's {b, c, f}
+    int last;                 // APPLY: the result goes to the sink
+    Sink sink;
+};
+
+// Tile u of the launch.  Symmetric products count the upper triangle column by column.
+template <int MODE>
+__device__ __forceinline__ void unit_tile(int u, const Params& P, int& tm, int& tn) {
+    if (MODE != APPLY) {
+        int j = static_cast<int>((sqrtf(8.0f * static_cast<float>(u) + 1.0f) - 1.0f) * 0.5f);
+        while (j * (j + 1) / 2 > u) --j;
+        while ((j + 1) * (j + 2) / 2 <= u) ++j;
+        tn = j;
+        tm = u - j * (j + 1) / 2;
+        return;
+    }
+    // bands of 8 tile columns, row after row inside a band: the tiles in flight share rows of A and columns of B in L2
+    constexpr int BAND = 8;
+    const int band = u / (BAND * P.tiles_m), first = band * BAND;
+    const int width = P.tiles_n - first < BAND ? P.tiles_n - first : BAND;
+    const int r = u - band * (BAND * P.tiles_m);
+    tm = r / width;
+    tn = first + r % width;
+}
+
+// A 32 x 32 block of the result, lane = row (the layout tcgen05.ld delivers), on its way to memory.  Stores and
+// loads of row-major arrays go through `stage`, so that 8 lanes share a row's 32 elements; the transposed side of a
+// symmetric product has its 32 contiguous elements in the 32 lanes already.
+template <int MODE>
+__device__ __forceinline__ void emit_block(const Params& P, bool mirror, int row_base, int lane, int col0, float (&v)[32], uint32_t* stage,
+                                           const float (&cf)[3]) {
+    if (col0 >= P.n || row_base >= P.m) return;  // the whole warp
+    const int row = row_base + lane;
+    const int sub = lane >> 3, c4 = (lane & 7) * 4;
+    if (MODE != APPLY) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            const int col = col0 + i;
+            float x;
+            if (MODE == GRAM) {
+                x = v[i] * (1.0f / 32768.0f);
+            } else {
+                // A[row, col] = A[col, row]: the read whose 32 lanes are neighbours
+                float a = 0.0f;
+                if (col < P.n && row < P.m) {
+                    const __half* s = P.src.hi + col * P.src.pitch + row;
+                    a = __half2float(s[0]) + __half2float(s[P.src.lo]);
+                }
+                x = fmaf(cf[0] * 0.5f, a, cf[1] * (1.0f / 65536.0f) * v[i]);
+            }
+            __half hi, lo;
+            split_half(x, hi, lo);
+            if (mirror && col < P.n && row < P.m) {
+                __half* d = P.dst.hi + col * P.dst.pitch + row;
+                d[0] = hi;
+                d[P.dst.lo] = lo;
+            }
+            stage[lane * OUT_PITCH + i] = static_cast<uint32_t>(__half_as_ushort(hi)) | (static_cast<uint32_t>(__half_as_ushort(lo)) << 16);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) stage[lane * OUT_PITCH + i] = __float_as_uint(v[i]);
+    }
+    __syncwarp();
+    const int64_t col = col0 + c4;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int r = i * 4 + sub;
+        if (row_base + r >= P.m || col >= P.n) continue;
+        const uint32_t* s = stage + r * OUT_PITCH + c4;
+        uint32_t w[4] = {s[0], s[1], s[2], s[3]};
+        if (MODE == APPLY) {
+            const __half* xp = P.src.hi + (row_base + r) * P.src.pitch + col;  // (pitches are multiples of 8: four elements never leave the row)
+            __half h4[4], l4[4];
+            *reinterpret_cast<uint2*>(h4) = __ldcg(reinterpret_cast<const uint2*>(xp));
+            *reinterpret_cast<uint2*>(l4) = __ldcg(reinterpret_cast<const uint2*>(xp + P.src.lo));
+            float o[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                o[e] = cf[2] * fmaf(kA, __half2float(h4[e]) + __half2float(l4[e]), __uint_as_float(w[e]) * (1.0f / 16384.0f));
+            if (P.last) {
+                float* out = P.sink.out + (row_base + r) * P.sink.ldo + col;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] *= 1.0f / kScaleX;
+                if (P.sink.vec && col + 4 <= P.n) {
+                    float4 old = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (P.sink.update) old = *reinterpret_cast<const float4*>(out);
+                    *reinterpret_cast<float4*>(out) = make_float4(sink_value(P.sink, o[0], old.x), sink_value(P.sink, o[1], old.y), sink_value(P.sink, o[2], old.z),
+                                                                  sink_value(P.sink, o[3], old.w));
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (col + e < P.n) out[e] = sink_value(P.sink, o[e], P.sink.update ? out[e] : 0.0f);
+                }
+                continue;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                __half hi, lo;
+                split_half(o[e], hi, lo);
+                w[e] = static_cast<uint32_t>(__half_as_ushort(hi)) | (static_cast<uint32_t>(__half_as_ushort(lo)) << 16);
+            }
+        }
+        __half* d = P.dst.hi + (row_base + r) * P.dst.pitch + col;
+        *reinterpret_cast<uint2*>(d) = make_uint2(__byte_perm(w[0], w[1], 0x5410), __byte_perm(w[2], w[3], 0x5410));
+        *reinterpret_cast<uint2*>(d + P.dst.lo) = make_uint2(__byte_perm(w[0], w[1], 0x7632), __byte_perm(w[2], w[3], 0x7632));
+    }
+    __syncwarp();
+}
+
+// D = A B^T over k, persistent.  GROUP 2: a pair of CTAs per 256 x 256 tile, each with 128 rows of A and 128 columns
+// of B; GROUP 1: a CTA per 128 x 128 tile.  A stage is one box of hi and lo per operand (K-major), or two, one per 64
+// columns (MN-major).  Two accumulators: the next chunk is multiplied while the epilogue warps add the last one.
+template <int GROUP, int MODE, bool A_MN, bool B_MN>
+__global__ void __launch_bounds__(THREADS, 1) ns_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Params P) {
+    using namespace t5;
+    constexpr int BN = 128 * GROUP;
+    constexpr int TMEM_COLS = 2 * BN;
+    constexpr int BLOCKS = BN / 64;  // 32-column blocks per epilogue warp: two warps share a row quarter
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint64_t bars[2 * STAGES + 4];
+    __shared__ uint32_t tmem_slot;
+    __shared__ volatile int abort_flag;
+    const uint32_t rank = GROUP == 2 ? cluster_ctarank() : 0;
+    const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint32_t* out_stage = reinterpret_cast<uint32_t*>(smem_raw + (smem_base - smem_u32(smem_raw)) + STAGES * STAGE_BYTES);
+    const uint32_t bar0 = smem_u32(bars);
+    auto full_bar = [&](int s) { return bar0 + 8u * s; };
+    auto empty_bar = [&](int s) { return bar0 + 8u * (STAGES + s); };
+    auto tfull_bar = [&](int a) { return bar0 + 8u * (2 * STAGES + a); };
+    auto tempty_bar = [&](int a) { return bar0 + 8u * (2 * STAGES + 2 + a); };
+    const uint32_t peer_abort = GROUP == 2 ? map_to_cta(smem_u32(const_cast<int*>(&abort_flag)), rank ^ 1u) : 0u;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        abort_flag = 0;
+        for (int s = 0; s < STAGES; ++s) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
+        for (int a = 0; a < 2; ++a) { mbar_init(tfull_bar(a), 1); mbar_init(tempty_bar(a), EPI_WARPS * GROUP); }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        prefetch_tmap(&map_a);
+        prefetch_tmap(&map_b);
+    }
+    if (warp == 1) tmem_alloc<GROUP>(smem_u32(&tmem_slot), TMEM_COLS);
+    fence_before();
+    __syncthreads();
+    if (GROUP == 2) cluster_sync_all();  // the peer's barriers exist before anything is signalled across
+    fence_after();
+    const uint32_t tmem_base = tmem_slot;
+    const int first_unit = blockIdx.x / GROUP, unit_step = gridDim.x / GROUP;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int stage = 0;
+            uint32_t phase = 0, issued = 0;
+            bool ok = true;
+            for (int u = first_unit; u < P.units && ok; u += unit_step) {
+                int tm, tn;
+                unit_tile<MODE>(u, P, tm, tn);
+                const int m0 = (tm * GROUP + static_cast<int>(rank)) * BM, n0 = tn * BN + static_cast<int>(rank) * BM;
+                for (int kb = 0; kb < P.num_kb; ++kb) {
+                    if (!mbar_wait(empty_bar(stage), phase ^ 1u, &abort_flag, &g_ns_status, 0x100 | stage)) { ok = false; break; }
+                    if (rank == 0) mbar_expect_tx(full_bar(stage), GROUP * STAGE_BYTES);
+                    const uint32_t fb = GROUP == 2 ? map_to_cta(full_bar(stage), 0) : full_bar(stage);
+                    const uint32_t base = smem_base + stage * STAGE_BYTES;
+                    const int k0 = kb * BK;
+                    if (A_MN) {
+                        tma_load_3d<GROUP>(base, &map_a, fb, m0, k0, 0);
+                        tma_load_3d<GROUP>(base + STAGE_BYTES / 4, &map_a, fb, m0 + 64, k0, 0);
+                    } else {
+                        tma_load_3d<GROUP>(base, &map_a, fb, k0, m0, 0);
+                    }
+                    if (B_MN) {
+                        tma_load_3d<GROUP>(base + STAGE_BYTES / 2, &map_b, fb, n0, k0, 0);
+                        tma_load_3d<GROUP>(base + 3 * (STAGE_BYTES / 4), &map_b, fb, n0 + 64, k0, 0);
+                    } else {
+                        tma_load_3d<GROUP>(base + STAGE_BYTES / 2, &map_b, fb, k0, n0, 0);
+                    }
+                    ++issued;
+                    if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+                }
+            }
+            // Every stage that was filled has been released: no copy and no arrival is in flight any more.  After a wait
+            // that ran out this is bounded too, and the copies in flight get a couple of milliseconds to land.
+            const uint32_t pending = issued < static_cast<uint32_t>(STAGES) ? issued : STAGES;
+            if (issued < static_cast<uint32_t>(STAGES)) { stage = 0; phase = 1u; }  // (the ring never came round: from its start)
+            for (uint32_t i = 0; i < pending && ok; ++i) {
+                if (!mbar_wait(empty_bar(stage), phase ^ 1u, &abort_flag, &g_ns_status, 0x180 | stage)) ok = false;
+                if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+            }
+            if (!ok) {
+                if (GROUP == 2) st_cluster_u32(peer_abort, 1u);
+                for (int i = 0; i < 2048; ++i) __nanosleep(1000);
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            constexpr uint32_t idesc = make_idesc(BM * GROUP, BN, A_MN, B_MN);
+            // hi and lo of a K-major tile lie half an operand apart; of an MN-major one a quarter, inside each column group
+            constexpr uint32_t a_lo = A_MN ? STAGE_BYTES / 8 : STAGE_BYTES / 4, b_lo = B_MN ? STAGE_BYTES / 8 : STAGE_BYTES / 4;
+            constexpr uint32_t a_step = A_MN ? 2048u : 32u, b_step = B_MN ? 2048u : 32u;
+            constexpr uint32_t a_lbo = A_MN ? STAGE_BYTES / 4 : 0u, b_lbo = B_MN ? STAGE_BYTES / 4 : 0u;
+            int stage = 0, acc = 0;
+            uint32_t phase = 0, acc_phase = 0;
+            bool ok = true;
+            for (int u = first_unit; u < P.units && ok; u += unit_step) {
+                for (int c0 = 0; c0 < P.num_kb && ok; c0 += CHUNK_KB) {
+                    const int c1 = c0 + CHUNK_KB < P.num_kb ? c0 + CHUNK_KB : P.num_kb;
+                    if (!mbar_wait(tempty_bar(acc), acc_phase ^ 1u, &abort_flag, &g_ns_status, 0x200 | acc)) { ok = false; break; }
+                    fence_after();
+                    const uint32_t d = tmem_base + static_cast<uint32_t>(acc * BN);
+                    for (int kb = c0; kb < c1; ++kb) {
+                        if (!mbar_wait(full_bar(stage), phase, &abort_flag, &g_ns_status, 0x210 | stage)) { ok = false; break; }
+                        fence_after();
+                        const uint32_t a = smem_base + stage * STAGE_BYTES, b = a + STAGE_BYTES / 2;
+                        uint32_t more = kb == c0 ? 0u : 1u;
+#pragma unroll
+                        for (int ks = 0; ks < BK / 16; ++ks) {  // the small terms first, while the accumulator is small
+                            mma_f16<GROUP>(d, make_desc(a + a_lo + ks * a_step, a_lbo), make_desc(b + ks * b_step, b_lbo), idesc, more);
+                            mma_f16<GROUP>(d, make_desc(a + ks * a_step, a_lbo), make_desc(b + b_lo + ks * b_step, b_lbo), idesc, 1u);
+                            more = 1u;
+                        }
+#pragma unroll
+                        for (int ks = 0; ks < BK / 16; ++ks)
+                            mma_f16<GROUP>(d, make_desc(a + ks * a_step, a_lbo), make_desc(b + ks * b_step, b_lbo), idesc, 1u);
+                        commit<GROUP>(empty_bar(stage));
+                        if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+                    }
+                    if (!ok) break;
+                    commit<GROUP>(tfull_bar(acc));
+                    if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
+                }
+            }
+            if (!ok && GROUP == 2) st_cluster_u32(peer_abort, 1u);
+        }
+    } else {
+        const int quarter = warp & 3, side = (warp - 2) >> 2;  // rows 32 quarter.., columns BN/2 side..
+        const uint32_t te0 = GROUP == 2 ? map_to_cta(tempty_bar(0), 0) : tempty_bar(0), te1 = GROUP == 2 ? map_to_cta(tempty_bar(1), 0) : tempty_bar(1);
+        const float cf[3] = {__ldg(P.coef), __ldg(P.coef + 1), __ldg(P.coef + 2)};
+        uint32_t* stage = out_stage + (warp - 2) * 32 * OUT_PITCH;
+        int acc = 0;
+        uint32_t acc_phase = 0;
+        bool ok = true;
+        for (int u = first_unit; u < P.units && ok; u += unit_step) {
+            int tm, tn;
+            unit_tile<MODE>(u, P, tm, tn);
+            float sum[BLOCKS][32];
+#pragma unroll
+            for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+                for (int i = 0; i < 32; ++i) sum[b][i] = 0.0f;
+            for (int c0 = 0; c0 < P.num_kb; c0 += CHUNK_KB) {
+                if (!mbar_wait(tfull_bar(acc), acc_phase, &abort_flag, &g_ns_status, 0x300 | acc)) { ok = false; break; }
+                fence_after();
+                const uint32_t t = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * BN + side * (BN / 2));
+#pragma unroll
+                for (int b = 0; b < BLOCKS; ++b) {
+                    uint32_t r[32];
+                    tmem_ld32(t + b * 32, r);
+                    tmem_ld_wait();
+                    if (b == BLOCKS - 1) {  // read completely: the next but one chunk may go there
+                        fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_cluster(acc ? te1 : te0);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) sum[b][i] += __uint_as_float(r[i]);
+                }
+                if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
+            }
+            if (!ok) break;
+            const int row_base = (tm * GROUP + static_cast<int>(rank)) * BM + quarter * 32;
+#pragma unroll
+            for (int b = 0; b < BLOCKS; ++b)
+                emit_block<MODE>(P, MODE != APPLY && tm != tn, row_base, lane, tn * BN + side * (BN / 2) + b * 32, sum[b], stage, cf);
+        }
+        if (!ok && GROUP == 2 && lane == 0) st_cluster_u32(peer_abort, 1u);
+    }
+
+    fence_before();
+    __syncthreads();
+    if (GROUP == 2) cluster_sync_all();  // neither CTA leaves (or frees TMEM) while the other may still signal it
+    if (warp == 1) {
+        fence_after();
+        tmem_dealloc<GROUP>(tmem_base, TMEM_COLS);
+    }
+}
+
+// ---- host side -------------------------------------------------------------------------------------------
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                                   CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+ctk_status get_encoder(EncodeTiledFn* out) {
+    static std::mutex mu;
+    static EncodeTiledFn encode = nullptr;
+    std::lock_guard<std::mutex> lock(mu);
+    if (!encode) {
+        void* fn = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        CTK_CUDA(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q));
+        if (!fn || q != cudaDriverEntryPointSuccess) return fail(CTK_ERR_CUDA, "cuTensorMapEncodeTiled not available from the driver");
+        encode = reinterpret_cast<EncodeTiledFn>(fn);
+    }
+    *out = encode;
+    return CTK_OK;
+}
+
+// {inner, outer, hi | lo} with box {64, box_outer, 2}: one copy brings hi and lo.  Elements past an extent read as zero.
+ctk_status make_map(CUtensorMap* map, const Pair& p, int64_t inner, int64_t outer, int box_outer) {
+    EncodeTiledFn enc;
+    ctk_status st = get_encoder(&enc);
+    if (st) return st;
+    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer), 2u};
+    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(p.pitch) * 2, static_cast<cuuint64_t>(p.lo) * 2};
+    const cuuint32_t box[3] = {64u, static_cast<cuuint32_t>(box_outer), 2u}, estr[3] = {1u, 1u, 1u};
+    const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, p.hi, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(CTK_ERR_CUDA, "cuTensorMapEncodeTiled failed with code " + std::to_string(static_cast<int>(r)));
+    return CTK_OK;
+}
+
+template <int GROUP, int MODE, bool A_MN, bool B_MN>
+ctk_status launch_product(const CUtensorMap& a, const CUtensorMap& b, Params P, cudaStream_t st) {
+    auto kernel = ns_product_kernel<GROUP, MODE, A_MN, B_MN>;
+    static int resident[64] = {0};  // tiles in flight on a device
+    int dev = 0;
+    CTK_CUDA(cudaGetDevice(&dev));
+    CTK_REQUIRE(dev >= 0 && dev < 64, "device ordinal out of range");
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = GROUP;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = SMEM_BYTES;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (!resident[dev]) {
+        CTK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES));
+        cfg.gridDim = dim3(static_cast<unsigned>(GROUP * ctk::sm_count()));
+        int n = 0;
+        CTK_CUDA(cudaOccupancyMaxActiveClusters(&n, kernel, &cfg));
+        CTK_REQUIRE(n > 0, "the device cannot hold the orthogonalisation kernel");
+        resident[dev] = n;
+    }
+    constexpr int T = BM * GROUP;
+    P.tiles_m = (P.m + T - 1) / T;
+    P.tiles_n = (P.n + T - 1) / T;
+    P.units = MODE == APPLY ? P.tiles_m * P.tiles_n : P.tiles_n * (P.tiles_n + 1) / 2;
+    cfg.gridDim = dim3(static_cast<unsigned>(GROUP * (P.units < resident[dev] ? P.units : resident[dev])));
+    CTK_CUDA(cudaLaunchKernelEx(&cfg, kernel, a, b, P));
+    CTK_LAUNCH_CHECK("ns_product_kernel");
+    return CTK_OK;
 }
 
 struct Layout {
-    size_t partial, x, x2, a, a2, total;
+    size_t partial, coef, x[2], a, b, total;
+    int64_t pitch_x, pitch_d;
 };
+constexpr int MAX_PARTS = 1024, MAX_STEPS = 64;
 Layout layout_for(int64_t rows, int64_t cols) {
-    const size_t d = static_cast<size_t>(rows < cols ? rows : cols), n = static_cast<size_t>(rows) * static_cast<size_t>(cols);
-    auto up = [](size_t b) { return (b + 255) & ~size_t(255); };
     Layout L;
+    const int64_t d = rows < cols ? rows : cols;
+    L.pitch_x = (cols + 7) / 8 * 8;
+    L.pitch_d = (d + 7) / 8 * 8;
     size_t at = 0;
-    auto take = [&](size_t b) { const size_t p = at; at += up(b); return p; };
-    L.partial = take(4096 * sizeof(double));
-    L.x = take(n * 4);
-    L.x2 = take(n * 4);
-    L.a = take(d * d * 4);
-    L.a2 = take(d * d * 4);
+    auto take = [&](size_t b) { const size_t p = at; at += (b + 255) & ~size_t(255); return p; };
+    L.partial = take(MAX_PARTS * sizeof(double));
+    L.coef = take(MAX_STEPS * 4 * sizeof(float));
+    L.x[0] = take(static_cast<size_t>(rows) * L.pitch_x * 4);
+    L.x[1] = take(static_cast<size_t>(rows) * L.pitch_x * 4);
+    L.a = take(static_cast<size_t>(d) * L.pitch_d * 4);
+    L.b = take(static_cast<size_t>(d) * L.pitch_d * 4);
     L.total = at;
     return L;
 }
 
-ctk_status newton_schulz(const Source& S, const Sink& K, int steps, float eps, void* workspace, void* stream) {
+template <int GROUP>
+ctk_status run_steps(const Layout& L, char* ws, int64_t rows, int64_t cols, Sink K, int steps, cudaStream_t st) {
+    const bool tall = rows > cols;
+    const int64_t d = tall ? cols : rows;
+    Pair X[2], A, B;
+    for (int i = 0; i < 2; ++i) X[i] = Pair{reinterpret_cast<__half*>(ws + L.x[i]), L.pitch_x, rows * L.pitch_x};
+    A = Pair{reinterpret_cast<__half*>(ws + L.a), L.pitch_d, d * L.pitch_d};
+    B = Pair{reinterpret_cast<__half*>(ws + L.b), L.pitch_d, d * L.pitch_d};
+    CUtensorMap mx_k[2], mx_mn[2], ma, mb;
+    ctk_status rc = CTK_OK;
+    for (int i = 0; i < 2 && !rc; ++i) {
+        rc = make_map(&mx_k[i], X[i], cols, rows, 128);
+        if (!rc) rc = make_map(&mx_mn[i], X[i], cols, rows, 64);
+    }
+    if (!rc) rc = make_map(&ma, A, d, d, 128);
+    if (!rc) rc = make_map(&mb, B, d, d, 128);
+    const float* coef = reinterpret_cast<const float*>(ws + L.coef);
+    auto blocks = [](int64_t k) { return static_cast<int>((k + BK - 1) / BK); };
+    for (int s = 0; s < steps && !rc; ++s) {
+        const int at = s & 1;
+        Params P = {};
+        P.coef = coef + 4 * s;
+        P.sink = K;
+        P.m = P.n = static_cast<int>(d);
+        P.num_kb = blocks(tall ? rows : cols);
+        P.dst = A;
+        rc = tall ? launch_product<GROUP, GRAM, true, true>(mx_mn[at], mx_mn[at], P, st) : launch_product<GROUP, GRAM, false, false>(mx_k[at], mx_k[at], P, st);
+        if (rc) return rc;
+        P.num_kb = blocks(d);
+        P.src = A;
+        P.dst = B;
+        rc = launch_product<GROUP, POLY, false, false>(ma, ma, P, st);
+        if (rc) return rc;
+        P.m = static_cast<int>(rows);
+        P.n = static_cast<int>(cols);
+        P.src = X[at];
+        P.dst = X[at ^ 1];
+        P.last = s + 1 == steps;
+        rc = tall ? launch_product<GROUP, APPLY, false, false>(mx_k[at], mb, P, st) : launch_product<GROUP, APPLY, false, true>(mb, mx_mn[at], P, st);
+    }
+    return rc;
+}
+
+ctk_status newton_schulz(const Source& S, Sink K, int steps, float eps, void* workspace, void* stream) {
     const Layout L = layout_for(S.rows, S.cols);
     StreamScratch scratch;
     if (!workspace) {
@@ -123,34 +622,25 @@ ctk_status newton_schulz(const Source& S, const Sink& K, int steps, float eps, v
     }
     char* ws = static_cast<char*>(workspace);
     double* partial = reinterpret_cast<double*>(ws + L.partial);
-    float *x = reinterpret_cast<float*>(ws + L.x), *x2 = reinterpret_cast<float*>(ws + L.x2);
-    float *a = reinterpret_cast<float*>(ws + L.a), *a2 = reinterpret_cast<float*>(ws + L.a2);
+    float* coef = reinterpret_cast<float*>(ws + L.coef);
     cudaStream_t st = as_stream(stream);
-    const int64_t rows = S.rows, cols = S.cols, n = rows * cols;
-    const bool tall = rows > cols;
-    const int64_t d = tall ? cols : rows;
-    const int grid = ctk_stream_grid(n, PREP_THREADS, 4);
-    prep_norm_kernel<<<grid, PREP_THREADS, 0, st>>>(S, partial);
-    CTK_LAUNCH_CHECK("orthogonalize: norm");
-    prep_scale_kernel<<<grid, PREP_THREADS, 0, st>>>(S, partial, grid, eps, x);
-    CTK_LAUNCH_CHECK("orthogonalize: scale");
-    auto blocks = [](int64_t c) { return static_cast<unsigned>((c + PREP_THREADS - 1) / PREP_THREADS); };
-    for (int s = 0; s < steps; ++s) {
-        ctk_status rc = tall ? ctk_matmul_f32(x, x, a, d, d, rows, 1, cols, cols, 1, CTK_MATMUL_FP32_SIMT, nullptr, stream)
-                             : ctk_matmul_f32(x, x, a, d, d, cols, cols, 1, 1, cols, CTK_MATMUL_FP32_SIMT, nullptr, stream);
-        if (!rc) rc = ctk_matmul_f32(a, a, a2, d, d, d, d, 1, d, 1, CTK_MATMUL_FP32_SIMT, nullptr, stream);
-        if (rc) return rc;
-        poly_kernel<<<blocks(d * d), PREP_THREADS, 0, st>>>(a, a2, d * d);
-        CTK_LAUNCH_CHECK("orthogonalize: polynomial");
-        rc = tall ? ctk_matmul_f32(x, a, x2, rows, cols, cols, cols, 1, cols, 1, CTK_MATMUL_FP32_SIMT, nullptr, stream)
-                  : ctk_matmul_f32(a, x, x2, rows, cols, rows, rows, 1, cols, 1, CTK_MATMUL_FP32_SIMT, nullptr, stream);
-        if (rc) return rc;
-        combine_kernel<<<blocks(n), PREP_THREADS, 0, st>>>(x, x2, n);
-        CTK_LAUNCH_CHECK("orthogonalize: combine");
-    }
-    sink_kernel<<<blocks(n), PREP_THREADS, 0, st>>>(K, x, rows, cols);
-    CTK_LAUNCH_CHECK("orthogonalize: result");
-    return CTK_OK;
+    const bool vec = S.cols % 4 == 0 && S.ldg % 4 == 0 && aligned_to(S.g, 16) && (!S.momentum || (S.ldm % 4 == 0 && aligned_to(S.momentum, 16)));
+    K.vec = K.ldo % 4 == 0 && aligned_to(K.out, 16);
+    int grid = ctk_stream_grid(S.rows * S.cols / (vec ? 4 : 1), PREP_THREADS, 6);
+    if (grid > MAX_PARTS) grid = MAX_PARTS;
+    const Pair X0{reinterpret_cast<__half*>(ws + L.x[0]), L.pitch_x, S.rows * L.pitch_x};
+    auto prep = [&](auto norm, auto split) -> ctk_status {
+        norm<<<grid, PREP_THREADS, 0, st>>>(S, partial);
+        CTK_LAUNCH_CHECK("orthogonalize: norm");
+        split<<<grid, PREP_THREADS, 0, st>>>(S, partial, grid, eps, steps, X0, coef);
+        CTK_LAUNCH_CHECK("orthogonalize: split");
+        return CTK_OK;
+    };
+    ctk_status rc = S.momentum ? (vec ? prep(prep_norm_kernel<4, true>, prep_split_kernel<4, true>) : prep(prep_norm_kernel<1, true>, prep_split_kernel<1, true>))
+                               : (vec ? prep(prep_norm_kernel<4, false>, prep_split_kernel<4, false>) : prep(prep_norm_kernel<1, false>, prep_split_kernel<1, false>));
+    if (rc) return rc;
+    const int64_t d = S.rows < S.cols ? S.rows : S.cols;
+    return d > 1024 ? run_steps<2>(L, ws, S.rows, S.cols, K, steps, st) : run_steps<1>(L, ws, S.rows, S.cols, K, steps, st);
 }
 
 ctk_status check_common(const char* who, int64_t rows, int64_t cols, int steps, float eps, const void* workspace) {
@@ -184,7 +674,7 @@ ctk_status ctk_orthogonalize_f32(const float* g, int64_t ldg, float* out, int64_
     CTK_REQUIRE(aligned_to(g, 4) && aligned_to(out, 4), "ctk_orthogonalize_f32: misaligned pointer");
     CTK_REQUIRE((g == out && ldg == ldo) || !spans_overlap(g, rows, cols, ldg, out, rows, cols, ldo), "ctk_orthogonalize_f32: out overlaps g (only in place is allowed)");
     const Source S{g, ldg, nullptr, 0, 0.0f, 0, rows, cols};
-    const Sink K{out, ldo, 0, 0.0f, 0.0f};
+    const Sink K{out, ldo, 0, 0.0f, 0.0f, 0};
     return newton_schulz(S, K, steps, eps, workspace, stream);
 }
 
@@ -201,14 +691,14 @@ ctk_status ctk_muon_update_f32(float* p, int64_t ldp, const float* g, int64_t ld
                     !spans_overlap(g, rows, cols, ldg, momentum, rows, cols, ldm),
                 "ctk_muon_update_f32: p, g and momentum must not overlap");
     const Source S{g, ldg, momentum, ldm, mu, nesterov, rows, cols};
-    const Sink K{p, ldp, 1, 1.0f - lr * weight_decay, lr * scale};
+    const Sink K{p, ldp, 1, 1.0f - lr * weight_decay, lr * scale, 0};
     return newton_schulz(S, K, steps, eps, workspace, stream);
 }
 
 ctk_status ctk_orthogonalize_status(int* status) {
     CTK_REQUIRE(status, "ctk_orthogonalize_status: null pointer");
     CTK_CUDA(cudaDeviceSynchronize());
-    *status = 0;
+    CTK_CUDA(cudaMemcpyFromSymbol(status, g_ns_status, sizeof(int)));
     return CTK_OK;
 }
 
