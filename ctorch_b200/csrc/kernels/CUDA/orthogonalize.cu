@@ -12,7 +12,7 @@
 // obstacle here: the singular values of X never pass 1.21 (the step's polynomial maps [0, 1.21] into itself), so
 // |X| <= 1.21, |A| <= 1.46 and |B| <= 2.81 element by element, and a fixed power of two puts them high in fp16's range
 // (2^15, 2^15, 2^14); elements 2^-24 below the largest keep 11 bits or more between hi and lo.
-// The tensor core truncates as it adds into its fp32 accumulator, so an accumulator holds CHUNK_KB * 64 terms
+// The tensor core truncates as it adds into its fp32 accumulator, so an accumulator holds 64 or 256 terms
 // at a time; the epilogue warps add those up in registers with rounding.
 #include <math.h>
 
@@ -183,7 +183,11 @@ constexpr int THREADS = 320;      // warp 0 loads, warp 1 multiplies, warps 2-9 
 constexpr int EPI_WARPS = 8;
 constexpr int STAGE_BYTES = 4 * BM * BK * 2;  // [A hi | lo][B hi | lo], 128 rows of each per CTA
 constexpr int STAGES = 3;
-constexpr int CHUNK_KB = 2;       // k-blocks summed in TMEM before they move to registers
+// k-blocks of 64 terms summed in TMEM before they move to registers.  Relative error of NS(G) against 64 bits at 784 x 128
+// with 1 / 2 / 4 / 8 blocks: 1.8 / 3.1 / 3.4 / 4.0e-6, at 4096 x 4096 0.7 / 0.9 / 1.6 / 3.0e-6 (fp32 library products: 1.4 and
+// 3.8e-6).  A drain of the 128 x 256 accumulator costs the tensor pipe about 0.6 us (4096 x 4096 APPLY: 350 / 335 / 315 us
+// with 2 / 4 / 8 blocks, 293 without drains), so large products take 4 and small ones, which are not bound by the pipe, 1.
+__host__ __device__ constexpr int chunk_kb(int group) { return group == 2 ? 4 : 1; }
 constexpr int OUT_PITCH = 33;
 constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_WARPS * 32 * OUT_PITCH * 4 + 1024;
 
@@ -217,89 +221,97 @@ __device__ __forceinline__ void unit_tile(int u, const Params& P, int& tm, int& 
     tn = first + r % width;
 }
 
-// A 32 x 32 block of the result, lane = row (the layout tcgen05.ld delivers), on its way to memory.  Stores and
-// loads of row-major arrays go through `stage`, so that 8 lanes share a row's 32 elements; the transposed side of a
-// symmetric product has its 32 contiguous elements in the 32 lanes already.
+// A 32 x 32 block of the result, lane = row (the layout tcgen05.ld delivers), on its way to memory.  It goes through
+// `stage`, so that 8 lanes share a row's 32 elements and every load and store is 64 contiguous bytes or more; the other
+// triangle of a symmetric product is read back transposed, two rows to a lane, hi in the lower 16 lanes and lo in the
+// upper.  (POLY with its A read and its mirror written element by element from the accumulator's own layout: 275 us at
+// 4096 x 4096, this way LATER us.)
+__device__ __forceinline__ uint32_t pack_hi_lo(float x) {
+    __half hi, lo;
+    split_half(x, hi, lo);
+    return static_cast<uint32_t>(__half_as_ushort(hi)) | (static_cast<uint32_t>(__half_as_ushort(lo)) << 16);
+}
 template <int MODE>
-__device__ __forceinline__ void emit_block(const Params& P, bool mirror, int row_base, int lane, int col0, float (&v)[32], uint32_t* stage,
+__device__ __forceinline__ void emit_block(const Params& P, bool mirror, int row_base, int lane, int col0, const float (&v)[32], uint32_t* stage,
                                            const float (&cf)[3]) {
     if (col0 >= P.n || row_base >= P.m) return;  // the whole warp
-    const int row = row_base + lane;
     const int sub = lane >> 3, c4 = (lane & 7) * 4;
-    if (MODE != APPLY) {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            const int col = col0 + i;
-            float x;
-            if (MODE == GRAM) {
-                x = v[i] * (1.0f / 32768.0f);
-            } else {
-                // A[row, col] = A[col, row]: the read whose 32 lanes are neighbours
-                float a = 0.0f;
-                if (col < P.n && row < P.m) {
-                    const __half* s = P.src.hi + col * P.src.pitch + row;
-                    a = __half2float(s[0]) + __half2float(s[P.src.lo]);
-                }
-                x = fmaf(cf[0] * 0.5f, a, cf[1] * (1.0f / 65536.0f) * v[i]);
-            }
-            __half hi, lo;
-            split_half(x, hi, lo);
-            if (mirror && col < P.n && row < P.m) {
-                __half* d = P.dst.hi + col * P.dst.pitch + row;
-                d[0] = hi;
-                d[P.dst.lo] = lo;
-            }
-            stage[lane * OUT_PITCH + i] = static_cast<uint32_t>(__half_as_ushort(hi)) | (static_cast<uint32_t>(__half_as_ushort(lo)) << 16);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) stage[lane * OUT_PITCH + i] = __float_as_uint(v[i]);
-    }
-    __syncwarp();
     const int64_t col = col0 + c4;
+    uint2 h4[8], l4[8];
+    if (MODE != GRAM) {  // all of the block's reads in flight before anything waits
+        const __half* xp = P.src.hi + (row_base + sub) * P.src.pitch + col;  // (pitches are multiples of 8: four elements never leave the row)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            h4[i] = l4[i] = make_uint2(0u, 0u);
+            if (row_base + i * 4 + sub < P.m && col < P.n) {
+                h4[i] = __ldcg(reinterpret_cast<const uint2*>(xp + i * 4 * P.src.pitch));
+                l4[i] = __ldcg(reinterpret_cast<const uint2*>(xp + i * 4 * P.src.pitch + P.src.lo));
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 32; ++i) stage[lane * OUT_PITCH + i] = __float_as_uint(v[i]);
+    __syncwarp();
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const int r = i * 4 + sub;
-        if (row_base + r >= P.m || col >= P.n) continue;
-        const uint32_t* s = stage + r * OUT_PITCH + c4;
-        uint32_t w[4] = {s[0], s[1], s[2], s[3]};
-        if (MODE == APPLY) {
-            const __half* xp = P.src.hi + (row_base + r) * P.src.pitch + col;  // (pitches are multiples of 8: four elements never leave the row)
-            __half h4[4], l4[4];
-            *reinterpret_cast<uint2*>(h4) = __ldcg(reinterpret_cast<const uint2*>(xp));
-            *reinterpret_cast<uint2*>(l4) = __ldcg(reinterpret_cast<const uint2*>(xp + P.src.lo));
-            float o[4];
+        uint32_t* s = stage + r * OUT_PITCH + c4;
+        const __half2 h0 = *reinterpret_cast<const __half2*>(&h4[i].x), h1 = *reinterpret_cast<const __half2*>(&h4[i].y);
+        const __half2 l0 = *reinterpret_cast<const __half2*>(&l4[i].x), l1 = *reinterpret_cast<const __half2*>(&l4[i].y);
+        const float src[4] = {__low2float(h0) + __low2float(l0), __high2float(h0) + __high2float(l0), __low2float(h1) + __low2float(l1),
+                              __high2float(h1) + __high2float(l1)};
+        float o[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                o[e] = cf[2] * fmaf(kA, __half2float(h4[e]) + __half2float(l4[e]), __uint_as_float(w[e]) * (1.0f / 16384.0f));
-            if (P.last) {
-                float* out = P.sink.out + (row_base + r) * P.sink.ldo + col;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[e] *= 1.0f / kScaleX;
-                if (P.sink.vec && col + 4 <= P.n) {
-                    float4 old = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (P.sink.update) old = *reinterpret_cast<const float4*>(out);
-                    *reinterpret_cast<float4*>(out) = make_float4(sink_value(P.sink, o[0], old.x), sink_value(P.sink, o[1], old.y), sink_value(P.sink, o[2], old.z),
-                                                                  sink_value(P.sink, o[3], old.w));
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (col + e < P.n) out[e] = sink_value(P.sink, o[e], P.sink.update ? out[e] : 0.0f);
-                }
-                continue;
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                __half hi, lo;
-                split_half(o[e], hi, lo);
-                w[e] = static_cast<uint32_t>(__half_as_ushort(hi)) | (static_cast<uint32_t>(__half_as_ushort(lo)) << 16);
-            }
+        for (int e = 0; e < 4; ++e) {
+            const float d = __uint_as_float(s[e]);
+            if (MODE == GRAM) o[e] = d * (1.0f / 32768.0f);
+            if (MODE == POLY) o[e] = fmaf(cf[0] * 0.5f, src[e], cf[1] * (1.0f / 65536.0f) * d);
+            if (MODE == APPLY) o[e] = cf[2] * fmaf(kA, src[e], d * (1.0f / 16384.0f));
         }
-        __half* d = P.dst.hi + (row_base + r) * P.dst.pitch + col;
-        *reinterpret_cast<uint2*>(d) = make_uint2(__byte_perm(w[0], w[1], 0x5410), __byte_perm(w[2], w[3], 0x5410));
-        *reinterpret_cast<uint2*>(d + P.dst.lo) = make_uint2(__byte_perm(w[0], w[1], 0x7632), __byte_perm(w[2], w[3], 0x7632));
+        const bool inside = row_base + r < P.m && col < P.n;
+        if (MODE == APPLY && P.last) {
+            if (!inside) continue;
+            float* out = P.sink.out + (row_base + r) * P.sink.ldo + col;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] *= 1.0f / kScaleX;
+            if (P.sink.vec && col + 4 <= P.n) {
+                float4 old = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (P.sink.update) old = *reinterpret_cast<const float4*>(out);
+                *reinterpret_cast<float4*>(out) = make_float4(sink_value(P.sink, o[0], old.x), sink_value(P.sink, o[1], old.y), sink_value(P.sink, o[2], old.z),
+                                                              sink_value(P.sink, o[3], old.w));
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (col + e < P.n) out[e] = sink_value(P.sink, o[e], P.sink.update ? out[e] : 0.0f);
+            }
+            continue;
+        }
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = pack_hi_lo(o[e]);
+        if (inside) {
+            __half* d = P.dst.hi + (row_base + r) * P.dst.pitch + col;
+            *reinterpret_cast<uint2*>(d) = make_uint2(__byte_perm(w[0], w[1], 0x5410), __byte_perm(w[2], w[3], 0x5410));
+            *reinterpret_cast<uint2*>(d + P.dst.lo) = make_uint2(__byte_perm(w[0], w[1], 0x7632), __byte_perm(w[2], w[3], 0x7632));
+        }
+        if (MODE != APPLY && mirror) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[e] = w[e];
+        }
     }
     __syncwarp();
+    if (MODE != APPLY && mirror) {
+        const int pair = (lane & 15) * 2;
+        __half* d = P.dst.hi + row_base + pair + (lane < 16 ? 0 : P.dst.lo);
+        if (row_base + pair < P.m) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                const uint32_t w = __byte_perm(stage[pair * OUT_PITCH + i], stage[(pair + 1) * OUT_PITCH + i], lane < 16 ? 0x5410 : 0x7632);
+                if (col0 + i < P.n) *reinterpret_cast<uint32_t*>(d + (col0 + i) * P.dst.pitch) = w;
+            }
+        }
+        __syncwarp();
+    }
 }
 
 // D = A B^T over k, persistent.  GROUP 2: a pair of CTAs per 256 x 256 tile, each with 128 rows of A and 128 columns
@@ -309,6 +321,7 @@ template <int GROUP, int MODE, bool A_MN, bool B_MN>
 __global__ void __launch_bounds__(THREADS, 1) ns_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Params P) {
     using namespace t5;
     constexpr int BN = 128 * GROUP;
+    constexpr int CHUNK_KB = chunk_kb(GROUP);
     constexpr int TMEM_COLS = 2 * BN;
     constexpr int BLOCKS = BN / 64;  // 32-column blocks per epilogue warp: two warps share a row quarter
     extern __shared__ uint8_t smem_raw[];
