@@ -119,6 +119,15 @@ __device__ __forceinline__ void split_half(float x, __half& hi, __half& lo) {
     lo = __float2half_rn(x - __half2float(hi));
 }
 
+// Two elements at a time: {hi0, hi1} and {lo0, lo1} as the conversion instruction packs them.
+__device__ __forceinline__ void split2(float x0, float x1, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(x0, x1);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(x0 - f.x, x1 - f.y);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+
 // One matrix as hi and lo arrays: [outer, pitch] each, lo behind hi.
 struct Pair {
     __half* hi;
@@ -225,12 +234,7 @@ __device__ __forceinline__ void unit_tile(int u, const Params& P, int& tm, int& 
 // `stage`, so that 8 lanes share a row's 32 elements and every load and store is 64 contiguous bytes or more; the other
 // triangle of a symmetric product is read back transposed, two rows to a lane, hi in the lower 16 lanes and lo in the
 // upper.  (POLY with its A read and its mirror written element by element from the accumulator's own layout: 275 us at
-// 4096 x 4096, this way LATER us.)
-__device__ __forceinline__ uint32_t pack_hi_lo(float x) {
-    __half hi, lo;
-    split_half(x, hi, lo);
-    return static_cast<uint32_t>(__half_as_ushort(hi)) | (static_cast<uint32_t>(__half_as_ushort(lo)) << 16);
-}
+// 4096 x 4096, this way 176 us.)
 template <int MODE>
 __device__ __forceinline__ void emit_block(const Params& P, bool mirror, int row_base, int lane, int col0, const float (&v)[32], uint32_t* stage,
                                            const float (&cf)[3]) {
@@ -286,17 +290,19 @@ __device__ __forceinline__ void emit_block(const Params& P, bool mirror, int row
             }
             continue;
         }
-        uint32_t w[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = pack_hi_lo(o[e]);
+        uint2 hi, lo;
+        split2(o[0], o[1], hi.x, lo.x);
+        split2(o[2], o[3], hi.y, lo.y);
         if (inside) {
             __half* d = P.dst.hi + (row_base + r) * P.dst.pitch + col;
-            *reinterpret_cast<uint2*>(d) = make_uint2(__byte_perm(w[0], w[1], 0x5410), __byte_perm(w[2], w[3], 0x5410));
-            *reinterpret_cast<uint2*>(d + P.dst.lo) = make_uint2(__byte_perm(w[0], w[1], 0x7632), __byte_perm(w[2], w[3], 0x7632));
+            *reinterpret_cast<uint2*>(d) = hi;
+            *reinterpret_cast<uint2*>(d + P.dst.lo) = lo;
         }
-        if (MODE != APPLY && mirror) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[e] = w[e];
+        if (MODE != APPLY && mirror) {  // {hi, lo} of one element in one word
+            s[0] = __byte_perm(hi.x, lo.x, 0x5410);
+            s[1] = __byte_perm(hi.x, lo.x, 0x7632);
+            s[2] = __byte_perm(hi.y, lo.y, 0x5410);
+            s[3] = __byte_perm(hi.y, lo.y, 0x7632);
         }
     }
     __syncwarp();
@@ -492,6 +498,363 @@ __global__ void __launch_bounds__(THREADS, 1) ns_product_kernel(const __grid_con
     }
 }
 
+// ---- small matrices: every step in one launch ------------------------------------------------------------
+// d <= 128 and L <= 2048: a cluster of C CTAs, C = 1, 2, 4, 8 or 16, holds X in shared memory, each CTA a slab of at most 128
+// of the L side, from the first read of G to the last write.  A slab row is one index of the short side, 128 bytes of 64
+// neighbours along L, 16-byte chunks XORed with row % 8 -- read along L it is the K-major operand of X X^T, read down the
+// rows the MN-major operand of B X, so one copy serves both (a tall G is transposed on its way in and out).  A step:
+//   X X^T of the slab -> global, fp32 | cluster barrier | each CTA adds d / C columns over all CTAs, in rank order, and
+//   writes A's hi and lo as shared memory has them -> global | cluster barrier | one bulk copy per array brings A back |
+//   A A, B and B X in each CTA for itself.
+// Everything a product reads is there before it starts, so the small terms go first; an accumulator takes half of K.
+// What bounds it is latency: at 784 x 128 a step is LATER us.  (The exchange through the other CTAs' shared memory
+// instead of L2 took 18000 of 37000 clocks a step there: 64 KB in and out of every CTA at 7 bytes a clock.)
+constexpr int CL_THREADS = 512;                    // 4 warps per quarter of the accumulator's rows, 32 columns each
+constexpr int CL_SIDE = 128;                       // largest d, widest slab
+constexpr int CL_GROUP = CL_SIDE * 128;            // bytes of a 64-wide column group of a matrix of 128 rows
+constexpr int CL_MATRIX = 4 * CL_GROUP;            // hi: 2 groups, lo: 2 groups
+constexpr int CL_PITCH = 132;                      // floats per row of the fp32 buffer
+constexpr int CL_MAX = 16;                         // CTAs of a cluster
+constexpr int CL_SMEM = 2 * CL_MATRIX + CL_SIDE * CL_PITCH * 4 + 1024;
+constexpr int CL_PARTIAL = CL_SIDE * CL_SIDE * 4;  // bytes of one CTA's X X^T
+constexpr size_t cl_workspace(int ctas) { return ctas > 1 ? static_cast<size_t>(ctas) * CL_PARTIAL + CL_MATRIX : 0; }
+
+// Byte offset of the 16-byte chunk with elements [8 c, 8 c + 8) of row r.
+__device__ __forceinline__ uint32_t cl_chunk(int r, int c) { return static_cast<uint32_t>((c >> 3) * CL_GROUP + r * 128 + (((c & 7) ^ (r & 7)) << 4)); }
+
+__device__ __forceinline__ void split8(const float (&x)[8], uint4& hi, uint4& lo) {
+    split2(x[0], x[1], hi.x, lo.x);
+    split2(x[2], x[3], hi.y, lo.y);
+    split2(x[4], x[5], hi.z, lo.z);
+    split2(x[6], x[7], hi.w, lo.w);
+}
+__device__ __forceinline__ void join8(const uint4& hi, const uint4& lo, float (&x)[8]) {
+    const uint32_t h[4] = {hi.x, hi.y, hi.z, hi.w}, l[4] = {lo.x, lo.y, lo.z, lo.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&h[e])), b = __half22float2(*reinterpret_cast<const __half2*>(&l[e]));
+        x[2 * e] = a.x + b.x;
+        x[2 * e + 1] = a.y + b.y;
+    }
+}
+
+struct ClusterArgs {
+    Source S;
+    Sink K;
+    int d, length, slab;  // short side, long side, columns of the long side per CTA (a multiple of 16)
+    int tall, steps;
+    float eps;
+    float4* partial;      // [C][32 column quads][128 rows]
+    uint8_t* image;       // A as it lies in shared memory
+};
+
+// V elements of the long (wide G) or the short side (tall G), whichever is contiguous, at a time.
+template <int V, bool MOMENTUM>
+__global__ void __launch_bounds__(CL_THREADS, 1) ns_cluster_kernel(const ClusterArgs P) {
+    using namespace t5;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint64_t done_bar, copy_bar;
+    __shared__ uint32_t tmem_slot;
+    __shared__ volatile int abort_flag;
+    __shared__ double norms[CL_MAX], sums[CL_THREADS / 32];
+    uint8_t* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint8_t* const X = smem;                        // hi, lo of this CTA's slab: [d][slab]
+    uint8_t* const A = smem + CL_MATRIX;            // hi, lo of A, then of B: [d][d]
+    float* const E = reinterpret_cast<float*>(smem + 2 * CL_MATRIX);
+    const uint32_t x_addr = smem_u32(X), a_addr = smem_u32(A), bar = smem_u32(&done_bar), cbar = smem_u32(&copy_bar);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int rank = static_cast<int>(cluster_ctarank()), ctas = static_cast<int>(gridDim.x);
+    const int d = P.d, d16 = (d + 15) & ~15, w16 = P.slab, n0 = rank * P.slab;
+    const int width = P.length - n0 < P.slab ? (P.length - n0 > 0 ? P.length - n0 : 0) : P.slab;  // this CTA's part that exists
+
+    if (tid == 0) {
+        abort_flag = 0;
+        mbar_init(bar, 1);
+        mbar_init(cbar, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 0) tmem_alloc<1>(smem_u32(&tmem_slot), 256);
+    // every operand byte a product may touch is defined: rows and columns past d and the slab are zero
+    for (int i = tid; i < 2 * CL_MATRIX / 16; i += CL_THREADS) *reinterpret_cast<uint4*>(smem + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+    if (width < w16)
+        for (int t = tid; t < d * (w16 - width); t += CL_THREADS) E[(t % d) * CL_PITCH + width + t / d] = 0.0f;
+
+    // ---- U into E, the momentum update, the norm ----
+    const Source& S = P.S;
+    const int fast = (P.tall ? d : width) / V, total = (P.tall ? width : d) * fast;  // accesses of V elements
+    constexpr int U = 4;                                                           // of them in flight per thread
+    double acc = 0.0;
+    for (int t0 = tid; t0 < total; t0 += U * CL_THREADS) {
+        Vec<V> u[U], m[U];
+        int sl[U], fa[U];
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            const int t = t0 + k * CL_THREADS;
+            sl[k] = t / fast;
+            fa[k] = (t - sl[k] * fast) * V;
+            if (t >= total) continue;
+            const int64_t r = P.tall ? n0 + sl[k] : sl[k], c = P.tall ? fa[k] : n0 + fa[k];
+            u[k] = load_vec<V>(S.g + r * S.ldg + c);
+            if (MOMENTUM) m[k] = load_vec<V>(S.momentum + r * S.ldm + c);
+        }
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            if (t0 + k * CL_THREADS >= total) continue;
+            if (MOMENTUM) {
+#pragma unroll
+                for (int q = 0; q < V; ++q) {
+                    m[k].v[q] = fmaf(S.mu, m[k].v[q], u[k].v[q]);
+                    u[k].v[q] = S.nesterov ? fmaf(S.mu, m[k].v[q], u[k].v[q]) : m[k].v[q];
+                }
+                *reinterpret_cast<Vec<V>*>(S.momentum + (P.tall ? n0 + sl[k] : sl[k]) * S.ldm + (P.tall ? fa[k] : n0 + fa[k])) = m[k];
+            }
+#pragma unroll
+            for (int q = 0; q < V; ++q) {
+                acc = fma(static_cast<double>(u[k].v[q]), static_cast<double>(u[k].v[q]), acc);
+                E[(P.tall ? fa[k] + q : sl[k]) * CL_PITCH + (P.tall ? sl[k] : fa[k] + q)] = u[k].v[q];
+            }
+        }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+    if (lane == 0) sums[warp] = acc;
+    cluster_sync_all();  // every CTA runs (its shared memory may be written), and this one's sums are there
+    if (tid < ctas) {
+        double part = 0.0;
+        for (int w = 0; w < CL_THREADS / 32; ++w) part += sums[w];
+        const uint32_t to = map_to_cta(smem_u32(&norms[rank]), static_cast<uint32_t>(tid));
+        asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(to), "d"(part) : "memory");
+    }
+    cluster_sync_all();
+    double sumsq = 0.0;
+    for (int i = 0; i < ctas; ++i) sumsq += norms[i];
+    const Normaliser N = normaliser(sumsq, P.eps);
+    int e = N.e;
+    for (int t = tid; t < d * (w16 / 8); t += CL_THREADS) {
+        const int i = t / (w16 / 8), c = t % (w16 / 8);
+        float x[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) x[q] = (E[i * CL_PITCH + c * 8 + q] * N.p2) * (N.rest * kScaleX);
+        uint4 hi, lo;
+        split8(x, hi, lo);
+        *reinterpret_cast<uint4*>(X + cl_chunk(i, c)) = hi;
+        *reinterpret_cast<uint4*>(X + 2 * CL_GROUP + cl_chunk(i, c)) = lo;
+    }
+    asm volatile("fence.proxy.async;" ::: "memory");
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = tmem_slot;
+    uint32_t phase = 0, copy_phase = 0;
+    const int row = (warp & 3) * 32 + lane, c0 = (warp >> 2) * 32;  // accumulator row and first of 32 columns of this thread
+    const uint32_t t_row = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + c0;
+    const bool live = row < d;
+
+    // operand a (K-major) times operand b over `kk` terms, the first half of them into columns 0.., the second into 128..;
+    // in each the small terms go first.
+    auto product = [&](uint32_t a, uint32_t b, bool b_mn, int n, int kk) {
+        if (tid != 0) return;
+        fence_after();
+        asm volatile("fence.proxy.async;" ::: "memory");
+        const uint32_t idesc = make_idesc(128, 0, false, b_mn) | (static_cast<uint32_t>(n >> 3) << 17);
+        // (descriptors hold addresses in units of 16 bytes: every step is an addition of a constant)
+        constexpr uint64_t LO = (2 * CL_GROUP) >> 4, GROUP = CL_GROUP >> 4, K16 = 32 >> 4, K16_MN = 2048 >> 4;
+        const uint64_t da = make_desc(a, 0), db = make_desc(b, b_mn ? CL_GROUP : 0);
+        const uint64_t b_step = b_mn ? K16_MN : K16, b_half = b_mn ? 4 * K16_MN : GROUP;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t acc_at = tmem + h * 128;
+            const uint64_t ah = da + h * GROUP, bh = db + h * b_half;
+            const int n16 = kk / 16 - h * 4;
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) {
+                if (ks >= n16) break;
+                mma_f16<1>(acc_at, ah + LO + ks * K16, bh + ks * b_step, idesc, ks > 0);
+                mma_f16<1>(acc_at, ah + ks * K16, bh + LO + ks * b_step, idesc, 1u);
+            }
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) {
+                if (ks >= n16) break;
+                mma_f16<1>(acc_at, ah + ks * K16, bh + ks * b_step, idesc, 1u);
+            }
+        }
+        commit<1>(bar);
+    };
+    // This thread's 32 columns of the last product.  (A wait that runs out is recorded; the kernel carries on to its end,
+    // so that no CTA is left at a cluster barrier.)
+    auto result = [&](int n, bool two, float (&v)[32]) {
+        mbar_wait(bar, phase, &abort_flag, &g_ns_status, 0x400);
+        phase ^= 1u;
+        fence_after();
+        if (c0 >= n) return false;  // (the same for the whole warp)
+        uint32_t r[32];
+        tmem_ld32(t_row, r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+        if (two) {
+            tmem_ld32(t_row + 128, r);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] += __uint_as_float(r[i]);
+        }
+        return live;
+    };
+    // The 16-byte chunk q of this thread's 32 columns, of hi or (lo != 0) lo.
+    auto chunk_of = [&](uint8_t* m, int q, int lo) { return reinterpret_cast<uint4*>(m + lo * 2 * CL_GROUP + cl_chunk(row, (c0 >> 3) + q)); };
+
+    for (int s = 0; s < P.steps; ++s) {
+        const int drop = e < 2 ? e : 2;
+        const float cb = ldexpf(kB, -2 * e) * 0.5f, cc = ldexpf(kC, -4 * e) * (1.0f / 65536.0f);
+        const bool last = s + 1 == P.steps;
+        const float f = ldexpf(1.0f, last ? -e : -drop);
+        e -= drop;
+        float v[32];
+
+        // ---- A = X X^T ----
+        product(x_addr, x_addr, false, d16, w16);
+        if (result(d16, w16 > 64, v)) {
+            if (ctas == 1) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    if (c0 + q * 8 >= d16) break;
+                    float x[8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) x[k] = v[q * 8 + k] * (1.0f / 32768.0f);
+                    uint4 hi, lo;
+                    split8(x, hi, lo);
+                    *chunk_of(A, q, 0) = hi;
+                    *chunk_of(A, q, 1) = lo;
+                }
+            } else {
+                float4* out = P.partial + (rank * 32 + (c0 >> 2)) * CL_SIDE + row;
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                    if (c0 + q * 4 < d16) __stcg(out + q * CL_SIDE, make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]));
+            }
+        }
+        if (ctas == 1) {
+            asm volatile("fence.proxy.async;" ::: "memory");
+            fence_before();
+            __syncthreads();
+        } else {
+            fence_before();
+            cluster_sync_all();
+            const int quads = d16 / 4;
+            for (int t = tid; t < ((quads - rank + ctas - 1) / ctas) * CL_SIDE; t += CL_THREADS) {
+                const int c = rank + (t / CL_SIDE) * ctas, i = t % CL_SIDE;  // columns 4c.., row i
+                if (c >= quads || i >= d) continue;
+                float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int k0 = 0; k0 < ctas; k0 += 8) {
+                    float4 p[8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        p[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (k0 + k < ctas) p[k] = __ldcg(P.partial + ((k0 + k) * 32 + c) * CL_SIDE + i);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) { sum.x += p[k].x; sum.y += p[k].y; sum.z += p[k].z; sum.w += p[k].w; }
+                }
+                constexpr float S2 = 1.0f / 32768.0f;
+                uint2 hi, lo;
+                split2(sum.x * S2, sum.y * S2, hi.x, lo.x);
+                split2(sum.z * S2, sum.w * S2, hi.y, lo.y);
+                uint8_t* to = P.image + cl_chunk(i, c >> 1) + (c & 1) * 8;
+                __stcg(reinterpret_cast<uint2*>(to), hi);
+                __stcg(reinterpret_cast<uint2*>(to + 2 * CL_GROUP), lo);
+            }
+            asm volatile("fence.proxy.async;" ::: "memory");  // the copies below read what these stores wrote
+            cluster_sync_all();
+            const int groups = d16 > 64 ? 2 : 1;
+            if (tid == 0) {
+                asm volatile("fence.proxy.async;" ::: "memory");
+                mbar_expect_tx(cbar, static_cast<uint32_t>(2 * groups * d * 128));
+                for (int g = 0; g < 2 * groups; ++g) {
+                    const uint32_t at = ((g & 1) * 2 + (g >> 1)) * CL_GROUP;  // hi and lo of group 0, then of group 1
+                    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                                 ::"r"(a_addr + at), "l"(P.image + at), "r"(static_cast<uint32_t>(d * 128)), "r"(cbar) : "memory");
+                }
+            }
+            mbar_wait(cbar, copy_phase, &abort_flag, &g_ns_status, 0x410);
+            copy_phase ^= 1u;
+        }
+
+        // ---- B = b A + c A A, in A's place ----
+        product(a_addr, a_addr, false, d16, d16);
+        if (result(d16, d16 > 64, v)) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                if (c0 + q * 8 >= d16) break;
+                float x[8];
+                uint4 hi = *chunk_of(A, q, 0), lo = *chunk_of(A, q, 1);
+                join8(hi, lo, x);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) x[k] = fmaf(cb, x[k], cc * v[q * 8 + k]);
+                split8(x, hi, lo);
+                *chunk_of(A, q, 0) = hi;
+                *chunk_of(A, q, 1) = lo;
+            }
+        }
+        asm volatile("fence.proxy.async;" ::: "memory");
+        fence_before();
+        __syncthreads();
+
+        // ---- X = f (a X + B X) ----
+        product(a_addr, x_addr, true, w16, d16);
+        if (result(w16, d16 > 64, v)) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                if (c0 + q * 8 >= w16) break;
+                float x[8];
+                uint4 hi = *chunk_of(X, q, 0), lo = *chunk_of(X, q, 1);
+                join8(hi, lo, x);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) x[k] = f * fmaf(kA, x[k], v[q * 8 + k] * (1.0f / 16384.0f));
+                if (last) {
+                    float4* out = reinterpret_cast<float4*>(E + row * CL_PITCH + c0 + q * 8);
+                    out[0] = make_float4(x[0], x[1], x[2], x[3]);
+                    out[1] = make_float4(x[4], x[5], x[6], x[7]);
+                } else {
+                    split8(x, hi, lo);
+                    *chunk_of(X, q, 0) = hi;
+                    *chunk_of(X, q, 1) = lo;
+                }
+            }
+        }
+        asm volatile("fence.proxy.async;" ::: "memory");
+        fence_before();
+        __syncthreads();
+    }
+
+    // ---- the result ----
+    for (int t0 = tid; t0 < total; t0 += U * CL_THREADS) {
+        Vec<V> old[U];
+        float* at[U];
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            const int t = t0 + k * CL_THREADS, sl = t / fast, fa = (t - sl * fast) * V;
+            at[k] = P.K.out + (P.tall ? n0 + sl : sl) * P.K.ldo + (P.tall ? fa : n0 + fa);
+            if (P.K.update && t < total) old[k] = load_vec<V>(at[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            const int t = t0 + k * CL_THREADS, sl = t / fast, fa = (t - sl * fast) * V;
+            if (t >= total) continue;
+            Vec<V> o;
+#pragma unroll
+            for (int q = 0; q < V; ++q)
+                o.v[q] = sink_value(P.K, E[(P.tall ? fa + q : sl) * CL_PITCH + (P.tall ? sl : fa + q)] * (1.0f / kScaleX), P.K.update ? old[k].v[q] : 0.0f);
+            *reinterpret_cast<Vec<V>*>(at[k]) = o;
+        }
+    }
+    if (ctas > 1) cluster_sync_all();  // no CTA leaves while another may still signal it
+    else __syncthreads();
+    if (warp == 0) {
+        fence_after();
+        tmem_dealloc<1>(tmem, 256);
+    }
+}
+
 // ---- host side -------------------------------------------------------------------------------------------
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
                                    CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -625,20 +988,76 @@ ctk_status run_steps(const Layout& L, char* ws, int64_t rows, int64_t cols, Sink
     return rc;
 }
 
+template <int V, bool MOMENTUM>
+ctk_status launch_cluster(const ClusterArgs& P, int ctas, cudaStream_t st) {
+    auto kernel = ns_cluster_kernel<V, MOMENTUM>;
+    static ctk::PerDeviceOnce attr_set;
+    if (attr_set.first()) {
+        CTK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, CL_SMEM));
+        CTK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    }
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(ctas);
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+    cfg.blockDim = dim3(CL_THREADS);
+    cfg.dynamicSmemBytes = CL_SMEM;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    CTK_CUDA(cudaLaunchKernelEx(&cfg, kernel, P));
+    CTK_LAUNCH_CHECK("ns_cluster_kernel");
+    return CTK_OK;
+}
+
+// How many CTAs take a matrix in one launch, 0 if it is too large for that.
+int cluster_ctas(int64_t d, int64_t length) {
+    if (d > CL_SIDE || length > CL_MAX * CL_SIDE) return 0;
+    int ctas = 1;
+    while (ctas * CL_SIDE < length) ctas *= 2;
+    return ctas;
+}
+size_t workspace_for(int64_t rows, int64_t cols) {
+    const int ctas = cluster_ctas(rows < cols ? rows : cols, rows < cols ? cols : rows);
+    return ctas ? (cl_workspace(ctas) ? cl_workspace(ctas) : 256) : layout_for(rows, cols).total;
+}
+
 ctk_status newton_schulz(const Source& S, Sink K, int steps, float eps, void* workspace, void* stream) {
-    const Layout L = layout_for(S.rows, S.cols);
+    const int64_t d = S.rows < S.cols ? S.rows : S.cols, length = S.rows < S.cols ? S.cols : S.rows;
+    const bool vec = S.cols % 4 == 0 && S.ldg % 4 == 0 && aligned_to(S.g, 16) && (!S.momentum || (S.ldm % 4 == 0 && aligned_to(S.momentum, 16)));
+    K.vec = K.ldo % 4 == 0 && aligned_to(K.out, 16);
     StreamScratch scratch;
-    if (!workspace) {
-        ctk_status st = scratch.get(L.total, stream);
+    const int ctas = cluster_ctas(d, length);
+    if (!workspace && ctas != 1) {
+        ctk_status st = scratch.get(workspace_for(S.rows, S.cols), stream);
         if (st) return st;
         workspace = scratch.p;
     }
+    if (ctas) {
+        ClusterArgs P = {};
+        P.S = S;
+        P.K = K;
+        P.d = static_cast<int>(d);
+        P.length = static_cast<int>(length);
+        P.slab = static_cast<int>((length + ctas - 1) / ctas + 15) / 16 * 16;
+        P.tall = S.rows > S.cols;
+        P.steps = steps;
+        P.eps = eps;
+        P.partial = static_cast<float4*>(workspace);
+        P.image = static_cast<uint8_t*>(workspace) + static_cast<size_t>(ctas) * CL_PARTIAL;
+        const bool v4 = vec && K.vec;
+        cudaStream_t st = as_stream(stream);
+        if (S.momentum) return v4 ? launch_cluster<4, true>(P, ctas, st) : launch_cluster<1, true>(P, ctas, st);
+        return v4 ? launch_cluster<4, false>(P, ctas, st) : launch_cluster<1, false>(P, ctas, st);
+    }
+    const Layout L = layout_for(S.rows, S.cols);
     char* ws = static_cast<char*>(workspace);
     double* partial = reinterpret_cast<double*>(ws + L.partial);
     float* coef = reinterpret_cast<float*>(ws + L.coef);
     cudaStream_t st = as_stream(stream);
-    const bool vec = S.cols % 4 == 0 && S.ldg % 4 == 0 && aligned_to(S.g, 16) && (!S.momentum || (S.ldm % 4 == 0 && aligned_to(S.momentum, 16)));
-    K.vec = K.ldo % 4 == 0 && aligned_to(K.out, 16);
     int grid = ctk_stream_grid(S.rows * S.cols / (vec ? 4 : 1), PREP_THREADS, 6);
     if (grid > MAX_PARTS) grid = MAX_PARTS;
     const Pair X0{reinterpret_cast<__half*>(ws + L.x[0]), L.pitch_x, S.rows * L.pitch_x};
@@ -652,7 +1071,6 @@ ctk_status newton_schulz(const Source& S, Sink K, int steps, float eps, void* wo
     ctk_status rc = S.momentum ? (vec ? prep(prep_norm_kernel<4, true>, prep_split_kernel<4, true>) : prep(prep_norm_kernel<1, true>, prep_split_kernel<1, true>))
                                : (vec ? prep(prep_norm_kernel<4, false>, prep_split_kernel<4, false>) : prep(prep_norm_kernel<1, false>, prep_split_kernel<1, false>));
     if (rc) return rc;
-    const int64_t d = S.rows < S.cols ? S.rows : S.cols;
     return d > 1024 ? run_steps<2>(L, ws, S.rows, S.cols, K, steps, st) : run_steps<1>(L, ws, S.rows, S.cols, K, steps, st);
 }
 
@@ -673,7 +1091,7 @@ extern "C" {
 
 size_t ctk_orthogonalize_workspace_bytes(int64_t rows, int64_t cols) {
     if (rows <= 0 || cols <= 0 || rows > (int64_t(1) << 30) || cols > (int64_t(1) << 30) / rows) return 0;
-    return layout_for(rows, cols).total;
+    return workspace_for(rows, cols);
 }
 
 ctk_status ctk_orthogonalize_f32(const float* g, int64_t ldg, float* out, int64_t ldo, int64_t rows, int64_t cols, int steps, float eps, void* workspace,

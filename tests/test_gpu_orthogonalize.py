@@ -227,3 +227,18 @@ def test_large_matrix_rows_against_float64(cb):
     """2100 x 2060: every tile row of the large kernels, edges included."""
     g = grad_like(np.random.default_rng(2), 2100, 2060)
     assert rel(cb.ops.orthogonalize(cb.to_device(g)).numpy(), ns64(g)) <= ns_tol(5)
+
+
+@pytest.mark.parametrize("shape", [(1, 2048), (2048, 1), (128, 2048), (2048, 128), (127, 2047), (65, 1025), (1030, 17), (16, 16), (17, 129), (128, 129), (129, 128),
+                                   (2, 3), (100, 640), (500, 33), (128, 2049), (2049, 128)])
+def test_sizes_around_the_one_launch_limit(cb, shape):
+    rng = np.random.default_rng(shape[0] + 3 * shape[1])
+    g, p, m = grad_like(rng, *shape), rng.standard_normal(shape).astype(np.float32), grad_like(rng, *shape)
+    assert rel(cb.ops.orthogonalize(cb.to_device(g)).numpy(), ns64(g)) <= ns_tol(5)
+    dp, dm = cb.to_device(p), cb.to_device(m)
+    cb.ops.muon_update(dp, cb.to_device(g), dm, lr=0.5, momentum=0.5, scale=1.0)
+    m64 = 0.5 * m.astype(np.float64) + g
+    o = ns64(g + 0.5 * m64)
+    assert np.linalg.norm(dp.numpy() - (p - 0.5 * o)) <= 0.5 * np.linalg.norm(o) * (ns_tol(5) + 3 * 2.0 ** -24) + 3 * 2.0 ** -24 * np.linalg.norm(p)
+    assert (np.abs(dm.numpy() - m64) <= 2.0 ** -23 * (np.abs(0.5 * m) + np.abs(g)) + 1e-38).all()
+    assert cb.ops.orthogonalize_status() == 0
