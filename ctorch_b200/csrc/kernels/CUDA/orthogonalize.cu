@@ -203,6 +203,7 @@ constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_WARPS * 32 * OUT_PITCH * 4
 struct Params {
     int m, n;                 // extents of the product's result
     int tiles_m, tiles_n, units, num_kb;
+    int split;                // medium matrices: CTAs that share a tile's k-blocks
     Pair src;                 // POLY: A; APPLY: X before the step
     Pair dst;                 // GRAM: A; POLY: B; APPLY: X after the step (unless last)
     const float* coef;        // this step's {b, c, f}
@@ -498,6 +499,233 @@ __global__ void __launch_bounds__(THREADS, 1) ns_product_kernel(const __grid_con
     }
 }
 
+__device__ __forceinline__ void split8(const float (&x)[8], uint4& hi, uint4& lo) {
+    split2(x[0], x[1], hi.x, lo.x);
+    split2(x[2], x[3], hi.y, lo.y);
+    split2(x[4], x[5], hi.z, lo.z);
+    split2(x[6], x[7], hi.w, lo.w);
+}
+__device__ __forceinline__ void join8(const uint4& hi, const uint4& lo, float (&x)[8]) {
+    const uint32_t h[4] = {hi.x, hi.y, hi.z, hi.w}, l[4] = {lo.x, lo.y, lo.z, lo.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&h[e])), b = __half22float2(*reinterpret_cast<const __half2*>(&l[e]));
+        x[2 * e] = a.x + b.x;
+        x[2 * e + 1] = a.y + b.y;
+    }
+}
+
+// ---- products of medium matrices -------------------------------------------------------------------------
+// A 128 x 128 tile per cluster of `split` CTAs, each with its share of the k-blocks: with d <= 1024 there are few tiles,
+// and a CTA alone takes its operands from L2 at one SM's rate (64 KB a k-block, about 0.9 us).  The CTAs' sums meet in L2
+// (fp32, [column quad][row], so that a warp's store is one run); after a cluster barrier each CTA adds 128 / split
+// columns over all of them, in rank order, and takes these through the epilogue from shared memory -- compact loops,
+// because at these sizes straight-line code spends its time on instruction fetches (the persistent kernel's unrolled
+// epilogue took 10 us for its one tile).
+constexpr int MID_THREADS = 576;  // warp 0 loads, warp 1 multiplies, warps 2-17: 4 per quarter of the rows, 32 columns each
+constexpr int MID_MAX_CTAS = 160;
+constexpr int MID_SMEM = STAGES * STAGE_BYTES + 1024;
+constexpr int MID_PITCH = 129;
+
+template <int MODE, bool A_MN, bool B_MN>
+__global__ void __launch_bounds__(MID_THREADS, 1) ns_tile_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Params P,
+                                                                 float4* __restrict__ partial) {
+    using namespace t5;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint64_t bars[2 * STAGES + 4];
+    __shared__ uint32_t tmem_slot;
+    __shared__ volatile int abort_flag;
+    const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    float* const E = reinterpret_cast<float*>(smem_raw + (smem_base - smem_u32(smem_raw)));  // after the main loop: the tile, [row][column]
+    const uint32_t bar0 = smem_u32(bars);
+    auto full_bar = [&](int s) { return bar0 + 8u * s; };
+    auto empty_bar = [&](int s) { return bar0 + 8u * (STAGES + s); };
+    auto tfull_bar = [&](int a) { return bar0 + 8u * (2 * STAGES + a); };
+    auto tempty_bar = [&](int a) { return bar0 + 8u * (2 * STAGES + 2 + a); };
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int split = P.split, rank = static_cast<int>(cluster_ctarank()), unit = blockIdx.x / split;
+    const int kb0 = P.num_kb * rank / split, kb1 = P.num_kb * (rank + 1) / split;
+    int tm, tn;
+    unit_tile<MODE>(unit, P, tm, tn);
+
+    if (tid == 0) {
+        abort_flag = 0;
+        for (int s = 0; s < STAGES; ++s) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
+        for (int a = 0; a < 2; ++a) { mbar_init(tfull_bar(a), 1); mbar_init(tempty_bar(a), 16); }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        prefetch_tmap(&map_a);
+        prefetch_tmap(&map_b);
+    }
+    if (warp == 1) tmem_alloc<1>(smem_u32(&tmem_slot), 256);
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = tmem_slot;
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // what the kernel before wrote is there
+
+    float v[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = 0.0f;
+    const int quarter = warp & 3, c0 = ((warp - 2) >> 2) * 32;  // epilogue warps: rows 32 quarter.., columns c0..
+    if (warp == 0) {
+        if (lane == 0) {
+            bool ok = true;
+            const int m0 = tm * BM, n0 = tn * BM;
+            int issued = 0;
+            for (int kb = kb0; kb < kb1; ++kb, ++issued) {
+                const int st = issued % STAGES;
+                if (!mbar_wait(empty_bar(st), ((issued / STAGES) & 1) ^ 1u, &abort_flag, &g_ns_status, 0x500 | st)) { ok = false; break; }
+                mbar_expect_tx(full_bar(st), STAGE_BYTES);
+                const uint32_t fb = full_bar(st), base = smem_base + st * STAGE_BYTES;
+                const int k0 = kb * BK;
+                if (A_MN) {
+                    tma_load_3d<1>(base, &map_a, fb, m0, k0, 0);
+                    tma_load_3d<1>(base + STAGE_BYTES / 4, &map_a, fb, m0 + 64, k0, 0);
+                } else {
+                    tma_load_3d<1>(base, &map_a, fb, k0, m0, 0);
+                }
+                if (B_MN) {
+                    tma_load_3d<1>(base + STAGE_BYTES / 2, &map_b, fb, n0, k0, 0);
+                    tma_load_3d<1>(base + 3 * (STAGE_BYTES / 4), &map_b, fb, n0 + 64, k0, 0);
+                } else {
+                    tma_load_3d<1>(base + STAGE_BYTES / 2, &map_b, fb, k0, n0, 0);
+                }
+            }
+            // (every copy issued has been waited for by the multiplying warp unless a wait ran out: then give the copies in flight
+            // a couple of milliseconds to land)
+            if (!ok)
+                for (int i = 0; i < 2048; ++i) __nanosleep(1000);
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            constexpr uint32_t idesc = make_idesc(BM, BM, A_MN, B_MN);
+            constexpr uint64_t a_lo = (A_MN ? STAGE_BYTES / 8 : STAGE_BYTES / 4) >> 4, b_lo = (B_MN ? STAGE_BYTES / 8 : STAGE_BYTES / 4) >> 4;
+            constexpr uint64_t a_step = (A_MN ? 2048u : 32u) >> 4, b_step = (B_MN ? 2048u : 32u) >> 4;
+            constexpr uint32_t a_lbo = A_MN ? STAGE_BYTES / 4 : 0u, b_lbo = B_MN ? STAGE_BYTES / 4 : 0u;
+            for (int i = 0; i < kb1 - kb0; ++i) {
+                const int st = i % STAGES, acc = i & 1;
+                if (!mbar_wait(tempty_bar(acc), ((i >> 1) & 1) ^ 1u, &abort_flag, &g_ns_status, 0x600 | acc)) break;
+                if (!mbar_wait(full_bar(st), (i / STAGES) & 1, &abort_flag, &g_ns_status, 0x610 | st)) break;
+                fence_after();
+                const uint32_t d = tmem + acc * 128;
+                const uint64_t a = make_desc(smem_base + st * STAGE_BYTES, a_lbo), b = make_desc(smem_base + st * STAGE_BYTES + STAGE_BYTES / 2, b_lbo);
+#pragma unroll
+                for (int ks = 0; ks < BK / 16; ++ks) {  // the small terms first, while the accumulator is small
+                    mma_f16<1>(d, a + a_lo + ks * a_step, b + ks * b_step, idesc, ks > 0);
+                    mma_f16<1>(d, a + ks * a_step, b + b_lo + ks * b_step, idesc, 1u);
+                }
+#pragma unroll
+                for (int ks = 0; ks < BK / 16; ++ks) mma_f16<1>(d, a + ks * a_step, b + ks * b_step, idesc, 1u);
+                commit<1>(empty_bar(st));
+                commit<1>(tfull_bar(acc));
+            }
+        }
+    } else {
+        const uint32_t t_row = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + c0;
+        for (int i = 0; i < kb1 - kb0; ++i) {
+            const int acc = i & 1;
+            if (!mbar_wait(tfull_bar(acc), (i >> 1) & 1, &abort_flag, &g_ns_status, 0x700 | acc)) break;
+            fence_after();
+            uint32_t r[32];
+            tmem_ld32(t_row + acc * 128, r);
+            tmem_ld_wait();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(tempty_bar(acc));
+#pragma unroll
+            for (int q = 0; q < 32; ++q) v[q] += __uint_as_float(r[q]);
+        }
+    }
+    // ---- the CTAs' sums meet; this CTA's columns of the tile into E ----
+    const int row = quarter * 32 + lane, cols = BM / split;  // (epilogue warps; columns this CTA finishes)
+    if (split > 1) {
+        if (warp >= 2) {
+            float4* out = partial + (static_cast<int64_t>(blockIdx.x) * 32 + (c0 >> 2)) * BM + row;
+#pragma unroll
+            for (int q = 0; q < 8; ++q) __stcg(out + q * BM, make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]));
+        }
+        fence_before();
+        cluster_sync_all();
+        for (int t = tid; t < (cols / 4) * BM; t += MID_THREADS) {
+            const int c = t / BM, i = t % BM;
+            const float4* in = partial + (static_cast<int64_t>(unit) * split * 32 + rank * (cols / 4) + c) * BM + i;
+            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f), p[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                p[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (k < split) p[k] = __ldcg(in + static_cast<int64_t>(k) * 32 * BM);
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) { sum.x += p[k].x; sum.y += p[k].y; sum.z += p[k].z; sum.w += p[k].w; }
+            float* e = E + i * MID_PITCH + c * 4;
+            e[0] = sum.x; e[1] = sum.y; e[2] = sum.z; e[3] = sum.w;
+        }
+    } else {
+        fence_before();
+        if (warp >= 2) {
+#pragma unroll
+            for (int q = 0; q < 32; ++q) E[row * MID_PITCH + c0 + q] = v[q];
+        }
+    }
+    __syncthreads();
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (warp == 1) {
+        fence_after();
+        tmem_dealloc<1>(tmem, 256);
+    }
+
+    // ---- the epilogue, 8 columns of a row at a time ----
+    const float cf0 = __ldg(P.coef), cf1 = __ldg(P.coef + 1), cf2 = __ldg(P.coef + 2);
+    const int chunks = cols / 8, col_base = tn * BM + rank * cols, row_base = tm * BM;
+    for (int t = tid; t < chunks * BM; t += MID_THREADS) {
+        const int i = t / chunks, c = (t - i * chunks) * 8;
+        const int64_t r = row_base + i, col = col_base + c;
+        if (r >= P.m || col >= P.n) continue;
+        float* e = E + i * MID_PITCH + c;
+        float x[8];
+        if (MODE != GRAM) {  // (pitches are multiples of 8: eight elements never leave the row)
+            const __half* sp = P.src.hi + r * P.src.pitch + col;
+            join8(__ldcg(reinterpret_cast<const uint4*>(sp)), __ldcg(reinterpret_cast<const uint4*>(sp + P.src.lo)), x);
+        }
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            if (MODE == GRAM) x[q] = e[q] * (1.0f / 32768.0f);
+            if (MODE == POLY) x[q] = fmaf(cf0 * 0.5f, x[q], cf1 * (1.0f / 65536.0f) * e[q]);
+            if (MODE == APPLY) x[q] = cf2 * fmaf(kA, x[q], e[q] * (1.0f / 16384.0f));
+        }
+        if (MODE == APPLY && P.last) {
+            float* out = P.sink.out + r * P.sink.ldo + col;
+            for (int q = 0; q < 8; ++q)
+                if (col + q < P.n) out[q] = sink_value(P.sink, x[q] * (1.0f / kScaleX), P.sink.update ? out[q] : 0.0f);
+            continue;
+        }
+        uint4 hi, lo;
+        split8(x, hi, lo);
+        __half* d = P.dst.hi + r * P.dst.pitch + col;
+        *reinterpret_cast<uint4*>(d) = hi;
+        *reinterpret_cast<uint4*>(d + P.dst.lo) = lo;
+        if (MODE != APPLY && tm != tn) {
+#pragma unroll
+            for (int q = 0; q < 8; ++q) e[q] = x[q];
+        }
+    }
+    if (MODE != APPLY && tm != tn) {  // the mirror place: 8 rows of a column at a time
+        __syncthreads();
+        for (int t = tid; t < cols * (BM / 8); t += MID_THREADS) {
+            const int c = t / (BM / 8), i = (t % (BM / 8)) * 8;
+            if (col_base + c >= P.n || row_base + i >= P.m) continue;
+            float x[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) x[q] = E[(i + q) * MID_PITCH + c];
+            uint4 hi, lo;
+            split8(x, hi, lo);
+            __half* d = P.dst.hi + static_cast<int64_t>(col_base + c) * P.dst.pitch + row_base + i;
+            *reinterpret_cast<uint4*>(d) = hi;
+            *reinterpret_cast<uint4*>(d + P.dst.lo) = lo;
+        }
+    }
+}
+
 // ---- small matrices: every step in one launch ------------------------------------------------------------
 // d <= 128 and L <= 2048: a cluster of C CTAs, C = 1, 2, 4, 8 or 16, holds X in shared memory, each CTA a slab of at most 128
 // of the L side, from the first read of G to the last write.  A slab row is one index of the short side, 128 bytes of 64
@@ -521,22 +749,6 @@ constexpr size_t cl_workspace(int ctas) { return ctas > 1 ? static_cast<size_t>(
 
 // Byte offset of the 16-byte chunk with elements [8 c, 8 c + 8) of row r.
 __device__ __forceinline__ uint32_t cl_chunk(int r, int c) { return static_cast<uint32_t>((c >> 3) * CL_GROUP + r * 128 + (((c & 7) ^ (r & 7)) << 4)); }
-
-__device__ __forceinline__ void split8(const float (&x)[8], uint4& hi, uint4& lo) {
-    split2(x[0], x[1], hi.x, lo.x);
-    split2(x[2], x[3], hi.y, lo.y);
-    split2(x[4], x[5], hi.z, lo.z);
-    split2(x[6], x[7], hi.w, lo.w);
-}
-__device__ __forceinline__ void join8(const uint4& hi, const uint4& lo, float (&x)[8]) {
-    const uint32_t h[4] = {hi.x, hi.y, hi.z, hi.w}, l[4] = {lo.x, lo.y, lo.z, lo.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&h[e])), b = __half22float2(*reinterpret_cast<const __half2*>(&l[e]));
-        x[2 * e] = a.x + b.x;
-        x[2 * e + 1] = a.y + b.y;
-    }
-}
 
 struct ClusterArgs {
     Source S;
@@ -923,11 +1135,43 @@ ctk_status launch_product(const CUtensorMap& a, const CUtensorMap& b, Params P, 
     return CTK_OK;
 }
 
+// PDL: the launch may start before the kernel in front of it has ended, up to its griddepcontrol.wait.
+template <int MODE, bool A_MN, bool B_MN>
+ctk_status launch_tile(const CUtensorMap& a, const CUtensorMap& b, Params P, float4* partial, cudaStream_t st) {
+    auto kernel = ns_tile_kernel<MODE, A_MN, B_MN>;
+    static ctk::PerDeviceOnce attr_set;
+    if (attr_set.first()) CTK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MID_SMEM));
+    P.tiles_m = (P.m + BM - 1) / BM;
+    P.tiles_n = (P.n + BM - 1) / BM;
+    P.units = MODE == APPLY ? P.tiles_m * P.tiles_n : P.tiles_n * (P.tiles_n + 1) / 2;
+    // as many CTAs to a tile as the SMs hold at once, each with a k-block at least
+    P.split = 1;
+    while (P.split < 8 && P.units * P.split * 2 <= MID_MAX_CTAS && P.units * P.split * 2 <= ctk::sm_count() && P.split * 2 <= P.num_kb) P.split *= 2;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(P.split);
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3(static_cast<unsigned>(P.units * P.split));
+    cfg.blockDim = dim3(MID_THREADS);
+    cfg.dynamicSmemBytes = MID_SMEM;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    CTK_CUDA(cudaLaunchKernelEx(&cfg, kernel, a, b, P, partial));
+    CTK_LAUNCH_CHECK("ns_tile_kernel");
+    return CTK_OK;
+}
+
 struct Layout {
-    size_t partial, coef, x[2], a, b, total;
+    size_t partial, coef, x[2], a, b, sums, total;
     int64_t pitch_x, pitch_d;
 };
 constexpr int MAX_PARTS = 1024, MAX_STEPS = 64;
+constexpr int64_t MID_SIDE = 1024;  // short sides up to this take the medium kernels
 Layout layout_for(int64_t rows, int64_t cols) {
     Layout L;
     const int64_t d = rows < cols ? rows : cols;
@@ -941,11 +1185,11 @@ Layout layout_for(int64_t rows, int64_t cols) {
     L.x[1] = take(static_cast<size_t>(rows) * L.pitch_x * 4);
     L.a = take(static_cast<size_t>(d) * L.pitch_d * 4);
     L.b = take(static_cast<size_t>(d) * L.pitch_d * 4);
+    L.sums = take(d > MID_SIDE ? 0 : static_cast<size_t>(MID_MAX_CTAS) * BM * BM * 4);
     L.total = at;
     return L;
 }
 
-template <int GROUP>
 ctk_status run_steps(const Layout& L, char* ws, int64_t rows, int64_t cols, Sink K, int steps, cudaStream_t st) {
     const bool tall = rows > cols;
     const int64_t d = tall ? cols : rows;
@@ -962,6 +1206,8 @@ ctk_status run_steps(const Layout& L, char* ws, int64_t rows, int64_t cols, Sink
     if (!rc) rc = make_map(&ma, A, d, d, 128);
     if (!rc) rc = make_map(&mb, B, d, d, 128);
     const float* coef = reinterpret_cast<const float*>(ws + L.coef);
+    const bool medium = d <= MID_SIDE;
+    float4* sums = reinterpret_cast<float4*>(ws + L.sums);
     auto blocks = [](int64_t k) { return static_cast<int>((k + BK - 1) / BK); };
     for (int s = 0; s < steps && !rc; ++s) {
         const int at = s & 1;
@@ -971,19 +1217,21 @@ ctk_status run_steps(const Layout& L, char* ws, int64_t rows, int64_t cols, Sink
         P.m = P.n = static_cast<int>(d);
         P.num_kb = blocks(tall ? rows : cols);
         P.dst = A;
-        rc = tall ? launch_product<GROUP, GRAM, true, true>(mx_mn[at], mx_mn[at], P, st) : launch_product<GROUP, GRAM, false, false>(mx_k[at], mx_k[at], P, st);
+        if (medium) rc = tall ? launch_tile<GRAM, true, true>(mx_mn[at], mx_mn[at], P, sums, st) : launch_tile<GRAM, false, false>(mx_k[at], mx_k[at], P, sums, st);
+        else rc = tall ? launch_product<2, GRAM, true, true>(mx_mn[at], mx_mn[at], P, st) : launch_product<2, GRAM, false, false>(mx_k[at], mx_k[at], P, st);
         if (rc) return rc;
         P.num_kb = blocks(d);
         P.src = A;
         P.dst = B;
-        rc = launch_product<GROUP, POLY, false, false>(ma, ma, P, st);
+        rc = medium ? launch_tile<POLY, false, false>(ma, ma, P, sums, st) : launch_product<2, POLY, false, false>(ma, ma, P, st);
         if (rc) return rc;
         P.m = static_cast<int>(rows);
         P.n = static_cast<int>(cols);
         P.src = X[at];
         P.dst = X[at ^ 1];
         P.last = s + 1 == steps;
-        rc = tall ? launch_product<GROUP, APPLY, false, false>(mx_k[at], mb, P, st) : launch_product<GROUP, APPLY, false, true>(mb, mx_mn[at], P, st);
+        if (medium) rc = tall ? launch_tile<APPLY, false, false>(mx_k[at], mb, P, sums, st) : launch_tile<APPLY, false, true>(mb, mx_mn[at], P, sums, st);
+        else rc = tall ? launch_product<2, APPLY, false, false>(mx_k[at], mb, P, st) : launch_product<2, APPLY, false, true>(mb, mx_mn[at], P, st);
     }
     return rc;
 }
@@ -1071,7 +1319,7 @@ ctk_status newton_schulz(const Source& S, Sink K, int steps, float eps, void* wo
     ctk_status rc = S.momentum ? (vec ? prep(prep_norm_kernel<4, true>, prep_split_kernel<4, true>) : prep(prep_norm_kernel<1, true>, prep_split_kernel<1, true>))
                                : (vec ? prep(prep_norm_kernel<4, false>, prep_split_kernel<4, false>) : prep(prep_norm_kernel<1, false>, prep_split_kernel<1, false>));
     if (rc) return rc;
-    return d > 1024 ? run_steps<2>(L, ws, S.rows, S.cols, K, steps, st) : run_steps<1>(L, ws, S.rows, S.cols, K, steps, st);
+    return run_steps(L, ws, S.rows, S.cols, K, steps, st);
 }
 
 ctk_status check_common(const char* who, int64_t rows, int64_t cols, int steps, float eps, const void* workspace) {
