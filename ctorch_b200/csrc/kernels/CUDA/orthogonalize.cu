@@ -852,7 +852,7 @@ __global__ void __launch_bounds__(CL_THREADS, 1) ns_cluster_kernel(const Cluster
         *reinterpret_cast<uint4*>(X + cl_chunk(i, c)) = hi;
         *reinterpret_cast<uint4*>(X + 2 * CL_GROUP + cl_chunk(i, c)) = lo;
     }
-    asm volatile("fence.proxy.async;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     fence_before();
     __syncthreads();
     fence_after();
@@ -867,7 +867,7 @@ __global__ void __launch_bounds__(CL_THREADS, 1) ns_cluster_kernel(const Cluster
     auto product = [&](uint32_t a, uint32_t b, bool b_mn, int n, int kk) {
         if (tid != 0) return;
         fence_after();
-        asm volatile("fence.proxy.async;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         const uint32_t idesc = make_idesc(128, 0, false, b_mn) | (static_cast<uint32_t>(n >> 3) << 17);
         // (descriptors hold addresses in units of 16 bytes: every step is an addition of a constant)
         constexpr uint64_t LO = (2 * CL_GROUP) >> 4, GROUP = CL_GROUP >> 4, K16 = 32 >> 4, K16_MN = 2048 >> 4;
@@ -946,7 +946,7 @@ __global__ void __launch_bounds__(CL_THREADS, 1) ns_cluster_kernel(const Cluster
             }
         }
         if (ctas == 1) {
-            asm volatile("fence.proxy.async;" ::: "memory");
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             fence_before();
             __syncthreads();
         } else {
@@ -1007,7 +1007,7 @@ __global__ void __launch_bounds__(CL_THREADS, 1) ns_cluster_kernel(const Cluster
                 *chunk_of(A, q, 1) = lo;
             }
         }
-        asm volatile("fence.proxy.async;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         fence_before();
         __syncthreads();
 
@@ -1033,7 +1033,7 @@ __global__ void __launch_bounds__(CL_THREADS, 1) ns_cluster_kernel(const Cluster
                 }
             }
         }
-        asm volatile("fence.proxy.async;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         fence_before();
         __syncthreads();
     }

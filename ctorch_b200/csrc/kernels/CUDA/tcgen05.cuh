@@ -1,4 +1,4 @@
-// PTX of the tcgen05 / TMA / mbarrier instructions that the orthogonalisation kernels use, fp16 operands.
+// PTX of the tcgen05 / TMA / mbarrier instructions that the orthogonalisation and the 4-bit kernels use.
 #pragma once
 #include <cuda.h>
 #include <cuda_fp16.h>
@@ -116,6 +116,22 @@ __device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t a_desc, uint64
             "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
             ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
 }
+// 8-bit operands, K = 32 per instruction, one CTA
+__device__ __forceinline__ void mma_f8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    __syncwarp();
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr) : "memory");
+}
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
     __syncwarp();
     asm volatile(
@@ -132,7 +148,8 @@ __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.
 
 // Shared-memory matrix descriptor (sm_100 format) of an fp16 tile under the 128-byte swizzle (code 2): start address
 // >> 4 in bits [0,14), leading byte offset >> 4 in [16,30), stride byte offset >> 4 in [32,46), version 1 in [46,48).
-//   K-major  [rows][64 of k] = 128-byte rows, 8-row groups 1024 B apart (SBO); a K=16 step advances the start by 32 B.
+//   K-major  [rows][64 of k] = 128-byte rows, 8-row groups 1024 B apart (SBO); a K=16 step advances the start by 32 B
+//            (8-bit elements: 128 of k in a row, K=32 a step).
 //   MN-major [k][64 of M/N] in 64-wide column groups: 8 k-rows (1024 B) form one atom (SBO), column groups are LBO
 //            bytes apart; a K=16 step advances the start by 2048 B.
 __device__ __forceinline__ uint64_t make_desc(uint32_t smem_addr, uint32_t lbo_bytes) {
@@ -144,7 +161,7 @@ __device__ __forceinline__ uint64_t make_desc(uint32_t smem_addr, uint32_t lbo_b
     d |= static_cast<uint64_t>(2) << 61;
     return d;
 }
-// Instruction descriptor of kind::f16 with fp16 operands (format 0) and fp32 accumulation: major-ness in bits 15/16
+// Instruction descriptor of kind::f16 with fp16 operands, or of kind::f8f6f4 with e4m3 operands (format 0 in both), and fp32 accumulation: major-ness in bits 15/16
 // (1 = MN-major), N >> 3 in [17,23), M >> 4 in [24,29).
 __host__ __device__ constexpr uint32_t make_idesc(int m, int n, bool a_mn, bool b_mn) {
     return (1u << 4) | (static_cast<uint32_t>(a_mn) << 15) | (static_cast<uint32_t>(b_mn) << 16) | (static_cast<uint32_t>(n >> 3) << 17) |

@@ -1,8 +1,6 @@
 // 4-bit weights with group scales: quantising, the values they stand for, and y = [relu](x W + bias).
 // The layout is described in ctorch_b200.h.
-#include <cuda_bf16.h>
-
-#include "common.cuh"
+#include "tcgen05.cuh"
 
 namespace {
 using namespace ctk;
@@ -102,28 +100,53 @@ __global__ void __launch_bounds__(W4_THREADS) w4_dequantize_kernel(const uint32_
 }
 
 // ---- y = [relu](x W + bias) ------------------------------------------------------------------------------
-// mma.sync on exact factors.  A code minus its zero point is an integer of at most 4 bits and a sign, exact in bf16; x is cut
-// into three bf16 parts of 8 bits that add up to it exactly (by truncation: no part overflows); the products are
-// exact and meet in fp32.  Within a group the tensor core adds (8 instructions at most), the group's sum is scaled and
-// added to the result with one rounded fma: fp32 accuracy with no conversion of the weight but the mask that puts two codes
-// beside each other under bf16's exponent (0x4300 | code = 128 + code) and one packed subtraction.
+// tcgen05 on whole numbers.  A code of 0..15 in a byte IS an e4m3 number: 0..7 are its subnormals, 8..15 its first
+// normals, and both count in steps of 2^-9, so the weight's operand is made by two masks and a shift per eight codes.  x is
+// taken in fixed point: 31 bits below the largest |x| of its row's 128 neighbours, as eight signed digits base 16, and
+// a digit of -8..8 in sign and magnitude is an e4m3 number of the same kind.  So each (row, digit) is a column of the
+// instruction's B, every product and every sum of a group is a whole number below 2^24 times 2^-18 -- exact in the fp32
+// accumulator whatever it does -- and so is the zero point's share, zero * (sum of the digits).  What rounds: x to its 31 bits,
+// eight digits joined in fp32, one fma per group with the scale.
 //
-// The weight is the instruction's A (16 output columns by 16 k), the parts of x its B: eight columns, (row, part) pairs, so one
-// instruction serves two rows and NT of them 8 NT / 3.  k may be taken in any order as long as A and B agree: thread t of a
-// quad holds GROUP / 32 whole words of a group, as they lie in memory.  For few rows the weight's bytes are the bound
-// (per 128 k of 16 columns: 1 KB, 72 instructions to unpack, 8 NT products), from NT = 3 on the products.
-//
-// A CTA: 8 warps of 16 columns each; a cluster of `split` CTAs shares the k of its columns.  x's parts lie in shared memory (XC k at a time), 16-byte pieces ordered so that a quad's four pieces are neighbours.
-constexpr int MM_THREADS = 256, MM_COLS = 128, R_PITCH = 132;
-template <int NT>
+// A first, small kernel writes x's digits (w4_digits_kernel: a warp per row and 128 k) block by block as the main kernel's
+// shared memory wants them.  A CTA of the main kernel takes 128 columns of W and, in blocks of 128 k, its share of k (a cluster
+// of `split` CTAs shares the whole):
+//   3 or 4      codes, a block each in turn: 16 bytes (32 codes) per load, a whole block ahead -- the first before x's digits
+//               are there --, masks, two 16-byte stores into the operand tile [128 columns][128 k] (128-byte rows, swizzled);
+//   1 warp      one bulk copy per block for x's digits, their sums and x's steps;
+//   1 warp      the products: one instruction per 32 k, an accumulator [128 columns][(row, digit)] per group;
+//   4 or 8      a thread per column: digits joined, zero point, scale, added to the column's results.
+// mma.sync with x cut into three bf16 parts, the form before this one, ran at about 32 clocks an instruction on this machine
+// and took 95 us for 4 x 16384 x 16384, 46 us for 64 x 4096 x 4096; this one LATER.
+constexpr int MM_COLS = 128, MM_BLOCK = 128;         // columns of a CTA, k of a block
+constexpr int MM_UNITS = MM_COLS * 4 / 32;           // 16-byte pieces of a block of codes per lane
+constexpr int R_PITCH = 132;
+
+template <int GROUP, int ROWS>
 struct MmCfg {
-    static constexpr int XC = NT == 1 ? 2048 : NT <= 3 ? 1024 : 512;  // k of x held at a time
-    static constexpr int PITCH = XC * 2 + 64;                         // bytes per (row, part): 4 pieces past a multiple of 8, no bank conflicts
-    static constexpr int X_BYTES = 8 * NT * PITCH;
-    static constexpr int R_BYTES = 8 * NT * R_PITCH * 4;                  // a CTA's sums, [(row, part)][column], in the same place afterwards
-    static constexpr int SMEM = X_BYTES > R_BYTES ? X_BYTES : R_BYTES;
-    static constexpr int ROWS = 8 * NT / 3;
+    static constexpr int N = 8 * ROWS;               // accumulator columns
+    static constexpr int GPB = MM_BLOCK / GROUP;     // groups of a block
+    static constexpr int STAGES = ROWS <= 8 ? 4 : 3;
+    static constexpr int ACCS = N <= 64 ? 4 : 2;     // accumulators in turn
+    static constexpr int TMEM_COLS = N * ACCS;       // 64 .. 512, a power of two
+    static constexpr int A_BYTES = MM_COLS * MM_BLOCK, B_BYTES = N * MM_BLOCK;
+    static constexpr int T_BYTES = (GPB * N + (ROWS < 4 ? 4 : ROWS)) * 4;  // sums of digits per (group, row, digit), x's step per row
+    static constexpr int X_BYTES = B_BYTES + T_BYTES;                      // a block of x as the first kernel leaves it
+    static constexpr int STAGE_BYTES = (A_BYTES + X_BYTES + 1023) / 1024 * 1024;
+    static constexpr int RING = STAGES * STAGE_BYTES, R_BYTES = ROWS * R_PITCH * 4;
+    static constexpr int SMEM = (RING > R_BYTES ? RING : R_BYTES) + 1024;
+    static constexpr int PER_SM = ROWS <= 16 ? 2 : 1;
+    static constexpr int DRAIN = ROWS <= 16 ? 4 : 8; // warps that take the accumulators: 4 per CTA's columns, or 8 with half of the rows each
+    static constexpr int MINE = ROWS * 4 / DRAIN;    // rows of such a warp
+    static constexpr int AHEAD = ROWS <= 4 ? 8 : ROWS <= 8 ? 4 : 2;  // groups whose scales are in flight
+    // Warps that unpack codes, each whole blocks: one per stage, so that a warp always fills the same stage and never waits for
+    // it more than one round ahead (a barrier's parity cannot tell two rounds from none).
+    static constexpr int FILL = STAGES;
+    static constexpr int THREADS = (DRAIN + 2 + FILL) * 32;
+    static_assert(X_BYTES % 16 == 0 && TMEM_COLS * PER_SM <= 512 && SMEM * PER_SM <= 225 * 1024, "");
 };
+
+__device__ int g_w4_status = 0;  // first bounded wait that ran out, else 0
 
 struct MmArgs {
     const float* x;
@@ -136,245 +159,327 @@ struct MmArgs {
     int64_t ldy;
     int64_t m, k, n, groups;
     int relu, split;
-    int vec_x;  // x can be read 16 bytes at a time
+    const uint8_t* image;  // x's digits, [row block][k block][X_BYTES]
 };
 
-__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-// codes (2p, 2p+1) of a word, minus the zero point: two bf16 integers
-__device__ __forceinline__ uint32_t pair_of(uint32_t word, int p, uint32_t zero2) {
-    const uint32_t biased = ((word >> (4 * p)) & 0x000F000Fu) | 0x43004300u;
-    const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&biased), *reinterpret_cast<const __nv_bfloat162*>(&zero2));
-    return *reinterpret_cast<const uint32_t*>(&d);
-}
-// x = p0 + p1 + p2 in bits 16-31 of the three: 8 leading bits each, truncated, so the sum is exact
-__device__ __forceinline__ void cut3(float x, uint32_t (&p)[3]) {
-    const uint32_t u = __float_as_uint(x);
-    if ((u & 0x7F800000u) == 0x7F800000u) {  // infinities stay, NaN stays NaN
-        p[0] = (u & 0x007FFFFFu) ? 0x7FC00000u : u;
-        p[1] = p[2] = 0u;
-        return;
+// x's digits.  A warp takes one row's 128 k of a block, lane l the k 4l .. 4l+3.  Rows past m give zeros.
+// The order of a word's codes in the operand's bytes: the masks leave the even nibbles, then the odd ones,
+// nibbles 0 2 4 6 = codes 0 4 1 5 and nibbles 1 3 5 7 = codes 2 6 3 7; x's digits are stored in that order.
+template <int GROUP, int ROWS>
+__global__ void __launch_bounds__(128) w4_digits_kernel(const float* __restrict__ x, int64_t ldx, int64_t m, int64_t k, int64_t k_blocks, uint8_t* __restrict__ image) {
+    using C = MmCfg<GROUP, ROWS>;
+    const int lane = threadIdx.x & 31;
+    const int64_t block = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+    const int row_block = blockIdx.y / ROWS, r = blockIdx.y % ROWS;
+    const int64_t row = blockIdx.y, k0 = block * MM_BLOCK + lane * 4;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (the main kernel starts with what does not depend on this one)
+    if (block >= k_blocks) return;
+    uint8_t* const out = image + (row_block * k_blocks + block) * C::X_BYTES;
+    float* const sums = reinterpret_cast<float*>(out + C::B_BYTES);
+    float v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = row < m && k0 + e < k ? __ldg(x + row * ldx + k0 + e) : 0.0f;
+    // the largest exponent (as bits, so that an infinity or a NaN wins)
+    uint32_t top = max(max(__float_as_uint(v[0]) & 0x7FFFFFFFu, __float_as_uint(v[1]) & 0x7FFFFFFFu), max(__float_as_uint(v[2]) & 0x7FFFFFFFu, __float_as_uint(v[3]) & 0x7FFFFFFFu));
+    top = __reduce_max_sync(0xffffffffu, top);
+    int ex = static_cast<int>(top >> 23);  // |v| < 2^(ex - 126)
+    const bool bad = ex == 255;
+    ex = max(ex, 31);                      // (that far down x has fewer bits anyway)
+    const float up = __uint_as_float(static_cast<uint32_t>(127 + 156 - ex) << 23);  // |v| 2^(156 - ex) < 2^30
+    uint32_t digits[4];                    // eight nibbles each, 8 too large
+#pragma unroll
+    for (int e = 0; e < 4; ++e) digits[e] = static_cast<uint32_t>(__float2int_rn(bad ? 0.0f : v[e] * up)) + 0x88888888u;
+    // four bytes of digit d: sign and magnitude of nibble - 8; this lane's four k are codes 0..3 (even lanes) or 4..7 of a word
+#pragma unroll
+    for (int d = 0; d < 8; ++d) {
+        uint32_t four = 0;
+        int sum = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int g = static_cast<int>((digits[e] >> (4 * d)) & 15u) - 8;
+            sum += g;
+            four |= (g < 0 ? static_cast<uint32_t>(0x80 - g) : static_cast<uint32_t>(g)) << (8 * e);
+        }
+        const uint32_t other = __shfl_xor_sync(0xffffffffu, four, 1);
+        const uint32_t first = lane & 1 ? other : four, second = lane & 1 ? four : other;
+        const uint32_t bytes = lane & 1 ? __byte_perm(first, second, 0x7362) : __byte_perm(first, second, 0x5140);
+        const int col = r * 8 + d;
+        *reinterpret_cast<uint32_t*>(out + col * 128 + (((lane >> 2) ^ (col & 7)) << 4) + (lane & 3) * 4) = bytes;
+#pragma unroll
+        for (int s = 1; s < GROUP / 4; s <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);  // of the group's lanes
+        if (lane % (GROUP / 4) == 0) sums[(lane / (GROUP / 4)) * C::N + col] = static_cast<float>(sum) * (1.0f / 262144.0f);
     }
-    p[0] = u & 0xFFFF0000u;
-    const float r = x - __uint_as_float(p[0]);
-    p[1] = __float_as_uint(r) & 0xFFFF0000u;
-    p[2] = __float_as_uint(r - __uint_as_float(p[1]));
+    // what one unit of digit 0 stands for, times 2^18
+    if (lane == 0) sums[C::GPB * C::N + r] = __uint_as_float(bad ? 0x7FC00000u : static_cast<uint32_t>(127 + ex - 156 + 18) << 23);
 }
 
-template <int GROUP>
-struct Words;
-template <>
-struct Words<32> { uint32_t w[1]; };
-template <>
-struct __align__(8) Words<64> { uint32_t w[2]; };
-template <>
-struct __align__(16) Words<128> { uint32_t w[4]; };
-
-template <int GROUP>
-__device__ __forceinline__ Words<GROUP> load_words(const uint32_t* p) {
-    Words<GROUP> r;
-    if (GROUP == 32) {
-        r.w[0] = __ldg(p);
-    } else if (GROUP == 64) {
-        *reinterpret_cast<uint2*>(&r) = __ldg(reinterpret_cast<const uint2*>(p));
-    } else {
-        *reinterpret_cast<uint4*>(&r) = __ldg(reinterpret_cast<const uint4*>(p));
-    }
-    return r;
-}
-
-template <int GROUP, int NT>
-__global__ void __launch_bounds__(MM_THREADS, 2) w4_matmul_kernel(const MmArgs P) {
-    using C = MmCfg<NT>;
-    constexpr int W = GROUP / 32;             // words of a group per thread of a quad
-    constexpr int AHEAD = GROUP == 32 ? 8 : 4;  // groups whose words are in flight
-    extern __shared__ __align__(16) uint8_t smem[];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gr = lane >> 2, qt = lane & 3;
+template <int GROUP, int ROWS>
+__global__ void __launch_bounds__((MmCfg<GROUP, ROWS>::THREADS), (MmCfg<GROUP, ROWS>::PER_SM)) w4_matmul_kernel(const MmArgs P) {
+    using namespace t5;
+    using C = MmCfg<GROUP, ROWS>;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint64_t bars[2 * C::STAGES + 2 * C::ACCS];
+    __shared__ uint32_t tmem_slot;
+    __shared__ volatile int abort_flag;
+    uint8_t* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    const uint32_t bar0 = smem_u32(bars), base = smem_u32(smem);
+    auto full_bar = [&](int s) { return bar0 + 8u * s; };
+    auto empty_bar = [&](int s) { return bar0 + 8u * (C::STAGES + s); };
+    auto afull_bar = [&](int a) { return bar0 + 8u * (2 * C::STAGES + a); };
+    auto aempty_bar = [&](int a) { return bar0 + 8u * (2 * C::STAGES + C::ACCS + a); };
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int split = P.split, rank = blockIdx.x % split;
-    const int64_t col_base = static_cast<int64_t>(blockIdx.x / split) * MM_COLS, row_base = static_cast<int64_t>(blockIdx.y) * C::ROWS;
-    const int rows = static_cast<int>(P.m - row_base < C::ROWS ? P.m - row_base : C::ROWS);
-    // this CTA's groups, taken XC / GROUP at a time
-    const int g_begin = static_cast<int>(P.groups * rank / split), g_end = static_cast<int>(P.groups * (rank + 1) / split);
-    constexpr int PIECE = C::XC / GROUP;
-    static_assert(PIECE % AHEAD == 0, "a piece starts at held[0]");
-    const bool idle = col_base + warp * 16 >= P.n;  // this warp has no columns: it only helps with x
+    const int64_t col_base = static_cast<int64_t>(blockIdx.x / split) * MM_COLS, row_base = static_cast<int64_t>(blockIdx.y) * ROWS;
+    const int rows = static_cast<int>(P.m - row_base < ROWS ? P.m - row_base : ROWS);
+    const int64_t all_blocks = (P.groups + C::GPB - 1) / C::GPB;
+    const int64_t b_begin = all_blocks * rank / split;
+    const int blocks = static_cast<int>(all_blocks * (rank + 1) / split - b_begin);  // of 128 k, this CTA's
 
-    const int64_t j0 = col_base + warp * 16 + gr, j1 = j0 + 8;  // this thread's two output columns
-    const int64_t c0 = j0 < P.n ? j0 : P.n - 1, c1 = j1 < P.n ? j1 : P.n - 1;  // (past the end: any column that exists)
-    const uint32_t* w0 = P.packed + c0 * (P.groups * (GROUP / 8)) + qt * W;
-    const uint32_t* w1 = P.packed + c1 * (P.groups * (GROUP / 8)) + qt * W;
-    const float *s0 = P.scales + c0 * P.groups, *s1 = P.scales + c1 * P.groups;
-    const uint8_t *z0 = P.zeros ? P.zeros + c0 * P.groups : nullptr, *z1 = P.zeros ? P.zeros + c1 * P.groups : nullptr;
+    if (tid == 0) {
+        abort_flag = 0;
+        for (int s = 0; s < C::STAGES; ++s) { mbar_init(full_bar(s), 2); mbar_init(empty_bar(s), 1 + C::DRAIN); }
+        for (int a = 0; a < C::ACCS; ++a) { mbar_init(afull_bar(a), 1); mbar_init(aempty_bar(a), C::DRAIN); }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == C::DRAIN) tmem_alloc<1>(smem_u32(&tmem_slot), C::TMEM_COLS);
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = tmem_slot;
 
-    float total[NT][4];
+    float result[C::MINE];
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) total[t][i] = 0.0f;
+    for (int r = 0; r < C::MINE; ++r) result[r] = 0.0f;
 
-    struct Held {
-        Words<GROUP> a, b;
-        float sa, sb;
-        uint32_t za, zb;
-    } held[AHEAD];
-    auto fetch = [&](Held& h, int g) {
-        if (g >= g_end || idle) return;
-        h.a = load_words<GROUP>(w0 + static_cast<int64_t>(g) * (GROUP / 8));
-        h.b = load_words<GROUP>(w1 + static_cast<int64_t>(g) * (GROUP / 8));
-        h.sa = __ldg(s0 + g);
-        h.sb = __ldg(s1 + g);
-        h.za = z0 ? __ldg(z0 + g) : 8u;
-        h.zb = z1 ? __ldg(z1 + g) : 8u;
-    };
+    if (warp >= C::DRAIN + 2) {
+        // ------------------------------ codes ------------------------------
+        const int fw = warp - (C::DRAIN + 2), q = lane & 3;  // blocks fw, fw + FILL, ..; 16-byte piece q of columns lane / 4, lane / 4 + 8, ..
+        const int64_t row_words = P.groups * (GROUP / 8);    // words of one column
+        // (a last block may hold fewer than 128 k: its missing groups are not read)
+        const int64_t whole = (row_words - q * 4 + MM_BLOCK / 8 - 1) / (MM_BLOCK / 8) - b_begin;
+        const int my_blocks = blocks < whole ? blocks : static_cast<int>(whole);
+        const uint32_t* const src = P.packed + b_begin * (MM_BLOCK / 8) + q * 4;
+        const uint32_t dst = static_cast<uint32_t>((lane >> 2) * 128 + (((2 * q) ^ (lane >> 2)) << 4));  // the first 16 of its 32 bytes
+        uint4 held[MM_UNITS];
+        auto fetch = [&](int u, int b) {
+            // a column past the end is replaced by one that exists, its results are dropped
+            const int64_t c = col_base + (lane >> 2) + u * 8;
+            if (b < my_blocks)
+                asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(held[u].x), "=r"(held[u].y), "=r"(held[u].z), "=r"(held[u].w)
+                             : "l"(src + (c < P.n ? c : P.n - 1) * row_words + static_cast<int64_t>(b) * (MM_BLOCK / 8)));
+            else held[u] = make_uint4(0u, 0u, 0u, 0u);
+        };
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) fetch(held[i], g_begin + i);
-
-    for (int p0 = g_begin; p0 < g_end; p0 += PIECE) {
-        const int p1 = p0 + PIECE < g_end ? p0 + PIECE : g_end;
-        if (p0 != g_begin) __syncthreads();  // the piece before has been read
-        // ---- x's parts: eight k of one row a thread, into the three columns of that row ----
-        const int pieces = (p1 - p0) * (GROUP / 8);
-        for (int t = tid; t < rows * pieces; t += MM_THREADS) {
-            const int r = t / pieces, q = t - r * pieces;
-            const int64_t k0 = static_cast<int64_t>(p0) * GROUP + q * 8;
-            const float* src = P.x + (row_base + r) * P.ldx + k0;
-            float v[8];
-            if (P.vec_x && k0 + 8 <= P.k) {
-                *reinterpret_cast<float4*>(v) = __ldg(reinterpret_cast<const float4*>(src));
-                *reinterpret_cast<float4*>(v + 4) = __ldg(reinterpret_cast<const float4*>(src) + 1);
-            } else {
+        for (int u = 0; u < MM_UNITS; ++u) fetch(u, fw);
+        for (int b = fw; b < blocks; b += C::FILL) {
+            const int st = b % C::STAGES;
+            if (!mbar_wait(empty_bar(st), ((b / C::STAGES) & 1) ^ 1u, &abort_flag, &g_w4_status, 0x100 | st)) break;
+            uint8_t* to = smem + st * C::STAGE_BYTES + dst;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = k0 + e < P.k ? __ldg(src + e) : 0.0f;
+            for (int u = 0; u < MM_UNITS; ++u) {
+                const uint4 w = held[u];
+                constexpr uint32_t M = 0x0F0F0F0Fu;
+                *reinterpret_cast<uint4*>(to + u * 1024) = make_uint4(w.x & M, (w.x >> 4) & M, w.y & M, (w.y >> 4) & M);
+                *reinterpret_cast<uint4*>(smem + st * C::STAGE_BYTES + (dst ^ 16u) + u * 1024) = make_uint4(w.z & M, (w.z >> 4) & M, w.w & M, (w.w >> 4) & M);
+                fetch(u, b + C::FILL);
             }
-            uint4 out[3];
-            uint32_t* o[3] = {&out[0].x, &out[1].x, &out[2].x};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                uint32_t a[3], b[3];
-                cut3(v[2 * e], a);
-                cut3(v[2 * e + 1], b);
-#pragma unroll
-                for (int part = 0; part < 3; ++part) o[part][e] = __byte_perm(a[part], b[part], 0x7632);
-            }
-            const int in = q % (GROUP / 8), at = (q - in) + (in % W) * 4 + in / W;  // piece (thread in / W, word in % W) of its group
-#pragma unroll
-            for (int part = 0; part < 3; ++part) *reinterpret_cast<uint4*>(smem + (r * 3 + part) * C::PITCH + at * 16) = out[part];
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(full_bar(st));
         }
-        __syncthreads();
-        // ---- the piece's groups ----
-        for (int g0 = p0; g0 < p1 && !idle; g0 += AHEAD) {
+    } else if (warp == C::DRAIN + 1) {
+        // ------------------------------ x ------------------------------
+        if (lane == 0) {
+            asm volatile("griddepcontrol.wait;" ::: "memory");  // x's digits are there
+            const uint8_t* from = P.image + (blockIdx.y * all_blocks + b_begin) * C::X_BYTES;
+            for (int b = 0; b < blocks; ++b) {
+                const int st = b % C::STAGES;
+                if (!mbar_wait(empty_bar(st), ((b / C::STAGES) & 1) ^ 1u, &abort_flag, &g_w4_status, 0x180 | st)) break;
+                mbar_expect_tx(full_bar(st), C::X_BYTES);
+                asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                             ::"r"(base + st * C::STAGE_BYTES + C::A_BYTES), "l"(from + static_cast<int64_t>(b) * C::X_BYTES), "r"(static_cast<uint32_t>(C::X_BYTES)), "r"(full_bar(st)) : "memory");
+            }
+        }
+    } else if (warp == C::DRAIN) {
+        // ------------------------------ products ------------------------------
+        if (lane == 0) {
+            constexpr uint32_t idesc = make_idesc(MM_COLS, C::N, false, false);
+            int acc = 0;
+            uint32_t acc_phase = 0;
+            bool ok = true;
+            for (int b = 0; b < blocks && ok; ++b) {
+                const int st = b % C::STAGES;
+                if (!mbar_wait(full_bar(st), (b / C::STAGES) & 1, &abort_flag, &g_w4_status, 0x200 | st)) break;
+                const uint64_t a = make_desc(base + st * C::STAGE_BYTES, 0), x = make_desc(base + st * C::STAGE_BYTES + C::A_BYTES, 0);
+                const int64_t left = P.groups - (b_begin + b) * C::GPB;
+                for (int g = 0; g < C::GPB && g < left; ++g) {
+                    if (!mbar_wait(aempty_bar(acc), acc_phase ^ 1u, &abort_flag, &g_w4_status, 0x210 | acc)) { ok = false; break; }
+                    fence_after();
 #pragma unroll
-            for (int i = 0; i < AHEAD; ++i) {
-                const int g = g0 + i;
-                if (g >= p1) break;
-                const Held h = held[i];
-                fetch(held[i], g + AHEAD);
-                const uint32_t za = 0x43004300u | h.za | (h.za << 16), zb = 0x43004300u | h.zb | (h.zb << 16);
-                float sum[NT][4];
+                    for (int ks = 0; ks < GROUP / 32; ++ks) mma_f8(tmem + acc * C::N, a + (g * (GROUP / 32) + ks) * 2, x + (g * (GROUP / 32) + ks) * 2, idesc, ks > 0);
+                    commit<1>(afull_bar(acc));
+                    if (++acc == C::ACCS) { acc = 0; acc_phase ^= 1u; }
+                }
+                if (ok) commit<1>(empty_bar(st));
+            }
+        }
+    } else {
+        // ------------------------------ results ------------------------------
+        const int quarter = warp & 3, r_first = (warp >> 2) * C::MINE;  // columns of the tile, rows of x
+        const int64_t col = col_base + quarter * 32 + lane, at = (col < P.n ? col : P.n - 1) * P.groups + b_begin * C::GPB;
+        const uint32_t t_row = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + r_first * 8;
+        const int64_t left = P.groups - b_begin * C::GPB;
+        const int groups = static_cast<int>(left < static_cast<int64_t>(blocks) * C::GPB ? left : static_cast<int64_t>(blocks) * C::GPB);
+        // scales and zero points, each lane its own row of them, AHEAD groups in flight: a load's latency is several groups long
+        float scale[C::AHEAD];
+        uint32_t zero[C::AHEAD];
+        auto fetch = [&](float& s, uint32_t& z, int g) {
+            s = g < groups ? __ldg(P.scales + at + g) : 0.0f;
+            z = g < groups && P.zeros ? __ldg(P.zeros + at + g) : 8u;
+        };
 #pragma unroll
-                for (int t = 0; t < NT; ++t)
+        for (int i = 0; i < C::AHEAD; ++i) fetch(scale[i], zero[i], i);
+        int acc = 0;
+        uint32_t acc_phase = 0;
+        bool ok = true;
+        for (int g0 = 0; g0 < groups && ok; g0 += C::AHEAD) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) sum[t][e] = 0.0f;
+            for (int i = 0; i < C::AHEAD; ++i) {
+                const int gi = g0 + i, b = gi / C::GPB, st = b % C::STAGES, g = gi % C::GPB;
+                if (gi >= groups || !ok) break;
+                const float* sums = reinterpret_cast<const float*>(smem + st * C::STAGE_BYTES + C::A_BYTES + C::B_BYTES);
+                const float* step = sums + C::GPB * C::N + r_first;
+                sums += g * C::N + r_first * 8;
+                if (g == 0 && !mbar_wait(full_bar(st), (b / C::STAGES) & 1, &abort_flag, &g_w4_status, 0x300 | st)) { ok = false; break; }
+                const float s = scale[i], z = -static_cast<float>(zero[i]);
+                fetch(scale[i], zero[i], gi + C::AHEAD);
+                if (!mbar_wait(afull_bar(acc), acc_phase, &abort_flag, &g_w4_status, 0x310 | acc)) { ok = false; break; }
+                fence_after();
+                // two rows at a time, the next two on their way while these are joined
+                uint32_t d[2][16];
+                tmem_ld16(t_row + acc * C::N, d[0]);
 #pragma unroll
-                for (int w = 0; w < W; ++w) {
-                    uint32_t a[4], b[4];
+                for (int r0 = 0; r0 < C::MINE; r0 += 2) {
+                    constexpr int LAST = C::MINE - 2;
+                    float ds[2][8], up[2];
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        a[q] = pair_of(h.a.w[w], q, za);
-                        b[q] = pair_of(h.b.w[w], q, zb);
+                    for (int r = 0; r < 2; ++r) {
+                        *reinterpret_cast<float4*>(ds[r]) = *reinterpret_cast<const float4*>(sums + (r0 + r) * 8);
+                        *reinterpret_cast<float4*>(ds[r] + 4) = *reinterpret_cast<const float4*>(sums + (r0 + r) * 8 + 4);
+                        up[r] = step[r0 + r] * s;
                     }
-                    const uint8_t* xs = smem + gr * C::PITCH + ((g - p0) * (GROUP / 8) + w * 4 + qt) * 16;
+                    tmem_ld_wait();
+                    if (r0 < LAST) {
+                        tmem_ld16(t_row + acc * C::N + (r0 + 2) * 8, d[((r0 >> 1) + 1) & 1]);
+                    } else {  // read completely
+                        fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(aempty_bar(acc));
+                    }
 #pragma unroll
-                    for (int t = 0; t < NT; ++t) {
-                        const uint4 xv = *reinterpret_cast<const uint4*>(xs + t * 8 * C::PITCH);
-                        mma_bf16(sum[t], a[0], b[0], a[1], b[1], xv.x, xv.y);
-                        mma_bf16(sum[t], a[2], b[2], a[3], b[3], xv.z, xv.w);
+                    for (int r = 0; r < 2; ++r) {
+                        float w[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) w[e] = fmaf(z, ds[r][e], __uint_as_float(d[(r0 >> 1) & 1][r * 8 + e]));
+                        // (pairs, then pairs of pairs: 256 and 65536 are exact factors, every level rounds once)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) w[e] = fmaf(w[2 * e + 1], 16.0f, w[2 * e]);
+                        w[0] = fmaf(w[1], 256.0f, w[0]);
+                        w[2] = fmaf(w[3], 256.0f, w[2]);
+                        result[r0 + r] = fmaf(fmaf(w[2], 65536.0f, w[0]), up[r], result[r0 + r]);
                     }
                 }
-#pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    total[t][0] = fmaf(h.sa, sum[t][0], total[t][0]);
-                    total[t][1] = fmaf(h.sa, sum[t][1], total[t][1]);
-                    total[t][2] = fmaf(h.sb, sum[t][2], total[t][2]);
-                    total[t][3] = fmaf(h.sb, sum[t][3], total[t][3]);
+                if (++acc == C::ACCS) { acc = 0; acc_phase ^= 1u; }
+                if (g == C::GPB - 1 || gi == groups - 1) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(empty_bar(st));
                 }
             }
         }
     }
 
-    // ---- the sums of the cluster's CTAs and of the three parts ----
+    // ---- the sums of the cluster's CTAs ----
+    fence_before();
+    __syncthreads();  // no operand is read any more
+    fence_after();
+    if (warp == C::DRAIN) tmem_dealloc<1>(tmem, C::TMEM_COLS);
     float* const R = reinterpret_cast<float*>(smem);
-    __syncthreads();  // x has been read
-    if (!idle) {
+    if (warp < C::DRAIN) {
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) R[(t * 8 + qt * 2 + (i & 1)) * R_PITCH + warp * 16 + gr + (i >> 1) * 8] = total[t][i];
+        for (int r = 0; r < C::MINE; ++r) R[((warp >> 2) * C::MINE + r) * R_PITCH + (warp & 3) * 32 + lane] = result[r];
     }
-    if (split > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (split > 1) cluster_sync_all();
     else __syncthreads();
     const int outs = rows * MM_COLS;
-    for (int t = rank * MM_THREADS + tid; t < outs; t += split * MM_THREADS) {
+    for (int t = rank * C::THREADS + tid; t < outs; t += split * C::THREADS) {
         const int r = t / MM_COLS, c = t % MM_COLS;
         if (col_base + c >= P.n) continue;
         float v = 0.0f;
-        const uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(R + r * 3 * R_PITCH + c));
-        for (int q = 0; q < split; ++q) {
-            float p[3];
+        if (split > 1) {
+            const uint32_t from = smem_u32(R + r * R_PITCH + c);
+            float p[8];
 #pragma unroll
-            for (int part = 0; part < 3; ++part) {
-                if (split > 1) {
-                    uint32_t from;
-                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(from) : "r"(at + part * R_PITCH * 4), "r"(q));
-                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(p[part]) : "r"(from) : "memory");
-                } else {
-                    p[part] = R[(r * 3 + part) * R_PITCH + c];
-                }
-            }
-            v += p[0] + (p[1] + p[2]);
+            for (int s = 0; s < 8; ++s)
+                if (s < split) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(p[s]) : "r"(map_to_cta(from, static_cast<uint32_t>(s))) : "memory");
+#pragma unroll
+            for (int s = 0; s < 8; ++s)
+                if (s < split) v += p[s];
+        } else {
+            v = R[r * R_PITCH + c];
         }
         if (P.bias) v += __ldg(P.bias + col_base + c);
         if (P.relu) v = v > 0.0f ? v : 0.0f;
         P.y[(row_base + r) * P.ldy + col_base + c] = v;
     }
-    if (split > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");  // the peers have read this CTA's sums
+    if (split > 1) cluster_sync_all();  // the peers have read this CTA's sums
 }
 
-template <int GROUP, int NT>
+template <int GROUP, int ROWS>
 ctk_status launch_matmul(MmArgs P, cudaStream_t st) {
-    using C = MmCfg<NT>;
-    auto kernel = w4_matmul_kernel<GROUP, NT>;
+    using C = MmCfg<GROUP, ROWS>;
+    auto kernel = w4_matmul_kernel<GROUP, ROWS>;
     static ctk::PerDeviceOnce attr_set;
     if (attr_set.first()) CTK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
-    const int64_t blocks = (P.n + MM_COLS - 1) / MM_COLS, row_blocks = (P.m + C::ROWS - 1) / C::ROWS;
-    // split k over a cluster while that fills idle SMs and leaves a CTA two groups
+    const int64_t col_blocks = (P.n + MM_COLS - 1) / MM_COLS, row_blocks = (P.m + ROWS - 1) / ROWS, k_blocks = (P.groups + C::GPB - 1) / C::GPB;
+    // split k over a cluster while that fills idle SMs and leaves a CTA two blocks
     P.split = 1;
-    while (P.split < 8 && blocks * row_blocks * P.split * 2 <= 3 * ctk::sm_count() && P.groups >= P.split * 4) P.split *= 2;
-    if (blocks * P.split > 0x7FFFFFFF || row_blocks > 65535) return fail(CTK_ERR_LIMIT, "ctk_w4_matmul_f32: too many rows or columns");
+    while (P.split < 8 && col_blocks * row_blocks * P.split * 2 <= 3 * ctk::sm_count() && k_blocks >= P.split * 4) P.split *= 2;
+    if (col_blocks * P.split > 0x7FFFFFFF || row_blocks * ROWS > 65535) return fail(CTK_ERR_LIMIT, "ctk_w4_matmul_f32: too many rows or columns");
+    StreamScratch scratch;
+    if (k_blocks) {
+        ctk_status rc = scratch.get(static_cast<size_t>(row_blocks * k_blocks) * C::X_BYTES, st);
+        if (rc) return rc;
+        uint8_t* image = static_cast<uint8_t*>(scratch.p);
+        P.image = image;
+        w4_digits_kernel<GROUP, ROWS><<<dim3(static_cast<unsigned>((k_blocks + 3) / 4), static_cast<unsigned>(row_blocks * ROWS)), 128, 0, st>>>(P.x, P.ldx, P.m, P.k, k_blocks, image);
+        CTK_LAUNCH_CHECK("w4_digits");
+    }
     cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = static_cast<unsigned>(P.split);
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
-    cfg.gridDim = dim3(static_cast<unsigned>(blocks * P.split), static_cast<unsigned>(row_blocks));
-    cfg.blockDim = dim3(MM_THREADS);
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // may start before the digits are written, up to its griddepcontrol.wait
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3(static_cast<unsigned>(col_blocks * P.split), static_cast<unsigned>(row_blocks));
+    cfg.blockDim = dim3(C::THREADS);
     cfg.dynamicSmemBytes = C::SMEM;
     cfg.stream = st;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = k_blocks ? 2 : 1;  // (without k there is nothing in front of it to wait for in the kernel)
     CTK_CUDA(cudaLaunchKernelEx(&cfg, kernel, P));
     CTK_LAUNCH_CHECK("w4_matmul");
     return CTK_OK;
 }
 template <int GROUP>
 ctk_status matmul_rows(const MmArgs& P, cudaStream_t st) {
-    if (P.m <= MmCfg<1>::ROWS) return launch_matmul<GROUP, 1>(P, st);
-    if (P.m <= MmCfg<2>::ROWS) return launch_matmul<GROUP, 2>(P, st);
-    if (P.m <= MmCfg<3>::ROWS) return launch_matmul<GROUP, 3>(P, st);
-    return launch_matmul<GROUP, 6>(P, st);
+    if (P.m <= 2) return launch_matmul<GROUP, 2>(P, st);
+    if (P.m <= 4) return launch_matmul<GROUP, 4>(P, st);
+    if (P.m <= 8) return launch_matmul<GROUP, 8>(P, st);
+    if (P.m <= 16) return launch_matmul<GROUP, 16>(P, st);
+    return launch_matmul<GROUP, 32>(P, st);
 }
 
 bool group_ok(int group) { return group == 32 || group == 64 || group == 128; }
@@ -454,7 +559,6 @@ ctk_status ctk_w4_matmul_f32(const float* x, int64_t ldx, const uint32_t* packed
     P.n = n;
     P.groups = (k + group - 1) / group;
     P.relu = relu;
-    P.vec_x = ldx % 4 == 0 && aligned_to(x, 16);
     cudaStream_t st = as_stream(stream);
     return group == 32 ? matmul_rows<32>(P, st) : group == 64 ? matmul_rows<64>(P, st) : matmul_rows<128>(P, st);
 }

@@ -203,3 +203,28 @@ def test_matmul_w4_streams_and_replay(cb, m):
         cb.check(cb.lib.ctk_graph_launch(exe, s.handle, 0))
         assert np.array_equal(y.numpy(stream=s), ref)
     cb.check(cb.lib.ctk_graph_destroy(exe))
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("m", [1, 3, 7, 12, 30])
+def test_matmul_w4_whole_numbers_are_exact(cb, m, group):
+    """Whole-number x, scales of 1: every sum stays below 2^24, so nothing may round."""
+    rng = np.random.default_rng(m + group)
+    k, n = 1000, 200
+    w4, _ = random_weight(cb, rng, k, n, group, False)
+    w4.scales.copy_from_host(np.ones((n, -(-k // group)), np.float32))
+    w = values64(w4.packed.numpy(), w4.scales.numpy(), w4.zeros.numpy(), k, group)
+    x = rng.integers(-999, 1000, (m, k)).astype(np.float32)
+    assert (np.abs(x.astype(np.float64)) @ np.abs(w)).max() < 2 ** 24
+    assert np.array_equal(cb.ops.matmul_w4(cb.to_device(x), w4).numpy(), x.astype(np.float64) @ w)
+
+
+def test_matmul_w4_one_row_of_many_sizes(cb):
+    """A row with elements of very different sizes: each block of 128 k is taken to 31 bits below its largest."""
+    rng = np.random.default_rng(55)
+    k, n = 512, 70
+    w4, w = random_weight(cb, rng, k, n, 64, False)
+    x = (rng.standard_normal((2, k)) * 10.0 ** rng.integers(-6, 6, (2, k))).astype(np.float32)
+    largest = np.abs(x).reshape(2, -1, 128).max(-1).repeat(128, axis=1).astype(np.float64)
+    bound = (64 + 8 + 40) * 2.0 ** -23 * (np.abs(x).astype(np.float64) @ np.abs(w)) + 2.0 ** -31 * (largest @ np.abs(w))
+    assert (np.abs(cb.ops.matmul_w4(cb.to_device(x), w4).numpy() - x.astype(np.float64) @ w) <= bound).all()
