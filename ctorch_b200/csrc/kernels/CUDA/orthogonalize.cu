@@ -16,8 +16,6 @@
 // at a time; the epilogue warps add those up in registers with rounding.
 #include <math.h>
 
-#include <mutex>
-
 #include "tcgen05.cuh"
 
 namespace {
@@ -407,11 +405,12 @@ __global__ void __launch_bounds__(THREADS, 1) ns_product_kernel(const __grid_con
             }
         }
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
+        if (rank == 0) {
             constexpr uint32_t idesc = make_idesc(BM * GROUP, BN, A_MN, B_MN);
             // hi and lo of a K-major tile lie half an operand apart; of an MN-major one a quarter, inside each column group
-            constexpr uint32_t a_lo = A_MN ? STAGE_BYTES / 8 : STAGE_BYTES / 4, b_lo = B_MN ? STAGE_BYTES / 8 : STAGE_BYTES / 4;
-            constexpr uint32_t a_step = A_MN ? 2048u : 32u, b_step = B_MN ? 2048u : 32u;
+            // (descriptors hold addresses in units of 16 bytes: every step is an addition of a constant)
+            constexpr uint64_t a_lo = (A_MN ? STAGE_BYTES / 8 : STAGE_BYTES / 4) >> 4, b_lo = (B_MN ? STAGE_BYTES / 8 : STAGE_BYTES / 4) >> 4;
+            constexpr uint64_t a_step = (A_MN ? 2048u : 32u) >> 4, b_step = (B_MN ? 2048u : 32u) >> 4;
             constexpr uint32_t a_lbo = A_MN ? STAGE_BYTES / 4 : 0u, b_lbo = B_MN ? STAGE_BYTES / 4 : 0u;
             int stage = 0, acc = 0;
             uint32_t phase = 0, acc_phase = 0;
@@ -420,31 +419,29 @@ __global__ void __launch_bounds__(THREADS, 1) ns_product_kernel(const __grid_con
                 for (int c0 = 0; c0 < P.num_kb && ok; c0 += CHUNK_KB) {
                     const int c1 = c0 + CHUNK_KB < P.num_kb ? c0 + CHUNK_KB : P.num_kb;
                     if (!mbar_wait(tempty_bar(acc), acc_phase ^ 1u, &abort_flag, &g_ns_status, 0x200 | acc)) { ok = false; break; }
-                    fence_after();
                     const uint32_t d = tmem_base + static_cast<uint32_t>(acc * BN);
                     for (int kb = c0; kb < c1; ++kb) {
                         if (!mbar_wait(full_bar(stage), phase, &abort_flag, &g_ns_status, 0x210 | stage)) { ok = false; break; }
                         fence_after();
-                        const uint32_t a = smem_base + stage * STAGE_BYTES, b = a + STAGE_BYTES / 2;
-                        uint32_t more = kb == c0 ? 0u : 1u;
+                        const uint64_t a = make_desc(smem_base + stage * STAGE_BYTES, a_lbo), b = make_desc(smem_base + stage * STAGE_BYTES + STAGE_BYTES / 2, b_lbo);
+                        __syncwarp();
+                        if (elect_one()) {
 #pragma unroll
-                        for (int ks = 0; ks < BK / 16; ++ks) {  // the small terms first, while the accumulator is small
-                            mma_f16<GROUP>(d, make_desc(a + a_lo + ks * a_step, a_lbo), make_desc(b + ks * b_step, b_lbo), idesc, more);
-                            mma_f16<GROUP>(d, make_desc(a + ks * a_step, a_lbo), make_desc(b + b_lo + ks * b_step, b_lbo), idesc, 1u);
-                            more = 1u;
+                            for (int ks = 0; ks < BK / 16; ++ks) {  // the small terms first, while the accumulator is small
+                                mma_f16<GROUP>(d, a + a_lo + ks * a_step, b + ks * b_step, idesc, kb > c0 || ks > 0);
+                                mma_f16<GROUP>(d, a + ks * a_step, b + b_lo + ks * b_step, idesc, 1u);
+                            }
+#pragma unroll
+                            for (int ks = 0; ks < BK / 16; ++ks) mma_f16<GROUP>(d, a + ks * a_step, b + ks * b_step, idesc, 1u);
+                            commit<GROUP>(empty_bar(stage));
+                            if (kb + 1 == c1) commit<GROUP>(tfull_bar(acc));
                         }
-#pragma unroll
-                        for (int ks = 0; ks < BK / 16; ++ks)
-                            mma_f16<GROUP>(d, make_desc(a + ks * a_step, a_lbo), make_desc(b + ks * b_step, b_lbo), idesc, 1u);
-                        commit<GROUP>(empty_bar(stage));
                         if (++stage == STAGES) { stage = 0; phase ^= 1u; }
                     }
-                    if (!ok) break;
-                    commit<GROUP>(tfull_bar(acc));
                     if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
                 }
             }
-            if (!ok && GROUP == 2) st_cluster_u32(peer_abort, 1u);
+            if (!ok && GROUP == 2 && lane == 0) st_cluster_u32(peer_abort, 1u);
         }
     } else {
         const int quarter = warp & 3, side = (warp - 2) >> 2;  // rows 32 quarter.., columns BN/2 side..
@@ -597,7 +594,7 @@ __global__ void __launch_bounds__(MID_THREADS, 1) ns_tile_kernel(const __grid_co
                 for (int i = 0; i < 2048; ++i) __nanosleep(1000);
         }
     } else if (warp == 1) {
-        if (lane == 0) {
+        {
             constexpr uint32_t idesc = make_idesc(BM, BM, A_MN, B_MN);
             constexpr uint64_t a_lo = (A_MN ? STAGE_BYTES / 8 : STAGE_BYTES / 4) >> 4, b_lo = (B_MN ? STAGE_BYTES / 8 : STAGE_BYTES / 4) >> 4;
             constexpr uint64_t a_step = (A_MN ? 2048u : 32u) >> 4, b_step = (B_MN ? 2048u : 32u) >> 4;
@@ -609,6 +606,8 @@ __global__ void __launch_bounds__(MID_THREADS, 1) ns_tile_kernel(const __grid_co
                 fence_after();
                 const uint32_t d = tmem + acc * 128;
                 const uint64_t a = make_desc(smem_base + st * STAGE_BYTES, a_lbo), b = make_desc(smem_base + st * STAGE_BYTES + STAGE_BYTES / 2, b_lbo);
+                __syncwarp();
+                if (!elect_one()) continue;
 #pragma unroll
                 for (int ks = 0; ks < BK / 16; ++ks) {  // the small terms first, while the accumulator is small
                     mma_f16<1>(d, a + a_lo + ks * a_step, b + ks * b_step, idesc, ks > 0);
@@ -865,9 +864,11 @@ __global__ void __launch_bounds__(CL_THREADS, 1) ns_cluster_kernel(const Cluster
     // operand a (K-major) times operand b over `kk` terms, the first half of them into columns 0.., the second into 128..;
     // in each the small terms go first.
     auto product = [&](uint32_t a, uint32_t b, bool b_mn, int n, int kk) {
-        if (tid != 0) return;
+        if (warp != 0) return;
+        __syncwarp();
         fence_after();
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        if (!elect_one()) return;
         const uint32_t idesc = make_idesc(128, 0, false, b_mn) | (static_cast<uint32_t>(n >> 3) << 17);
         // (descriptors hold addresses in units of 16 bytes: every step is an addition of a constant)
         constexpr uint64_t LO = (2 * CL_GROUP) >> 4, GROUP = CL_GROUP >> 4, K16 = 32 >> 4, K16_MN = 2048 >> 4;
@@ -1068,27 +1069,10 @@ __global__ void __launch_bounds__(CL_THREADS, 1) ns_cluster_kernel(const Cluster
 }
 
 // ---- host side -------------------------------------------------------------------------------------------
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
-                                   CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-ctk_status get_encoder(EncodeTiledFn* out) {
-    static std::mutex mu;
-    static EncodeTiledFn encode = nullptr;
-    std::lock_guard<std::mutex> lock(mu);
-    if (!encode) {
-        void* fn = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        CTK_CUDA(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q));
-        if (!fn || q != cudaDriverEntryPointSuccess) return fail(CTK_ERR_CUDA, "cuTensorMapEncodeTiled not available from the driver");
-        encode = reinterpret_cast<EncodeTiledFn>(fn);
-    }
-    *out = encode;
-    return CTK_OK;
-}
-
 // {inner, outer, hi | lo} with box {64, box_outer, 2}: one copy brings hi and lo.  Elements past an extent read as zero.
 ctk_status make_map(CUtensorMap* map, const Pair& p, int64_t inner, int64_t outer, int box_outer) {
-    EncodeTiledFn enc;
-    ctk_status st = get_encoder(&enc);
+    t5::EncodeTiledFn enc;
+    ctk_status st = t5::get_encoder(&enc);
     if (st) return st;
     const cuuint64_t dims[3] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer), 2u};
     const cuuint64_t strides[2] = {static_cast<cuuint64_t>(p.pitch) * 2, static_cast<cuuint64_t>(p.lo) * 2};

@@ -111,39 +111,39 @@ __global__ void __launch_bounds__(W4_THREADS) w4_dequantize_kernel(const uint32_
 // A first, small kernel writes x's digits (w4_digits_kernel: a warp per row and 128 k) block by block as the main kernel's
 // shared memory wants them.  A CTA of the main kernel takes 128 columns of W and, in blocks of 128 k, its share of k (a cluster
 // of `split` CTAs shares the whole):
-//   3 or 4      codes, a block each in turn: 16 bytes (32 codes) per load, a whole block ahead -- the first before x's digits
-//               are there --, masks, two 16-byte stores into the operand tile [128 columns][128 k] (128-byte rows, swizzled);
-//   1 warp      one bulk copy per block for x's digits, their sums and x's steps;
+//   2 warps     loads: the block's codes (one TMA copy, 128 columns x 64 bytes, RAW blocks in flight, the first of them before
+//               x's digits are there) and x's digits, their sums and x's steps (one bulk copy);
+//   4 warps     a thread per column: its 64 bytes of codes, masked, into the operand's place in tensor memory;
 //   1 warp      the products: one instruction per 32 k, an accumulator [128 columns][(row, digit)] per group;
 //   4 or 8      a thread per column: digits joined, zero point, scale, added to the column's results.
-// mma.sync with x cut into three bf16 parts, the form before this one, ran at about 32 clocks an instruction on this machine
-// and took 95 us for 4 x 16384 x 16384, 46 us for 64 x 4096 x 4096; this one LATER.
+// Before this: mma.sync with x cut into three bf16 parts (about 32 clocks an instruction on this machine) 95 us for
+// 4 x 16384 x 16384 and 46 us for 64 x 4096 x 4096; the operand in shared memory, its codes through registers, 96 and 35 us
+// (the load and store unit was the bound); this one LATER and LATER.
 constexpr int MM_COLS = 128, MM_BLOCK = 128;         // columns of a CTA, k of a block
-constexpr int MM_UNITS = MM_COLS * 4 / 32;           // 16-byte pieces of a block of codes per lane
+constexpr int MM_RAW_BYTES = MM_COLS * MM_BLOCK / 2; // codes of a block
+constexpr int MM_A_COLS = MM_BLOCK / 4;              // tensor memory columns of a block's operand
 constexpr int R_PITCH = 132;
 
 template <int GROUP, int ROWS>
 struct MmCfg {
     static constexpr int N = 8 * ROWS;               // accumulator columns
     static constexpr int GPB = MM_BLOCK / GROUP;     // groups of a block
-    static constexpr int STAGES = ROWS <= 8 ? 4 : 3;
-    static constexpr int ACCS = N <= 64 ? 4 : 2;     // accumulators in turn
-    static constexpr int TMEM_COLS = N * ACCS;       // 64 .. 512, a power of two
-    static constexpr int A_BYTES = MM_COLS * MM_BLOCK, B_BYTES = N * MM_BLOCK;
-    static constexpr int T_BYTES = (GPB * N + (ROWS < 4 ? 4 : ROWS)) * 4;  // sums of digits per (group, row, digit), x's step per row
-    static constexpr int X_BYTES = B_BYTES + T_BYTES;                      // a block of x as the first kernel leaves it
-    static constexpr int STAGE_BYTES = (A_BYTES + X_BYTES + 1023) / 1024 * 1024;
-    static constexpr int RING = STAGES * STAGE_BYTES, R_BYTES = ROWS * R_PITCH * 4;
+    static constexpr int RAW = 8, STAGES = 4;        // blocks of codes in flight; blocks of operands
+    static constexpr int ACCS = N <= 32 ? 4 : 2;     // accumulators in turn
+    static constexpr int USED_COLS = N * ACCS + STAGES * MM_A_COLS;
+    static constexpr int TMEM_COLS = USED_COLS <= 256 ? 256 : 512;
+    static constexpr int PER_SM = 512 / TMEM_COLS;
+    static constexpr int B_BYTES = N * MM_BLOCK;
+    static constexpr int T_BYTES = (GPB * ROWS * 4 + (ROWS < 4 ? 4 : ROWS)) * 4;  // joined sums of digits per (group, row), x's step per row
+    static constexpr int X_BYTES = B_BYTES + T_BYTES;                             // a block of x as the first kernel leaves it
+    static constexpr int X_STAGE = (X_BYTES + 1023) / 1024 * 1024;
+    static constexpr int RING = RAW * MM_RAW_BYTES + STAGES * X_STAGE, R_BYTES = ROWS * R_PITCH * 4;
     static constexpr int SMEM = (RING > R_BYTES ? RING : R_BYTES) + 1024;
-    static constexpr int PER_SM = ROWS <= 16 ? 2 : 1;
-    static constexpr int DRAIN = ROWS <= 16 ? 4 : 8; // warps that take the accumulators: 4 per CTA's columns, or 8 with half of the rows each
+    static constexpr int DRAIN = ROWS <= 8 ? 4 : 8;  // warps that take the accumulators: 4, or 8 with half of the rows each
     static constexpr int MINE = ROWS * 4 / DRAIN;    // rows of such a warp
-    static constexpr int AHEAD = ROWS <= 4 ? 8 : ROWS <= 8 ? 4 : 2;  // groups whose scales are in flight
-    // Warps that unpack codes, each whole blocks: one per stage, so that a warp always fills the same stage and never waits for
-    // it more than one round ahead (a barrier's parity cannot tell two rounds from none).
-    static constexpr int FILL = STAGES;
-    static constexpr int THREADS = (DRAIN + 2 + FILL) * 32;
-    static_assert(X_BYTES % 16 == 0 && TMEM_COLS * PER_SM <= 512 && SMEM * PER_SM <= 225 * 1024, "");
+    static constexpr int AHEAD = ROWS <= 4 ? 8 : 4;  // groups whose scales are in flight
+    static constexpr int THREADS = (DRAIN + 4 + 3) * 32;
+    static_assert(X_BYTES % 16 == 0 && USED_COLS <= 512 && SMEM * PER_SM <= 225 * 1024 && MINE % 2 == 0, "");
 };
 
 __device__ int g_w4_status = 0;  // first bounded wait that ran out, else 0
@@ -190,6 +190,7 @@ __global__ void __launch_bounds__(128) w4_digits_kernel(const float* __restrict_
 #pragma unroll
     for (int e = 0; e < 4; ++e) digits[e] = static_cast<uint32_t>(__float2int_rn(bad ? 0.0f : v[e] * up)) + 0x88888888u;
     // four bytes of digit d: sign and magnitude of nibble - 8; this lane's four k are codes 0..3 (even lanes) or 4..7 of a word
+    int pair = 0;  // sums over the group of digit 2p and 16 times digit 2p + 1
 #pragma unroll
     for (int d = 0; d < 8; ++d) {
         uint32_t four = 0;
@@ -207,26 +208,34 @@ __global__ void __launch_bounds__(128) w4_digits_kernel(const float* __restrict_
         *reinterpret_cast<uint32_t*>(out + col * 128 + (((lane >> 2) ^ (col & 7)) << 4) + (lane & 3) * 4) = bytes;
 #pragma unroll
         for (int s = 1; s < GROUP / 4; s <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);  // of the group's lanes
-        if (lane % (GROUP / 4) == 0) sums[(lane / (GROUP / 4)) * C::N + col] = static_cast<float>(sum) * (1.0f / 262144.0f);
+        pair = d & 1 ? pair + 16 * sum : sum;
+        if ((d & 1) && lane % (GROUP / 4) == 0) sums[((lane / (GROUP / 4)) * ROWS + r) * 4 + d / 2] = static_cast<float>(pair) * (1.0f / 262144.0f);
     }
     // what one unit of digit 0 stands for, times 2^18
-    if (lane == 0) sums[C::GPB * C::N + r] = __uint_as_float(bad ? 0x7FC00000u : static_cast<uint32_t>(127 + ex - 156 + 18) << 23);
+    if (lane == 0) sums[C::GPB * ROWS * 4 + r] = __uint_as_float(bad ? 0x7FC00000u : static_cast<uint32_t>(127 + ex - 156 + 18) << 23);
 }
 
 template <int GROUP, int ROWS>
-__global__ void __launch_bounds__((MmCfg<GROUP, ROWS>::THREADS), (MmCfg<GROUP, ROWS>::PER_SM)) w4_matmul_kernel(const MmArgs P) {
+__global__ void __launch_bounds__((MmCfg<GROUP, ROWS>::THREADS), (MmCfg<GROUP, ROWS>::PER_SM))
+w4_matmul_kernel(const __grid_constant__ CUtensorMap codes, const MmArgs P) {
     using namespace t5;
     using C = MmCfg<GROUP, ROWS>;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t bars[2 * C::STAGES + 2 * C::ACCS];
+    __shared__ uint64_t bars[2 * C::RAW + 4 * C::STAGES + 2 * C::ACCS];
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int abort_flag;
-    uint8_t* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint8_t* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);  // [x stages][raw blocks]
     const uint32_t bar0 = smem_u32(bars), base = smem_u32(smem);
-    auto full_bar = [&](int s) { return bar0 + 8u * s; };
-    auto empty_bar = [&](int s) { return bar0 + 8u * (C::STAGES + s); };
-    auto afull_bar = [&](int a) { return bar0 + 8u * (2 * C::STAGES + a); };
-    auto aempty_bar = [&](int a) { return bar0 + 8u * (2 * C::STAGES + C::ACCS + a); };
+    auto raw_full = [&](int i) { return bar0 + 8u * i; };
+    auto raw_empty = [&](int i) { return bar0 + 8u * (C::RAW + i); };
+    auto x_full = [&](int s) { return bar0 + 8u * (2 * C::RAW + s); };
+    auto x_empty = [&](int s) { return bar0 + 8u * (2 * C::RAW + C::STAGES + s); };
+    auto op_full = [&](int s) { return bar0 + 8u * (2 * C::RAW + 2 * C::STAGES + s); };
+    auto op_empty = [&](int s) { return bar0 + 8u * (2 * C::RAW + 3 * C::STAGES + s); };
+    auto acc_full = [&](int a) { return bar0 + 8u * (2 * C::RAW + 4 * C::STAGES + a); };
+    auto acc_empty = [&](int a) { return bar0 + 8u * (2 * C::RAW + 4 * C::STAGES + C::ACCS + a); };
+    constexpr uint32_t RAW_AT = C::STAGES * C::X_STAGE;
+    constexpr int W_OP = C::DRAIN, W_MMA = W_OP + 4, W_CODES = W_MMA + 1, W_X = W_CODES + 1;  // warps by role (W_OP a multiple of 4)
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int split = P.split, rank = blockIdx.x % split;
     const int64_t col_base = static_cast<int64_t>(blockIdx.x / split) * MM_COLS, row_base = static_cast<int64_t>(blockIdx.y) * ROWS;
@@ -237,91 +246,109 @@ __global__ void __launch_bounds__((MmCfg<GROUP, ROWS>::THREADS), (MmCfg<GROUP, R
 
     if (tid == 0) {
         abort_flag = 0;
-        for (int s = 0; s < C::STAGES; ++s) { mbar_init(full_bar(s), 2); mbar_init(empty_bar(s), 1 + C::DRAIN); }
-        for (int a = 0; a < C::ACCS; ++a) { mbar_init(afull_bar(a), 1); mbar_init(aempty_bar(a), C::DRAIN); }
+        for (int i = 0; i < C::RAW; ++i) { mbar_init(raw_full(i), 1); mbar_init(raw_empty(i), 4); }
+        for (int s = 0; s < C::STAGES; ++s) {
+            mbar_init(x_full(s), 1);
+            mbar_init(x_empty(s), 1 + C::DRAIN);
+            mbar_init(op_full(s), 4);
+            mbar_init(op_empty(s), 1);
+        }
+        for (int a = 0; a < C::ACCS; ++a) { mbar_init(acc_full(a), 1); mbar_init(acc_empty(a), C::DRAIN); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == C::DRAIN) tmem_alloc<1>(smem_u32(&tmem_slot), C::TMEM_COLS);
+    if (warp == W_MMA) tmem_alloc<1>(smem_u32(&tmem_slot), C::TMEM_COLS);
     fence_before();
     __syncthreads();
     fence_after();
-    const uint32_t tmem = tmem_slot;
+    const uint32_t tmem = tmem_slot, op_tmem = tmem + C::N * C::ACCS;
 
     float result[C::MINE];
 #pragma unroll
     for (int r = 0; r < C::MINE; ++r) result[r] = 0.0f;
 
-    if (warp >= C::DRAIN + 2) {
-        // ------------------------------ codes ------------------------------
-        const int fw = warp - (C::DRAIN + 2), q = lane & 3;  // blocks fw, fw + FILL, ..; 16-byte piece q of columns lane / 4, lane / 4 + 8, ..
-        const int64_t row_words = P.groups * (GROUP / 8);    // words of one column
-        // (a last block may hold fewer than 128 k: its missing groups are not read)
-        const int64_t whole = (row_words - q * 4 + MM_BLOCK / 8 - 1) / (MM_BLOCK / 8) - b_begin;
-        const int my_blocks = blocks < whole ? blocks : static_cast<int>(whole);
-        const uint32_t* const src = P.packed + b_begin * (MM_BLOCK / 8) + q * 4;
-        const uint32_t dst = static_cast<uint32_t>((lane >> 2) * 128 + (((2 * q) ^ (lane >> 2)) << 4));  // the first 16 of its 32 bytes
-        uint4 held[MM_UNITS];
-        auto fetch = [&](int u, int b) {
-            // a column past the end is replaced by one that exists, its results are dropped
-            const int64_t c = col_base + (lane >> 2) + u * 8;
-            if (b < my_blocks)
-                asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];"
-                             : "=r"(held[u].x), "=r"(held[u].y), "=r"(held[u].z), "=r"(held[u].w)
-                             : "l"(src + (c < P.n ? c : P.n - 1) * row_words + static_cast<int64_t>(b) * (MM_BLOCK / 8)));
-            else held[u] = make_uint4(0u, 0u, 0u, 0u);
-        };
-#pragma unroll
-        for (int u = 0; u < MM_UNITS; ++u) fetch(u, fw);
-        for (int b = fw; b < blocks; b += C::FILL) {
-            const int st = b % C::STAGES;
-            if (!mbar_wait(empty_bar(st), ((b / C::STAGES) & 1) ^ 1u, &abort_flag, &g_w4_status, 0x100 | st)) break;
-            uint8_t* to = smem + st * C::STAGE_BYTES + dst;
-#pragma unroll
-            for (int u = 0; u < MM_UNITS; ++u) {
-                const uint4 w = held[u];
-                constexpr uint32_t M = 0x0F0F0F0Fu;
-                *reinterpret_cast<uint4*>(to + u * 1024) = make_uint4(w.x & M, (w.x >> 4) & M, w.y & M, (w.y >> 4) & M);
-                *reinterpret_cast<uint4*>(smem + st * C::STAGE_BYTES + (dst ^ 16u) + u * 1024) = make_uint4(w.z & M, (w.z >> 4) & M, w.w & M, (w.w >> 4) & M);
-                fetch(u, b + C::FILL);
+    if (warp == W_CODES) {
+        // ------------------------------ codes: global -> shared ------------------------------
+        if (lane == 0) {
+            for (int b = 0; b < blocks; ++b) {
+                const int i = b % C::RAW;
+                if (!mbar_wait(raw_empty(i), ((b / C::RAW) & 1) ^ 1u, &abort_flag, &g_w4_status, 0x100 | i)) break;
+                mbar_expect_tx(raw_full(i), MM_RAW_BYTES);
+                tma_load_2d(base + RAW_AT + i * MM_RAW_BYTES, &codes, raw_full(i), static_cast<int>((b_begin + b) * (MM_BLOCK / 8)), static_cast<int>(col_base));
             }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(full_bar(st));
         }
-    } else if (warp == C::DRAIN + 1) {
-        // ------------------------------ x ------------------------------
+    } else if (warp == W_X) {
+        // ------------------------------ x: global -> shared ------------------------------
         if (lane == 0) {
             asm volatile("griddepcontrol.wait;" ::: "memory");  // x's digits are there
             const uint8_t* from = P.image + (blockIdx.y * all_blocks + b_begin) * C::X_BYTES;
             for (int b = 0; b < blocks; ++b) {
                 const int st = b % C::STAGES;
-                if (!mbar_wait(empty_bar(st), ((b / C::STAGES) & 1) ^ 1u, &abort_flag, &g_w4_status, 0x180 | st)) break;
-                mbar_expect_tx(full_bar(st), C::X_BYTES);
-                asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                             ::"r"(base + st * C::STAGE_BYTES + C::A_BYTES), "l"(from + static_cast<int64_t>(b) * C::X_BYTES), "r"(static_cast<uint32_t>(C::X_BYTES)), "r"(full_bar(st)) : "memory");
+                if (!mbar_wait(x_empty(st), ((b / C::STAGES) & 1) ^ 1u, &abort_flag, &g_w4_status, 0x180 | st)) break;
+                mbar_expect_tx(x_full(st), C::X_BYTES);
+                bulk_load(base + st * C::X_STAGE, from + static_cast<int64_t>(b) * C::X_BYTES, C::X_BYTES, x_full(st));
             }
         }
-    } else if (warp == C::DRAIN) {
-        // ------------------------------ products ------------------------------
-        if (lane == 0) {
-            constexpr uint32_t idesc = make_idesc(MM_COLS, C::N, false, false);
-            int acc = 0;
-            uint32_t acc_phase = 0;
-            bool ok = true;
-            for (int b = 0; b < blocks && ok; ++b) {
-                const int st = b % C::STAGES;
-                if (!mbar_wait(full_bar(st), (b / C::STAGES) & 1, &abort_flag, &g_w4_status, 0x200 | st)) break;
-                const uint64_t a = make_desc(base + st * C::STAGE_BYTES, 0), x = make_desc(base + st * C::STAGE_BYTES + C::A_BYTES, 0);
-                const int64_t left = P.groups - (b_begin + b) * C::GPB;
-                for (int g = 0; g < C::GPB && g < left; ++g) {
-                    if (!mbar_wait(aempty_bar(acc), acc_phase ^ 1u, &abort_flag, &g_w4_status, 0x210 | acc)) { ok = false; break; }
-                    fence_after();
+    } else if (warp >= W_OP && warp < W_MMA) {
+        // ------------------------------ codes: shared -> operand ------------------------------
+        const int row = (warp & 3) * 32 + lane;  // this thread's column of W
+        for (int b = 0; b < blocks; ++b) {
+            const int i = b % C::RAW, st = b % C::STAGES;
+            if (!mbar_wait(raw_full(i), (b / C::RAW) & 1, &abort_flag, &g_w4_status, 0x400 | i)) break;
+            const uint8_t* raw = smem + RAW_AT + i * MM_RAW_BYTES + row * 64;
+            uint32_t o[32];
 #pragma unroll
-                    for (int ks = 0; ks < GROUP / 32; ++ks) mma_f8(tmem + acc * C::N, a + (g * (GROUP / 32) + ks) * 2, x + (g * (GROUP / 32) + ks) * 2, idesc, ks > 0);
-                    commit<1>(afull_bar(acc));
-                    if (++acc == C::ACCS) { acc = 0; acc_phase ^= 1u; }
+            for (int c = 0; c < 4; ++c) {  // (the copy's 64-byte swizzle: 16-byte pieces XOR row / 2 % 4)
+                const uint4 w = *reinterpret_cast<const uint4*>(raw + ((c ^ ((row >> 1) & 3)) << 4));
+                constexpr uint32_t M = 0x0F0F0F0Fu;
+                o[c * 8] = w.x & M; o[c * 8 + 1] = (w.x >> 4) & M;
+                o[c * 8 + 2] = w.y & M; o[c * 8 + 3] = (w.y >> 4) & M;
+                o[c * 8 + 4] = w.z & M; o[c * 8 + 5] = (w.z >> 4) & M;
+                o[c * 8 + 6] = w.w & M; o[c * 8 + 7] = (w.w >> 4) & M;
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(raw_empty(i));
+            if (!mbar_wait(op_empty(st), ((b / C::STAGES) & 1) ^ 1u, &abort_flag, &g_w4_status, 0x410 | st)) break;
+            fence_after();
+            tmem_st32(op_tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + st * MM_A_COLS, o);
+            tmem_st_wait();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(op_full(st));
+        }
+    } else if (warp == W_MMA) {
+        // ------------------------------ products ------------------------------
+        constexpr uint32_t idesc = make_idesc(MM_COLS, C::N, false, false);
+        int acc = 0;
+        uint32_t acc_phase = 0;
+        bool ok = true;
+        for (int b = 0; b < blocks && ok; ++b) {
+            const int st = b % C::STAGES;
+            const uint32_t parity = (b / C::STAGES) & 1;
+            if (!mbar_wait(x_full(st), parity, &abort_flag, &g_w4_status, 0x200 | st)) break;
+            if (!mbar_wait(op_full(st), parity, &abort_flag, &g_w4_status, 0x208 | st)) break;
+            const uint64_t x = make_desc(base + st * C::X_STAGE, 0);
+            const int64_t left = P.groups - (b_begin + b) * C::GPB;
+            const int here = left < C::GPB ? static_cast<int>(left) : C::GPB;
+#pragma unroll
+            for (int g = 0; g < C::GPB; ++g) {
+                if (g >= here) break;
+                if (!mbar_wait(acc_empty(acc), acc_phase ^ 1u, &abort_flag, &g_w4_status, 0x210 | acc)) { ok = false; break; }
+                fence_after();
+                __syncwarp();
+                if (elect_one()) {
+#pragma unroll
+                    for (int ks = 0; ks < GROUP / 32; ++ks) {
+                        const int k32 = g * (GROUP / 32) + ks;
+                        mma_f8_ts(tmem + acc * C::N, op_tmem + st * MM_A_COLS + k32 * 8, x + k32 * 2, idesc, ks > 0);
+                    }
+                    commit<1>(acc_full(acc));
                 }
-                if (ok) commit<1>(empty_bar(st));
+                if (++acc == C::ACCS) { acc = 0; acc_phase ^= 1u; }
+            }
+            __syncwarp();
+            if (ok && elect_one()) {
+                commit<1>(op_empty(st));
+                commit<1>(x_empty(st));
             }
         }
     } else {
@@ -348,13 +375,13 @@ __global__ void __launch_bounds__((MmCfg<GROUP, ROWS>::THREADS), (MmCfg<GROUP, R
             for (int i = 0; i < C::AHEAD; ++i) {
                 const int gi = g0 + i, b = gi / C::GPB, st = b % C::STAGES, g = gi % C::GPB;
                 if (gi >= groups || !ok) break;
-                const float* sums = reinterpret_cast<const float*>(smem + st * C::STAGE_BYTES + C::A_BYTES + C::B_BYTES);
-                const float* step = sums + C::GPB * C::N + r_first;
-                sums += g * C::N + r_first * 8;
-                if (g == 0 && !mbar_wait(full_bar(st), (b / C::STAGES) & 1, &abort_flag, &g_w4_status, 0x300 | st)) { ok = false; break; }
+                const float* sums = reinterpret_cast<const float*>(smem + st * C::X_STAGE + C::B_BYTES);
+                const float* step = sums + C::GPB * ROWS * 4 + r_first;
+                sums += (g * ROWS + r_first) * 4;
+                if (g == 0 && !mbar_wait(x_full(st), (b / C::STAGES) & 1, &abort_flag, &g_w4_status, 0x300 | st)) { ok = false; break; }
                 const float s = scale[i], z = -static_cast<float>(zero[i]);
                 fetch(scale[i], zero[i], gi + C::AHEAD);
-                if (!mbar_wait(afull_bar(acc), acc_phase, &abort_flag, &g_w4_status, 0x310 | acc)) { ok = false; break; }
+                if (!mbar_wait(acc_full(acc), acc_phase, &abort_flag, &g_w4_status, 0x310 | acc)) { ok = false; break; }
                 fence_after();
                 // two rows at a time, the next two on their way while these are joined
                 uint32_t d[2][16];
@@ -362,11 +389,11 @@ __global__ void __launch_bounds__((MmCfg<GROUP, ROWS>::THREADS), (MmCfg<GROUP, R
 #pragma unroll
                 for (int r0 = 0; r0 < C::MINE; r0 += 2) {
                     constexpr int LAST = C::MINE - 2;
-                    float ds[2][8], up[2];
+                    float4 ds[2];
+                    float up[2];
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
-                        *reinterpret_cast<float4*>(ds[r]) = *reinterpret_cast<const float4*>(sums + (r0 + r) * 8);
-                        *reinterpret_cast<float4*>(ds[r] + 4) = *reinterpret_cast<const float4*>(sums + (r0 + r) * 8 + 4);
+                        ds[r] = *reinterpret_cast<const float4*>(sums + (r0 + r) * 4);
                         up[r] = step[r0 + r] * s;
                     }
                     tmem_ld_wait();
@@ -375,25 +402,20 @@ __global__ void __launch_bounds__((MmCfg<GROUP, ROWS>::THREADS), (MmCfg<GROUP, R
                     } else {  // read completely
                         fence_before();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(aempty_bar(acc));
+                        if (lane == 0) mbar_arrive(acc_empty(acc));
                     }
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
-                        float w[8];
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) w[e] = fmaf(z, ds[r][e], __uint_as_float(d[(r0 >> 1) & 1][r * 8 + e]));
-                        // (pairs, then pairs of pairs: 256 and 65536 are exact factors, every level rounds once)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) w[e] = fmaf(w[2 * e + 1], 16.0f, w[2 * e]);
-                        w[0] = fmaf(w[1], 256.0f, w[0]);
-                        w[2] = fmaf(w[3], 256.0f, w[2]);
-                        result[r0 + r] = fmaf(fmaf(w[2], 65536.0f, w[0]), up[r], result[r0 + r]);
+                        const uint32_t* q = &d[(r0 >> 1) & 1][r * 8];
+                        auto pair = [&](int e) { return fmaf(__uint_as_float(q[2 * e + 1]), 16.0f, __uint_as_float(q[2 * e])); };  // exact: below 2^19
+                        const float w0 = fmaf(z, ds[r].x, pair(0)), w1 = fmaf(z, ds[r].y, pair(1)), w2 = fmaf(z, ds[r].z, pair(2)), w3 = fmaf(z, ds[r].w, pair(3));
+                        result[r0 + r] = fmaf(fmaf(fmaf(w3, 256.0f, w2), 65536.0f, fmaf(w1, 256.0f, w0)), up[r], result[r0 + r]);
                     }
                 }
                 if (++acc == C::ACCS) { acc = 0; acc_phase ^= 1u; }
                 if (g == C::GPB - 1 || gi == groups - 1) {
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(empty_bar(st));
+                    if (lane == 0) mbar_arrive(x_empty(st));
                 }
             }
         }
@@ -403,7 +425,7 @@ __global__ void __launch_bounds__((MmCfg<GROUP, ROWS>::THREADS), (MmCfg<GROUP, R
     fence_before();
     __syncthreads();  // no operand is read any more
     fence_after();
-    if (warp == C::DRAIN) tmem_dealloc<1>(tmem, C::TMEM_COLS);
+    if (warp == W_MMA) tmem_dealloc<1>(tmem, C::TMEM_COLS);
     float* const R = reinterpret_cast<float*>(smem);
     if (warp < C::DRAIN) {
 #pragma unroll
@@ -455,6 +477,19 @@ ctk_status launch_matmul(MmArgs P, cudaStream_t st) {
         w4_digits_kernel<GROUP, ROWS><<<dim3(static_cast<unsigned>((k_blocks + 3) / 4), static_cast<unsigned>(row_blocks * ROWS)), 128, 0, st>>>(P.x, P.ldx, P.m, P.k, k_blocks, image);
         CTK_LAUNCH_CHECK("w4_digits");
     }
+    // the codes as a matrix of 32-bit words, 128 columns x 16 words a copy; what lies past its extents reads as zero
+    CUtensorMap codes = {};
+    if (k_blocks) {
+        t5::EncodeTiledFn enc;
+        ctk_status rc = t5::get_encoder(&enc);
+        if (rc) return rc;
+        const cuuint64_t words = static_cast<cuuint64_t>(P.groups) * (GROUP / 8);
+        const cuuint64_t dims[2] = {words, static_cast<cuuint64_t>(P.n)}, strides[1] = {words * 4};
+        const cuuint32_t box[2] = {MM_BLOCK / 8, MM_COLS}, estr[2] = {1u, 1u};
+        const CUresult r = enc(&codes, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<uint32_t*>(P.packed), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                               CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        if (r != CUDA_SUCCESS) return fail(CTK_ERR_CUDA, "cuTensorMapEncodeTiled failed with code " + std::to_string(static_cast<int>(r)));
+    }
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -469,7 +504,7 @@ ctk_status launch_matmul(MmArgs P, cudaStream_t st) {
     cfg.stream = st;
     cfg.attrs = attr;
     cfg.numAttrs = k_blocks ? 2 : 1;  // (without k there is nothing in front of it to wait for in the kernel)
-    CTK_CUDA(cudaLaunchKernelEx(&cfg, kernel, P));
+    CTK_CUDA(cudaLaunchKernelEx(&cfg, kernel, codes, P));
     CTK_LAUNCH_CHECK("w4_matmul");
     return CTK_OK;
 }
@@ -479,7 +514,7 @@ ctk_status matmul_rows(const MmArgs& P, cudaStream_t st) {
     if (P.m <= 4) return launch_matmul<GROUP, 4>(P, st);
     if (P.m <= 8) return launch_matmul<GROUP, 8>(P, st);
     if (P.m <= 16) return launch_matmul<GROUP, 16>(P, st);
-    return launch_matmul<GROUP, 32>(P, st);
+    return launch_matmul<GROUP, 24>(P, st);
 }
 
 bool group_ok(int group) { return group == 32 || group == 64 || group == 128; }
