@@ -108,42 +108,44 @@ __global__ void __launch_bounds__(W4_THREADS) w4_dequantize_kernel(const uint32_
 // accumulator whatever it does -- and so is the zero point's share, zero * (sum of the digits).  What rounds: x to its 31 bits,
 // eight digits joined in fp32, one fma per group with the scale.
 //
-// A first, small kernel writes x's digits (w4_digits_kernel: a warp per row and 128 k) block by block as the main kernel's
-// shared memory wants them.  A CTA of the main kernel takes 128 columns of W and, in blocks of 128 k, its share of k (a cluster
+// A first, small kernel writes x's digits (w4_digits_kernel: a warp per row and 128 k) piece by piece as the main kernel's
+// shared memory wants them.  A CTA of the main kernel takes 128 columns of W and, in blocks of 256 k, its share of k (a cluster
 // of `split` CTAs shares the whole):
-//   2 warps     loads: the block's codes (one TMA copy, 128 columns x 64 bytes, RAW blocks in flight, the first of them before
+//   2 warps     loads: the block's codes (one TMA copy, 128 columns x 128 bytes, RAW blocks in flight, the first of them before
 //               x's digits are there) and x's digits, their sums and x's steps (one bulk copy);
-//   4 warps     a thread per column: its 64 bytes of codes, masked, into the operand's place in tensor memory;
-//   1 warp      the products: one instruction per 32 k, an accumulator [128 columns][(row, digit)] per group;
+//   4 warps     a thread per column: its 128 bytes of codes, masked, into the operand's place in tensor memory;
+//   1 warp      the products: one instruction per 32 k, an accumulator [128 columns][(row, digit)] per group, BATCH groups to a
+//               hand-over;
 //   4 or 8      a thread per column: digits joined, zero point, scale, added to the column's results.
-// Before this: mma.sync with x cut into three bf16 parts (about 32 clocks an instruction on this machine) 95 us for
-// 4 x 16384 x 16384 and 46 us for 64 x 4096 x 4096; the operand in shared memory, its codes through registers, 96 and 35 us
-// (the load and store unit was the bound); this one LATER and LATER.
-constexpr int MM_COLS = 128, MM_BLOCK = 128;         // columns of a CTA, k of a block
-constexpr int MM_RAW_BYTES = MM_COLS * MM_BLOCK / 2; // codes of a block
-constexpr int MM_A_COLS = MM_BLOCK / 4;              // tensor memory columns of a block's operand
+// A hand-over between warps (an mbarrier's arrival and wait) takes some 200 clocks, the bytes of 128 columns x 128 k take 180 at
+// HBM's rate: hence the large blocks.  Before this: mma.sync with x cut into three bf16 parts (about 32 clocks an instruction on
+// this machine) 95 us for 4 x 16384 x 16384 and 46 us for 64 x 4096 x 4096; the operand in shared memory, its codes through
+// registers, 96 and 35 us (the load and store unit was the bound); blocks of 128 k, 69 and 37 us; this one LATER and LATER.
+constexpr int MM_COLS = 128, MM_PIECE = 128, MM_BLOCK = 256;  // columns of a CTA; k of one piece of x and of a block
+constexpr int MM_RAW_BYTES = MM_COLS * MM_BLOCK / 2;          // codes of a block
+constexpr int MM_A_COLS = MM_BLOCK / 4;                       // tensor memory columns of a block's operand
 constexpr int R_PITCH = 132;
 
 template <int GROUP, int ROWS>
 struct MmCfg {
-    static constexpr int N = 8 * ROWS;               // accumulator columns
-    static constexpr int GPB = MM_BLOCK / GROUP;     // groups of a block
-    static constexpr int RAW = 8, STAGES = 4;        // blocks of codes in flight; blocks of operands
-    static constexpr int ACCS = N <= 32 ? 4 : 2;     // accumulators in turn
-    static constexpr int USED_COLS = N * ACCS + STAGES * MM_A_COLS;
+    static constexpr int N = 8 * ROWS;               // columns of one accumulator
+    static constexpr int GPP = MM_PIECE / GROUP, GPB = MM_BLOCK / GROUP;  // groups of a piece, of a block
+    static constexpr int STAGES = 2;                 // blocks of operands in tensor memory
+    static constexpr int BATCH = N >= 64 ? 1 : 64 / N < GPB ? 64 / N : GPB;  // groups whose accumulators are handed over together
+    static constexpr int USED_COLS = 2 * BATCH * N + STAGES * MM_A_COLS;     // two such batches in turn
     static constexpr int TMEM_COLS = USED_COLS <= 256 ? 256 : 512;
     static constexpr int PER_SM = 512 / TMEM_COLS;
-    static constexpr int B_BYTES = N * MM_BLOCK;
-    static constexpr int T_BYTES = (GPB * ROWS * 4 + (ROWS < 4 ? 4 : ROWS)) * 4;  // joined sums of digits per (group, row), x's step per row
-    static constexpr int X_BYTES = B_BYTES + T_BYTES;                             // a block of x as the first kernel leaves it
-    static constexpr int X_STAGE = (X_BYTES + 1023) / 1024 * 1024;
-    static constexpr int RING = RAW * MM_RAW_BYTES + STAGES * X_STAGE, R_BYTES = ROWS * R_PITCH * 4;
+    static constexpr int RAW = ROWS == 8 ? 3 : 4, XS = ROWS <= 4 ? 4 : 3;    // blocks of codes and of x in flight or in use
+    static constexpr int B_BYTES = N * MM_PIECE;
+    static constexpr int T_BYTES = (GPP * ROWS * 4 + ROWS) * 4;              // joined sums of digits per (group, row), x's step per row
+    static constexpr int X_BYTES = (B_BYTES + T_BYTES + 1023) / 1024 * 1024; // a piece of x as the first kernel leaves it
+    static constexpr int RING = RAW * MM_RAW_BYTES + XS * 2 * X_BYTES, R_BYTES = ROWS * R_PITCH * 4;
     static constexpr int SMEM = (RING > R_BYTES ? RING : R_BYTES) + 1024;
     static constexpr int DRAIN = ROWS <= 8 ? 4 : 8;  // warps that take the accumulators: 4, or 8 with half of the rows each
     static constexpr int MINE = ROWS * 4 / DRAIN;    // rows of such a warp
     static constexpr int AHEAD = ROWS <= 4 ? 8 : 4;  // groups whose scales are in flight
     static constexpr int THREADS = (DRAIN + 4 + 3) * 32;
-    static_assert(X_BYTES % 16 == 0 && USED_COLS <= 512 && SMEM * PER_SM <= 225 * 1024 && MINE % 2 == 0, "");
+    static_assert(USED_COLS <= 512 && SMEM * PER_SM <= 225 * 1024 && MINE % 2 == 0 && GPB % BATCH == 0, "");
 };
 
 __device__ int g_w4_status = 0;  // first bounded wait that ran out, else 0
@@ -159,22 +161,22 @@ struct MmArgs {
     int64_t ldy;
     int64_t m, k, n, groups;
     int relu, split;
-    const uint8_t* image;  // x's digits, [row block][k block][X_BYTES]
+    const uint8_t* image;  // x's digits, [row block][piece][X_BYTES]
 };
 
-// x's digits.  A warp takes one row's 128 k of a block, lane l the k 4l .. 4l+3.  Rows past m give zeros.
+// x's digits.  A warp takes one row's 128 k of a piece, lane l the k 4l .. 4l+3.  Rows past m give zeros.
 // The order of a word's codes in the operand's bytes: the masks leave the even nibbles, then the odd ones,
 // nibbles 0 2 4 6 = codes 0 4 1 5 and nibbles 1 3 5 7 = codes 2 6 3 7; x's digits are stored in that order.
 template <int GROUP, int ROWS>
-__global__ void __launch_bounds__(128) w4_digits_kernel(const float* __restrict__ x, int64_t ldx, int64_t m, int64_t k, int64_t k_blocks, uint8_t* __restrict__ image) {
+__global__ void __launch_bounds__(128) w4_digits_kernel(const float* __restrict__ x, int64_t ldx, int64_t m, int64_t k, int64_t pieces, uint8_t* __restrict__ image) {
     using C = MmCfg<GROUP, ROWS>;
     const int lane = threadIdx.x & 31;
-    const int64_t block = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+    const int64_t piece = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
     const int row_block = blockIdx.y / ROWS, r = blockIdx.y % ROWS;
-    const int64_t row = blockIdx.y, k0 = block * MM_BLOCK + lane * 4;
+    const int64_t row = blockIdx.y, k0 = piece * MM_PIECE + lane * 4;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (the main kernel starts with what does not depend on this one)
-    if (block >= k_blocks) return;
-    uint8_t* const out = image + (row_block * k_blocks + block) * C::X_BYTES;
+    if (piece >= pieces) return;
+    uint8_t* const out = image + (row_block * pieces + piece) * C::X_BYTES;
     float* const sums = reinterpret_cast<float*>(out + C::B_BYTES);
     float v[4];
 #pragma unroll
@@ -212,7 +214,7 @@ __global__ void __launch_bounds__(128) w4_digits_kernel(const float* __restrict_
         if ((d & 1) && lane % (GROUP / 4) == 0) sums[((lane / (GROUP / 4)) * ROWS + r) * 4 + d / 2] = static_cast<float>(pair) * (1.0f / 262144.0f);
     }
     // what one unit of digit 0 stands for, times 2^18
-    if (lane == 0) sums[C::GPB * ROWS * 4 + r] = __uint_as_float(bad ? 0x7FC00000u : static_cast<uint32_t>(127 + ex - 156 + 18) << 23);
+    if (lane == 0) sums[C::GPP * ROWS * 4 + r] = __uint_as_float(bad ? 0x7FC00000u : static_cast<uint32_t>(127 + ex - 156 + 18) << 23);
 }
 
 template <int GROUP, int ROWS>
@@ -221,46 +223,43 @@ w4_matmul_kernel(const __grid_constant__ CUtensorMap codes, const MmArgs P) {
     using namespace t5;
     using C = MmCfg<GROUP, ROWS>;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t bars[2 * C::RAW + 4 * C::STAGES + 2 * C::ACCS];
+    __shared__ uint64_t bars[2 * C::RAW + 2 * C::XS + 2 * C::STAGES + 4];
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int abort_flag;
-    uint8_t* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);  // [x stages][raw blocks]
+    uint8_t* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);  // [blocks of x][blocks of codes]
     const uint32_t bar0 = smem_u32(bars), base = smem_u32(smem);
     auto raw_full = [&](int i) { return bar0 + 8u * i; };
     auto raw_empty = [&](int i) { return bar0 + 8u * (C::RAW + i); };
-    auto x_full = [&](int s) { return bar0 + 8u * (2 * C::RAW + s); };
-    auto x_empty = [&](int s) { return bar0 + 8u * (2 * C::RAW + C::STAGES + s); };
-    auto op_full = [&](int s) { return bar0 + 8u * (2 * C::RAW + 2 * C::STAGES + s); };
-    auto op_empty = [&](int s) { return bar0 + 8u * (2 * C::RAW + 3 * C::STAGES + s); };
-    auto acc_full = [&](int a) { return bar0 + 8u * (2 * C::RAW + 4 * C::STAGES + a); };
-    auto acc_empty = [&](int a) { return bar0 + 8u * (2 * C::RAW + 4 * C::STAGES + C::ACCS + a); };
-    constexpr uint32_t RAW_AT = C::STAGES * C::X_STAGE;
+    auto x_full = [&](int i) { return bar0 + 8u * (2 * C::RAW + i); };
+    auto x_empty = [&](int i) { return bar0 + 8u * (2 * C::RAW + C::XS + i); };
+    auto op_full = [&](int s) { return bar0 + 8u * (2 * C::RAW + 2 * C::XS + s); };
+    auto op_empty = [&](int s) { return bar0 + 8u * (2 * C::RAW + 2 * C::XS + C::STAGES + s); };
+    auto acc_full = [&](int a) { return bar0 + 8u * (2 * C::RAW + 2 * C::XS + 2 * C::STAGES + a); };
+    auto acc_empty = [&](int a) { return bar0 + 8u * (2 * C::RAW + 2 * C::XS + 2 * C::STAGES + 2 + a); };
+    constexpr uint32_t RAW_AT = C::XS * 2 * C::X_BYTES;
     constexpr int W_OP = C::DRAIN, W_MMA = W_OP + 4, W_CODES = W_MMA + 1, W_X = W_CODES + 1;  // warps by role (W_OP a multiple of 4)
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int split = P.split, rank = blockIdx.x % split;
     const int64_t col_base = static_cast<int64_t>(blockIdx.x / split) * MM_COLS, row_base = static_cast<int64_t>(blockIdx.y) * ROWS;
     const int rows = static_cast<int>(P.m - row_base < ROWS ? P.m - row_base : ROWS);
-    const int64_t all_blocks = (P.groups + C::GPB - 1) / C::GPB;
-    const int64_t b_begin = all_blocks * rank / split;
-    const int blocks = static_cast<int>(all_blocks * (rank + 1) / split - b_begin);  // of 128 k, this CTA's
+    // this CTA's share: pieces of 128 k, groups, blocks
+    const int64_t all_pieces = (P.groups + C::GPP - 1) / C::GPP, p_begin = all_pieces * rank / split, p_end = all_pieces * (rank + 1) / split;
+    const int pieces = static_cast<int>(p_end - p_begin), blocks = (pieces + 1) / 2;
+    const int groups = static_cast<int>((p_end * C::GPP < P.groups ? p_end * C::GPP : P.groups) - p_begin * C::GPP);
 
     if (tid == 0) {
         abort_flag = 0;
         for (int i = 0; i < C::RAW; ++i) { mbar_init(raw_full(i), 1); mbar_init(raw_empty(i), 4); }
-        for (int s = 0; s < C::STAGES; ++s) {
-            mbar_init(x_full(s), 1);
-            mbar_init(x_empty(s), 1 + C::DRAIN);
-            mbar_init(op_full(s), 4);
-            mbar_init(op_empty(s), 1);
-        }
-        for (int a = 0; a < C::ACCS; ++a) { mbar_init(acc_full(a), 1); mbar_init(acc_empty(a), C::DRAIN); }
+        for (int i = 0; i < C::XS; ++i) { mbar_init(x_full(i), 1); mbar_init(x_empty(i), 1 + C::DRAIN); }
+        for (int s = 0; s < C::STAGES; ++s) { mbar_init(op_full(s), 4); mbar_init(op_empty(s), 1); }
+        for (int a = 0; a < 2; ++a) { mbar_init(acc_full(a), 1); mbar_init(acc_empty(a), C::DRAIN); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == W_MMA) tmem_alloc<1>(smem_u32(&tmem_slot), C::TMEM_COLS);
     fence_before();
     __syncthreads();
     fence_after();
-    const uint32_t tmem = tmem_slot, op_tmem = tmem + C::N * C::ACCS;
+    const uint32_t tmem = tmem_slot, op_tmem = tmem + 2 * C::BATCH * C::N;
 
     float result[C::MINE];
 #pragma unroll
@@ -273,19 +272,20 @@ w4_matmul_kernel(const __grid_constant__ CUtensorMap codes, const MmArgs P) {
                 const int i = b % C::RAW;
                 if (!mbar_wait(raw_empty(i), ((b / C::RAW) & 1) ^ 1u, &abort_flag, &g_w4_status, 0x100 | i)) break;
                 mbar_expect_tx(raw_full(i), MM_RAW_BYTES);
-                tma_load_2d(base + RAW_AT + i * MM_RAW_BYTES, &codes, raw_full(i), static_cast<int>((b_begin + b) * (MM_BLOCK / 8)), static_cast<int>(col_base));
+                tma_load_2d(base + RAW_AT + i * MM_RAW_BYTES, &codes, raw_full(i), static_cast<int>(p_begin * (MM_PIECE / 8)) + b * (MM_BLOCK / 8), static_cast<int>(col_base));
             }
         }
     } else if (warp == W_X) {
         // ------------------------------ x: global -> shared ------------------------------
         if (lane == 0) {
             asm volatile("griddepcontrol.wait;" ::: "memory");  // x's digits are there
-            const uint8_t* from = P.image + (blockIdx.y * all_blocks + b_begin) * C::X_BYTES;
+            const uint8_t* from = P.image + (blockIdx.y * all_pieces + p_begin) * C::X_BYTES;
             for (int b = 0; b < blocks; ++b) {
-                const int st = b % C::STAGES;
-                if (!mbar_wait(x_empty(st), ((b / C::STAGES) & 1) ^ 1u, &abort_flag, &g_w4_status, 0x180 | st)) break;
-                mbar_expect_tx(x_full(st), C::X_BYTES);
-                bulk_load(base + st * C::X_STAGE, from + static_cast<int64_t>(b) * C::X_BYTES, C::X_BYTES, x_full(st));
+                const int i = b % C::XS;
+                const uint32_t bytes = (2 * b + 1 < pieces ? 2 : 1) * C::X_BYTES;
+                if (!mbar_wait(x_empty(i), ((b / C::XS) & 1) ^ 1u, &abort_flag, &g_w4_status, 0x180 | i)) break;
+                mbar_expect_tx(x_full(i), bytes);
+                bulk_load(base + i * 2 * C::X_BYTES, from + static_cast<int64_t>(b) * 2 * C::X_BYTES, bytes, x_full(i));
             }
         }
     } else if (warp >= W_OP && warp < W_MMA) {
@@ -294,26 +294,33 @@ w4_matmul_kernel(const __grid_constant__ CUtensorMap codes, const MmArgs P) {
         for (int b = 0; b < blocks; ++b) {
             const int i = b % C::RAW, st = b % C::STAGES;
             if (!mbar_wait(raw_full(i), (b / C::RAW) & 1, &abort_flag, &g_w4_status, 0x400 | i)) break;
-            const uint8_t* raw = smem + RAW_AT + i * MM_RAW_BYTES + row * 64;
-            uint32_t o[32];
+            const uint8_t* raw = smem + RAW_AT + i * MM_RAW_BYTES + row * 128;
+            uint4 w[8];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {  // (the copy's 64-byte swizzle: 16-byte pieces XOR row / 2 % 4)
-                const uint4 w = *reinterpret_cast<const uint4*>(raw + ((c ^ ((row >> 1) & 3)) << 4));
-                constexpr uint32_t M = 0x0F0F0F0Fu;
-                o[c * 8] = w.x & M; o[c * 8 + 1] = (w.x >> 4) & M;
-                o[c * 8 + 2] = w.y & M; o[c * 8 + 3] = (w.y >> 4) & M;
-                o[c * 8 + 4] = w.z & M; o[c * 8 + 5] = (w.z >> 4) & M;
-                o[c * 8 + 6] = w.w & M; o[c * 8 + 7] = (w.w >> 4) & M;
-            }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(raw_empty(i));
+            for (int c = 0; c < 8; ++c) w[c] = *reinterpret_cast<const uint4*>(raw + ((c ^ (row & 7)) << 4));  // (the copy's 128-byte swizzle)
             if (!mbar_wait(op_empty(st), ((b / C::STAGES) & 1) ^ 1u, &abort_flag, &g_w4_status, 0x410 | st)) break;
             fence_after();
-            tmem_st32(op_tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + st * MM_A_COLS, o);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint32_t o[32];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const uint4 v = w[h * 4 + c];
+                    constexpr uint32_t M = 0x0F0F0F0Fu;
+                    o[c * 8] = v.x & M; o[c * 8 + 1] = (v.x >> 4) & M;
+                    o[c * 8 + 2] = v.y & M; o[c * 8 + 3] = (v.y >> 4) & M;
+                    o[c * 8 + 4] = v.z & M; o[c * 8 + 5] = (v.z >> 4) & M;
+                    o[c * 8 + 6] = v.w & M; o[c * 8 + 7] = (v.w >> 4) & M;
+                }
+                tmem_st32(op_tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + st * MM_A_COLS + h * 32, o);
+            }
             tmem_st_wait();
             fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(op_full(st));
+            if (lane == 0) {
+                mbar_arrive(op_full(st));
+                mbar_arrive(raw_empty(i));
+            }
         }
     } else if (warp == W_MMA) {
         // ------------------------------ products ------------------------------
@@ -322,42 +329,43 @@ w4_matmul_kernel(const __grid_constant__ CUtensorMap codes, const MmArgs P) {
         uint32_t acc_phase = 0;
         bool ok = true;
         for (int b = 0; b < blocks && ok; ++b) {
-            const int st = b % C::STAGES;
-            const uint32_t parity = (b / C::STAGES) & 1;
-            if (!mbar_wait(x_full(st), parity, &abort_flag, &g_w4_status, 0x200 | st)) break;
-            if (!mbar_wait(op_full(st), parity, &abort_flag, &g_w4_status, 0x208 | st)) break;
-            const uint64_t x = make_desc(base + st * C::X_STAGE, 0);
-            const int64_t left = P.groups - (b_begin + b) * C::GPB;
-            const int here = left < C::GPB ? static_cast<int>(left) : C::GPB;
+            const int st = b % C::STAGES, xi = b % C::XS;
+            const int here = groups - b * C::GPB < C::GPB ? groups - b * C::GPB : C::GPB;
+            if (!mbar_wait(x_full(xi), (b / C::XS) & 1, &abort_flag, &g_w4_status, 0x200 | xi)) break;
+            if (!mbar_wait(op_full(st), (b / C::STAGES) & 1, &abort_flag, &g_w4_status, 0x208 | st)) break;
+            const uint64_t x = make_desc(base + xi * 2 * C::X_BYTES, 0);
 #pragma unroll
-            for (int g = 0; g < C::GPB; ++g) {
-                if (g >= here) break;
+            for (int g0 = 0; g0 < C::GPB; g0 += C::BATCH) {
+                if (g0 >= here) break;
                 if (!mbar_wait(acc_empty(acc), acc_phase ^ 1u, &abort_flag, &g_w4_status, 0x210 | acc)) { ok = false; break; }
                 fence_after();
                 __syncwarp();
                 if (elect_one()) {
 #pragma unroll
-                    for (int ks = 0; ks < GROUP / 32; ++ks) {
-                        const int k32 = g * (GROUP / 32) + ks;
-                        mma_f8_ts(tmem + acc * C::N, op_tmem + st * MM_A_COLS + k32 * 8, x + k32 * 2, idesc, ks > 0);
+                    for (int i = 0; i < C::BATCH; ++i) {
+                        const int g = g0 + i;
+                        if (g >= here) break;
+#pragma unroll
+                        for (int ks = 0; ks < GROUP / 32; ++ks) {
+                            const int k32 = g * (GROUP / 32) + ks;  // of the block; four of them are a piece of x
+                            mma_f8_ts(tmem + (acc * C::BATCH + i) * C::N, op_tmem + st * MM_A_COLS + k32 * 8, x + (k32 / 4) * (C::X_BYTES / 16) + (k32 % 4) * 2, idesc, ks > 0);
+                        }
                     }
                     commit<1>(acc_full(acc));
+                    if (g0 + C::BATCH >= here) {
+                        commit<1>(op_empty(st));
+                        commit<1>(x_empty(xi));
+                    }
                 }
-                if (++acc == C::ACCS) { acc = 0; acc_phase ^= 1u; }
-            }
-            __syncwarp();
-            if (ok && elect_one()) {
-                commit<1>(op_empty(st));
-                commit<1>(x_empty(st));
+                acc ^= 1;
+                acc_phase ^= static_cast<uint32_t>(acc == 0);
             }
         }
     } else {
         // ------------------------------ results ------------------------------
         const int quarter = warp & 3, r_first = (warp >> 2) * C::MINE;  // columns of the tile, rows of x
-        const int64_t col = col_base + quarter * 32 + lane, at = (col < P.n ? col : P.n - 1) * P.groups + b_begin * C::GPB;
+        const int64_t col = col_base + quarter * 32 + lane, at = (col < P.n ? col : P.n - 1) * P.groups + p_begin * C::GPP;
         const uint32_t t_row = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + r_first * 8;
-        const int64_t left = P.groups - b_begin * C::GPB;
-        const int groups = static_cast<int>(left < static_cast<int64_t>(blocks) * C::GPB ? left : static_cast<int64_t>(blocks) * C::GPB);
         // scales and zero points, each lane its own row of them, AHEAD groups in flight: a load's latency is several groups long
         float scale[C::AHEAD];
         uint32_t zero[C::AHEAD];
@@ -373,19 +381,23 @@ w4_matmul_kernel(const __grid_constant__ CUtensorMap codes, const MmArgs P) {
         for (int g0 = 0; g0 < groups && ok; g0 += C::AHEAD) {
 #pragma unroll
             for (int i = 0; i < C::AHEAD; ++i) {
-                const int gi = g0 + i, b = gi / C::GPB, st = b % C::STAGES, g = gi % C::GPB;
+                const int gi = g0 + i, b = gi / C::GPB, xi = b % C::XS, piece = (gi / C::GPP) & 1;
                 if (gi >= groups || !ok) break;
-                const float* sums = reinterpret_cast<const float*>(smem + st * C::X_STAGE + C::B_BYTES);
-                const float* step = sums + C::GPB * ROWS * 4 + r_first;
-                sums += (g * ROWS + r_first) * 4;
-                if (g == 0 && !mbar_wait(x_full(st), (b / C::STAGES) & 1, &abort_flag, &g_w4_status, 0x300 | st)) { ok = false; break; }
+                const float* sums = reinterpret_cast<const float*>(smem + (xi * 2 + piece) * C::X_BYTES + C::B_BYTES);
+                const float* step = sums + C::GPP * ROWS * 4 + r_first;
+                sums += ((gi % C::GPP) * ROWS + r_first) * 4;
                 const float s = scale[i], z = -static_cast<float>(zero[i]);
                 fetch(scale[i], zero[i], gi + C::AHEAD);
-                if (!mbar_wait(acc_full(acc), acc_phase, &abort_flag, &g_w4_status, 0x310 | acc)) { ok = false; break; }
-                fence_after();
+                if (gi % C::GPB == 0 && !mbar_wait(x_full(xi), (b / C::XS) & 1, &abort_flag, &g_w4_status, 0x300 | xi)) { ok = false; break; }
+                if (gi % C::BATCH == 0) {
+                    if (!mbar_wait(acc_full(acc), acc_phase, &abort_flag, &g_w4_status, 0x310 | acc)) { ok = false; break; }
+                    fence_after();
+                }
+                const uint32_t t_acc = t_row + (acc * C::BATCH + gi % C::BATCH) * C::N;
+                const bool hand_over = gi % C::BATCH == C::BATCH - 1 || gi == groups - 1;
                 // two rows at a time, the next two on their way while these are joined
                 uint32_t d[2][16];
-                tmem_ld16(t_row + acc * C::N, d[0]);
+                tmem_ld16(t_acc, d[0]);
 #pragma unroll
                 for (int r0 = 0; r0 < C::MINE; r0 += 2) {
                     constexpr int LAST = C::MINE - 2;
@@ -398,8 +410,8 @@ w4_matmul_kernel(const __grid_constant__ CUtensorMap codes, const MmArgs P) {
                     }
                     tmem_ld_wait();
                     if (r0 < LAST) {
-                        tmem_ld16(t_row + acc * C::N + (r0 + 2) * 8, d[((r0 >> 1) + 1) & 1]);
-                    } else {  // read completely
+                        tmem_ld16(t_acc + (r0 + 2) * 8, d[((r0 >> 1) + 1) & 1]);
+                    } else if (hand_over) {  // read completely
                         fence_before();
                         __syncwarp();
                         if (lane == 0) mbar_arrive(acc_empty(acc));
@@ -412,10 +424,13 @@ w4_matmul_kernel(const __grid_constant__ CUtensorMap codes, const MmArgs P) {
                         result[r0 + r] = fmaf(fmaf(fmaf(w3, 256.0f, w2), 65536.0f, fmaf(w1, 256.0f, w0)), up[r], result[r0 + r]);
                     }
                 }
-                if (++acc == C::ACCS) { acc = 0; acc_phase ^= 1u; }
-                if (g == C::GPB - 1 || gi == groups - 1) {
+                if (hand_over) {
+                    acc ^= 1;
+                    acc_phase ^= static_cast<uint32_t>(acc == 0);
+                }
+                if (gi % C::GPB == C::GPB - 1 || gi == groups - 1) {
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(x_empty(st));
+                    if (lane == 0) mbar_arrive(x_empty(xi));
                 }
             }
         }
@@ -463,23 +478,23 @@ ctk_status launch_matmul(MmArgs P, cudaStream_t st) {
     auto kernel = w4_matmul_kernel<GROUP, ROWS>;
     static ctk::PerDeviceOnce attr_set;
     if (attr_set.first()) CTK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
-    const int64_t col_blocks = (P.n + MM_COLS - 1) / MM_COLS, row_blocks = (P.m + ROWS - 1) / ROWS, k_blocks = (P.groups + C::GPB - 1) / C::GPB;
-    // split k over a cluster while that fills idle SMs and leaves a CTA two blocks
+    const int64_t col_blocks = (P.n + MM_COLS - 1) / MM_COLS, row_blocks = (P.m + ROWS - 1) / ROWS, pieces = (P.groups + C::GPP - 1) / C::GPP;
+    // split k over a cluster while that fills idle SMs and leaves a CTA two pieces of k
     P.split = 1;
-    while (P.split < 8 && col_blocks * row_blocks * P.split * 2 <= 3 * ctk::sm_count() && k_blocks >= P.split * 4) P.split *= 2;
+    while (P.split < 8 && col_blocks * row_blocks * P.split * 2 <= 3 * ctk::sm_count() && pieces >= P.split * 4) P.split *= 2;
     if (col_blocks * P.split > 0x7FFFFFFF || row_blocks * ROWS > 65535) return fail(CTK_ERR_LIMIT, "ctk_w4_matmul_f32: too many rows or columns");
     StreamScratch scratch;
-    if (k_blocks) {
-        ctk_status rc = scratch.get(static_cast<size_t>(row_blocks * k_blocks) * C::X_BYTES, st);
+    if (pieces) {
+        ctk_status rc = scratch.get(static_cast<size_t>(row_blocks * pieces) * C::X_BYTES, st);
         if (rc) return rc;
         uint8_t* image = static_cast<uint8_t*>(scratch.p);
         P.image = image;
-        w4_digits_kernel<GROUP, ROWS><<<dim3(static_cast<unsigned>((k_blocks + 3) / 4), static_cast<unsigned>(row_blocks * ROWS)), 128, 0, st>>>(P.x, P.ldx, P.m, P.k, k_blocks, image);
+        w4_digits_kernel<GROUP, ROWS><<<dim3(static_cast<unsigned>((pieces + 3) / 4), static_cast<unsigned>(row_blocks * ROWS)), 128, 0, st>>>(P.x, P.ldx, P.m, P.k, pieces, image);
         CTK_LAUNCH_CHECK("w4_digits");
     }
-    // the codes as a matrix of 32-bit words, 128 columns x 16 words a copy; what lies past its extents reads as zero
+    // the codes as a matrix of 32-bit words, 128 columns x 32 words a copy; what lies past its extents reads as zero
     CUtensorMap codes = {};
-    if (k_blocks) {
+    if (pieces) {
         t5::EncodeTiledFn enc;
         ctk_status rc = t5::get_encoder(&enc);
         if (rc) return rc;
@@ -487,7 +502,7 @@ ctk_status launch_matmul(MmArgs P, cudaStream_t st) {
         const cuuint64_t dims[2] = {words, static_cast<cuuint64_t>(P.n)}, strides[1] = {words * 4};
         const cuuint32_t box[2] = {MM_BLOCK / 8, MM_COLS}, estr[2] = {1u, 1u};
         const CUresult r = enc(&codes, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<uint32_t*>(P.packed), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                               CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
         if (r != CUDA_SUCCESS) return fail(CTK_ERR_CUDA, "cuTensorMapEncodeTiled failed with code " + std::to_string(static_cast<int>(r)));
     }
     cudaLaunchConfig_t cfg = {};
@@ -503,7 +518,7 @@ ctk_status launch_matmul(MmArgs P, cudaStream_t st) {
     cfg.dynamicSmemBytes = C::SMEM;
     cfg.stream = st;
     cfg.attrs = attr;
-    cfg.numAttrs = k_blocks ? 2 : 1;  // (without k there is nothing in front of it to wait for in the kernel)
+    cfg.numAttrs = pieces ? 2 : 1;  // (without k there is nothing in front of it to wait for in the kernel)
     CTK_CUDA(cudaLaunchKernelEx(&cfg, kernel, codes, P));
     CTK_LAUNCH_CHECK("w4_matmul");
     return CTK_OK;
