@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(W4_THREADS) w4_dequantize_kernel(const uint32_
 //   4 warps     a thread per column: its 128 bytes of codes, masked, into the operand's place in tensor memory;
 //   1 warp      the products: one instruction per 32 k, an accumulator [128 columns][(row, digit)] per group, BATCH groups to a
 //               hand-over;
-//   4 or 8      a thread per column: digits joined, zero point, scale, added to the column's results.
+//   4 or 16     a thread per column: digits joined, zero point, scale, added to the column's results.
 // A hand-over between warps (an mbarrier's arrival and wait) takes some 200 clocks, the bytes of 128 columns x 128 k take 180 at
 // HBM's rate: hence the large blocks.  Before this: mma.sync with x cut into three bf16 parts (about 32 clocks an instruction on
 // this machine) 95 us for 4 x 16384 x 16384 and 46 us for 64 x 4096 x 4096; the operand in shared memory, its codes through
@@ -141,11 +141,12 @@ struct MmCfg {
     static constexpr int X_BYTES = (B_BYTES + T_BYTES + 1023) / 1024 * 1024; // a piece of x as the first kernel leaves it
     static constexpr int RING = RAW * MM_RAW_BYTES + XS * 2 * X_BYTES, R_BYTES = ROWS * R_PITCH * 4;
     static constexpr int SMEM = (RING > R_BYTES ? RING : R_BYTES) + 1024;
-    static constexpr int DRAIN = ROWS <= 8 ? 4 : 8;  // warps that take the accumulators: 4, or 8 with half of the rows each
+    static constexpr int DRAIN = ROWS <= 8 ? 4 : 16; // warps that take the accumulators: 4, or 16 with a quarter of the rows each
     static constexpr int MINE = ROWS * 4 / DRAIN;    // rows of such a warp
-    static constexpr int AHEAD = ROWS <= 4 ? 8 : 4;  // groups whose scales are in flight
+    static constexpr int RC = 2;                     // rows joined at a time
+    static constexpr int U = GPB < 4 ? GPB : 4;      // groups whose scales are read together
     static constexpr int THREADS = (DRAIN + 4 + 3) * 32;
-    static_assert(USED_COLS <= 512 && SMEM * PER_SM <= 225 * 1024 && MINE % 2 == 0 && GPB % BATCH == 0, "");
+    static_assert(USED_COLS <= 512 && SMEM * PER_SM <= 225 * 1024 && MINE % 2 == 0 && GPB % BATCH == 0 && BATCH <= 4, "");
 };
 
 __device__ int g_w4_status = 0;  // first bounded wait that ran out, else 0
@@ -161,6 +162,7 @@ struct MmArgs {
     int64_t ldy;
     int64_t m, k, n, groups;
     int relu, split;
+    int quads;             // scales and zero points can be read four at a time
     const uint8_t* image;  // x's digits, [row block][piece][X_BYTES]
 };
 
@@ -243,7 +245,10 @@ w4_matmul_kernel(const __grid_constant__ CUtensorMap codes, const MmArgs P) {
     const int64_t col_base = static_cast<int64_t>(blockIdx.x / split) * MM_COLS, row_base = static_cast<int64_t>(blockIdx.y) * ROWS;
     const int rows = static_cast<int>(P.m - row_base < ROWS ? P.m - row_base : ROWS);
     // this CTA's share: pieces of 128 k, groups, blocks
-    const int64_t all_pieces = (P.groups + C::GPP - 1) / C::GPP, p_begin = all_pieces * rank / split, p_end = all_pieces * (rank + 1) / split;
+    // (a share starts at a multiple of four groups, so that their scales can be read together)
+    constexpr int QUAD = C::GPP >= 4 ? 1 : 4 / C::GPP;
+    const int64_t all_pieces = (P.groups + C::GPP - 1) / C::GPP, p_begin = all_pieces * rank / split / QUAD * QUAD;
+    const int64_t p_end = rank + 1 == split ? all_pieces : all_pieces * (rank + 1) / split / QUAD * QUAD;
     const int pieces = static_cast<int>(p_end - p_begin), blocks = (pieces + 1) / 2;
     const int groups = static_cast<int>((p_end * C::GPP < P.groups ? p_end * C::GPP : P.groups) - p_begin * C::GPP);
 
@@ -366,72 +371,101 @@ w4_matmul_kernel(const __grid_constant__ CUtensorMap codes, const MmArgs P) {
         const int quarter = warp & 3, r_first = (warp >> 2) * C::MINE;  // columns of the tile, rows of x
         const int64_t col = col_base + quarter * 32 + lane, at = (col < P.n ? col : P.n - 1) * P.groups + p_begin * C::GPP;
         const uint32_t t_row = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + r_first * 8;
-        // scales and zero points, each lane its own row of them, AHEAD groups in flight: a load's latency is several groups long
-        float scale[C::AHEAD];
-        uint32_t zero[C::AHEAD];
-        auto fetch = [&](float& s, uint32_t& z, int g) {
-            s = g < groups ? __ldg(P.scales + at + g) : 0.0f;
-            z = g < groups && P.zeros ? __ldg(P.zeros + at + g) : 8u;
-        };
-#pragma unroll
-        for (int i = 0; i < C::AHEAD; ++i) fetch(scale[i], zero[i], i);
-        int acc = 0;
-        uint32_t acc_phase = 0;
-        bool ok = true;
-        for (int g0 = 0; g0 < groups && ok; g0 += C::AHEAD) {
-#pragma unroll
-            for (int i = 0; i < C::AHEAD; ++i) {
-                const int gi = g0 + i, b = gi / C::GPB, xi = b % C::XS, piece = (gi / C::GPP) & 1;
-                if (gi >= groups || !ok) break;
-                const float* sums = reinterpret_cast<const float*>(smem + (xi * 2 + piece) * C::X_BYTES + C::B_BYTES);
-                const float* step = sums + C::GPP * ROWS * 4 + r_first;
-                sums += ((gi % C::GPP) * ROWS + r_first) * 4;
-                const float s = scale[i], z = -static_cast<float>(zero[i]);
-                fetch(scale[i], zero[i], gi + C::AHEAD);
-                if (gi % C::GPB == 0 && !mbar_wait(x_full(xi), (b / C::XS) & 1, &abort_flag, &g_w4_status, 0x300 | xi)) { ok = false; break; }
-                if (gi % C::BATCH == 0) {
-                    if (!mbar_wait(acc_full(acc), acc_phase, &abort_flag, &g_w4_status, 0x310 | acc)) { ok = false; break; }
-                    fence_after();
+        // Scales and zero points, each lane its own row of them: U groups at a time, two such units ahead (a load's latency is
+        // several groups long).  Read together where rows of them are aligned for it: one by one, each brings its sector of
+        // 32 bytes from L2 again.
+        constexpr int U = C::U;
+        float scale[U], scale1[U], scale2[U];
+        uint32_t zero = 0, zero1 = 0, zero2 = 0;
+        auto fetch = [&](float (&s)[U], uint32_t& z, int g) {
+            z = 0x08080808u;
+            if (g >= groups) return;
+            const float* ps = P.scales + at + g;
+            const uint8_t* pz = P.zeros + at + g;
+            if (P.quads) {
+                if constexpr (U == 4) {
+                    *reinterpret_cast<float4*>(s) = __ldg(reinterpret_cast<const float4*>(ps));
+                    if (P.zeros) z = __ldg(reinterpret_cast<const uint32_t*>(pz));
+                } else {
+                    *reinterpret_cast<float2*>(s) = __ldg(reinterpret_cast<const float2*>(ps));
+                    if (P.zeros) z = __ldg(reinterpret_cast<const uint16_t*>(pz));
                 }
-                const uint32_t t_acc = t_row + (acc * C::BATCH + gi % C::BATCH) * C::N;
-                const bool hand_over = gi % C::BATCH == C::BATCH - 1 || gi == groups - 1;
-                // two rows at a time, the next two on their way while these are joined
-                uint32_t d[2][16];
-                tmem_ld16(t_acc, d[0]);
+                return;
+            }
+            uint32_t w = 0;
 #pragma unroll
-                for (int r0 = 0; r0 < C::MINE; r0 += 2) {
-                    constexpr int LAST = C::MINE - 2;
-                    float4 ds[2];
-                    float up[2];
+            for (int e = 0; e < U; ++e) {
+                s[e] = g + e < groups ? __ldg(ps + e) : 0.0f;
+                if (P.zeros && g + e < groups) w |= static_cast<uint32_t>(__ldg(pz + e)) << (8 * e);
+            }
+            if (P.zeros) z = w;
+        };
+        fetch(scale1, zero1, 0);
+        fetch(scale2, zero2, U);
+        int acc = 0, xi = 0;
+        uint32_t acc_phase = 0, x_phase = 0;
+        bool ok = true;
+        // A unit of U groups: code for each of them, so that what depends on the group's place costs nothing, but no more of it
+        // -- unrolled further it does not fit the instruction caches beside the other warps' and took up to twice the time.
+#pragma unroll 1
+        for (int g0 = 0; g0 < groups && ok; g0 += U) {
 #pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        ds[r] = *reinterpret_cast<const float4*>(sums + (r0 + r) * 4);
-                        up[r] = step[r0 + r] * s;
+            for (int e = 0; e < U; ++e) { scale[e] = scale1[e]; scale1[e] = scale2[e]; }
+            zero = zero1;
+            zero1 = zero2;
+            fetch(scale2, zero2, g0 + 2 * U);
+            const int in_block = C::GPB == U ? 0 : g0 % C::GPB;  // groups of the block before this unit
+            if (in_block == 0 && !mbar_wait(x_full(xi), x_phase, &abort_flag, &g_w4_status, 0x300 | xi)) break;
+            const uint8_t* x_block = smem + xi * 2 * C::X_BYTES + C::B_BYTES;
+#pragma unroll
+            for (int b0 = 0; b0 < U; b0 += C::BATCH) {
+                if (g0 + b0 >= groups) break;
+                if (!mbar_wait(acc_full(acc), acc_phase, &abort_flag, &g_w4_status, 0x310 | acc)) { ok = false; break; }
+                fence_after();
+                // RC rows of a group at a time, the next on their way while these are joined
+                constexpr int RC = C::RC, PER_GROUP = C::MINE / RC, CHUNKS = C::BATCH * PER_GROUP;
+                const uint32_t t_acc = t_row + acc * C::BATCH * C::N;
+                uint32_t d[2][RC * 8];
+                tmem_ld_cols(t_acc, d[0]);
+#pragma unroll
+                for (int c = 0; c < CHUNKS; ++c) {
+                    const int g = b0 + c / PER_GROUP, r0 = c % PER_GROUP * RC;  // group of the unit, first row
+                    const int gb = in_block + g;                               // ... of the block
+                    const float* tables = reinterpret_cast<const float*>(x_block + gb / C::GPP * C::X_BYTES);
+                    const float* sums = tables + ((gb % C::GPP) * ROWS + r_first + r0) * 4;
+                    const float* step = tables + C::GPP * ROWS * 4 + r_first + r0;
+                    const float z = -static_cast<float>((zero >> (8 * g)) & 255u);
+                    float4 ds[RC];
+                    float up[RC];
+#pragma unroll
+                    for (int r = 0; r < RC; ++r) {
+                        ds[r] = *reinterpret_cast<const float4*>(sums + r * 4);
+                        up[r] = step[r] * scale[g];
                     }
                     tmem_ld_wait();
-                    if (r0 < LAST) {
-                        tmem_ld16(t_acc + (r0 + 2) * 8, d[((r0 >> 1) + 1) & 1]);
-                    } else if (hand_over) {  // read completely
+                    if (c + 1 < CHUNKS) {
+                        tmem_ld_cols(t_acc + (c + 1) / PER_GROUP * C::N + (c + 1) % PER_GROUP * RC * 8, d[(c + 1) & 1]);
+                    } else {  // read completely
                         fence_before();
                         __syncwarp();
                         if (lane == 0) mbar_arrive(acc_empty(acc));
                     }
+                    if (g0 + g >= groups) continue;  // (a batch cut short: nothing was multiplied into this accumulator)
 #pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        const uint32_t* q = &d[(r0 >> 1) & 1][r * 8];
+                    for (int r = 0; r < RC; ++r) {
+                        const uint32_t* q = &d[c & 1][r * 8];
                         auto pair = [&](int e) { return fmaf(__uint_as_float(q[2 * e + 1]), 16.0f, __uint_as_float(q[2 * e])); };  // exact: below 2^19
                         const float w0 = fmaf(z, ds[r].x, pair(0)), w1 = fmaf(z, ds[r].y, pair(1)), w2 = fmaf(z, ds[r].z, pair(2)), w3 = fmaf(z, ds[r].w, pair(3));
                         result[r0 + r] = fmaf(fmaf(fmaf(w3, 256.0f, w2), 65536.0f, fmaf(w1, 256.0f, w0)), up[r], result[r0 + r]);
                     }
                 }
-                if (hand_over) {
-                    acc ^= 1;
-                    acc_phase ^= static_cast<uint32_t>(acc == 0);
-                }
-                if (gi % C::GPB == C::GPB - 1 || gi == groups - 1) {
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(x_empty(xi));
-                }
+                acc ^= 1;
+                acc_phase ^= static_cast<uint32_t>(acc == 0);
+            }
+            if (in_block + U == C::GPB || g0 + U >= groups) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(x_empty(xi));
+                if (++xi == C::XS) { xi = 0; x_phase ^= 1u; }
             }
         }
     }
@@ -479,9 +513,9 @@ ctk_status launch_matmul(MmArgs P, cudaStream_t st) {
     static ctk::PerDeviceOnce attr_set;
     if (attr_set.first()) CTK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
     const int64_t col_blocks = (P.n + MM_COLS - 1) / MM_COLS, row_blocks = (P.m + ROWS - 1) / ROWS, pieces = (P.groups + C::GPP - 1) / C::GPP;
-    // split k over a cluster while that fills idle SMs and leaves a CTA two pieces of k
+    // split k over a cluster while that fills idle SMs and leaves a CTA four groups of k
     P.split = 1;
-    while (P.split < 8 && col_blocks * row_blocks * P.split * 2 <= 3 * ctk::sm_count() && pieces >= P.split * 4) P.split *= 2;
+    while (P.split < 8 && col_blocks * row_blocks * P.split * 2 <= 3 * ctk::sm_count() && pieces >= P.split * 2 * (C::GPP >= 4 ? 1 : 4 / C::GPP)) P.split *= 2;
     if (col_blocks * P.split > 0x7FFFFFFF || row_blocks * ROWS > 65535) return fail(CTK_ERR_LIMIT, "ctk_w4_matmul_f32: too many rows or columns");
     StreamScratch scratch;
     if (pieces) {
@@ -609,6 +643,7 @@ ctk_status ctk_w4_matmul_f32(const float* x, int64_t ldx, const uint32_t* packed
     P.n = n;
     P.groups = (k + group - 1) / group;
     P.relu = relu;
+    P.quads = P.groups % 4 == 0 && aligned_to(scales, 16) && aligned_to(zeros, 4);
     cudaStream_t st = as_stream(stream);
     return group == 32 ? matmul_rows<32>(P, st) : group == 64 ? matmul_rows<64>(P, st) : matmul_rows<128>(P, st);
 }
