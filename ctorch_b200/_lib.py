@@ -46,6 +46,12 @@ def load():
     L.ctk_matmul_split_bytes.argtypes = [ctypes.c_int64, ctypes.c_int64]
     L.ctk_orthogonalize_workspace_bytes.restype = ctypes.c_size_t
     L.ctk_w4_packed_bytes.restype = ctypes.c_size_t
+    p, i64, i32, f32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float
+    L.ctk_orthogonalize_f32.argtypes = [p, i64, p, i64, i64, i64, i32, f32, p, p]
+    L.ctk_muon_update_f32.argtypes = [p, i64, p, i64, p, i64, i64, i64, f32, f32, i32, f32, f32, i32, f32, p, p]
+    L.ctk_w4_quantize_f32.argtypes = [p, i64, i64, i64, i32, p, p, p, p]
+    L.ctk_w4_dequantize_f32.argtypes = [p, p, p, i64, i64, i32, p, i64, p]
+    L.ctk_w4_matmul_f32.argtypes = [p, i64, p, p, p, p, i32, p, i64, i64, i64, i64, i32, p]
     L.cth_last_error.restype = ctypes.c_char_p
     L.cth_error_count.restype = ctypes.c_uint64
     _lib = L

@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(W4_THREADS) w4_dequantize_kernel(const uint32_
 //   4 warps     a thread per column: its 128 bytes of codes, masked, into the operand's place in tensor memory;
 //   1 warp      the products: one instruction per 32 k, an accumulator [128 columns][(row, digit)] per group, BATCH groups to a
 //               hand-over;
-//   4 or 16     a thread per column: digits joined, zero point, scale, added to the column's results.
+//   4 or 8      a thread per column: digits joined, zero point, scale, added to the column's results.
 // A hand-over between warps (an mbarrier's arrival and wait) takes some 200 clocks, the bytes of 128 columns x 128 k take 180 at
 // HBM's rate: hence the large blocks.  Before this: mma.sync with x cut into three bf16 parts (about 32 clocks an instruction on
 // this machine) 95 us for 4 x 16384 x 16384 and 46 us for 64 x 4096 x 4096; the operand in shared memory, its codes through
@@ -141,9 +141,9 @@ struct MmCfg {
     static constexpr int X_BYTES = (B_BYTES + T_BYTES + 1023) / 1024 * 1024; // a piece of x as the first kernel leaves it
     static constexpr int RING = RAW * MM_RAW_BYTES + XS * 2 * X_BYTES, R_BYTES = ROWS * R_PITCH * 4;
     static constexpr int SMEM = (RING > R_BYTES ? RING : R_BYTES) + 1024;
-    static constexpr int DRAIN = ROWS <= 8 ? 4 : 16; // warps that take the accumulators: 4, or 16 with a quarter of the rows each
+    static constexpr int DRAIN = ROWS <= 8 ? 4 : 8;  // warps that take the accumulators: 4, or 8 with half of the rows each
     static constexpr int MINE = ROWS * 4 / DRAIN;    // rows of such a warp
-    static constexpr int RC = 2;                     // rows joined at a time
+    static constexpr int RC = ROWS <= 8 ? 2 : 4;     // rows joined at a time
     static constexpr int U = GPB < 4 ? GPB : 4;      // groups whose scales are read together
     static constexpr int THREADS = (DRAIN + 4 + 3) * 32;
     static_assert(USED_COLS <= 512 && SMEM * PER_SM <= 225 * 1024 && MINE % 2 == 0 && GPB % BATCH == 0 && BATCH <= 4, "");
@@ -507,15 +507,13 @@ w4_matmul_kernel(const __grid_constant__ CUtensorMap codes, const MmArgs P) {
 }
 
 template <int GROUP, int ROWS>
-ctk_status launch_matmul(MmArgs P, cudaStream_t st) {
+ctk_status launch_matmul(MmArgs P, int split, cudaStream_t st) {
     using C = MmCfg<GROUP, ROWS>;
     auto kernel = w4_matmul_kernel<GROUP, ROWS>;
     static ctk::PerDeviceOnce attr_set;
     if (attr_set.first()) CTK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
     const int64_t col_blocks = (P.n + MM_COLS - 1) / MM_COLS, row_blocks = (P.m + ROWS - 1) / ROWS, pieces = (P.groups + C::GPP - 1) / C::GPP;
-    // split k over a cluster while that fills idle SMs and leaves a CTA four groups of k
-    P.split = 1;
-    while (P.split < 8 && col_blocks * row_blocks * P.split * 2 <= 3 * ctk::sm_count() && pieces >= P.split * 2 * (C::GPP >= 4 ? 1 : 4 / C::GPP)) P.split *= 2;
+    P.split = split;
     if (col_blocks * P.split > 0x7FFFFFFF || row_blocks * ROWS > 65535) return fail(CTK_ERR_LIMIT, "ctk_w4_matmul_f32: too many rows or columns");
     StreamScratch scratch;
     if (pieces) {
@@ -557,13 +555,46 @@ ctk_status launch_matmul(MmArgs P, cudaStream_t st) {
     CTK_LAUNCH_CHECK("w4_matmul");
     return CTK_OK;
 }
+// How many rows a CTA takes and how many CTAs share a column's k: the pair with the least estimated time.  A CTA's start and end
+// cost START clocks (barriers, first loads, the cluster's sums), a block of 256 k in an SM that is full (two CTAs up to 8 rows,
+// one above) PER_BLOCK; alone on its SM a CTA of few rows is 1.4 times slower per block.  From 16384 x 16384 g128: 31.6 / 36 /
+// 45 / 68 us with 2 / 4 / 8 / 16 rows, 253 us for 64 rows in three passes of 24.  So 64 x 4096 x 4096 takes 16 rows and whole
+// columns (128 CTAs: 21.6 us; 24 rows and a split of 4: 31.8 us; 8 rows: 23.2 us) and 1 x 4096 x 4096 2 rows and a split of 8.
+struct Shape {
+    int rows, split;
+};
+Shape pick_shape(int64_t m, int64_t n, int64_t groups, int group) {
+    constexpr int ROWS[5] = {2, 4, 8, 16, 24}, PER_SM[5] = {2, 2, 2, 1, 1};
+    constexpr double PER_BLOCK[5] = {1060, 1200, 1490, 2330, 2900}, START = 5000;
+    const int64_t sms = ctk::sm_count(), cols = (n + MM_COLS - 1) / MM_COLS, blocks = (groups * group + MM_BLOCK - 1) / MM_BLOCK;
+    Shape best = {24, 1};
+    double least = 1e300;
+    for (int i = 0; i < 5; ++i) {
+        if (i && ROWS[i - 1] >= m) break;  // fewer rows hold them all
+        const int64_t row_blocks = (m + ROWS[i] - 1) / ROWS[i];
+        for (int split = 1; split <= 8 && (split == 1 || groups >= 8 * split); split *= 2) {
+            const int64_t ctas = cols * row_blocks * split, waves = (ctas + sms * PER_SM[i] - 1) / (sms * PER_SM[i]);
+            const bool alone = PER_SM[i] == 2 && ctas <= sms;
+            const double per_cta = static_cast<double>((blocks + split - 1) / split);
+            const double t = static_cast<double>(waves) * (START + per_cta * PER_BLOCK[i] * (alone ? 1.4 : PER_SM[i]));
+            if (t < least) {
+                least = t;
+                best = {ROWS[i], split};
+            }
+        }
+    }
+    return best;
+}
 template <int GROUP>
 ctk_status matmul_rows(const MmArgs& P, cudaStream_t st) {
-    if (P.m <= 2) return launch_matmul<GROUP, 2>(P, st);
-    if (P.m <= 4) return launch_matmul<GROUP, 4>(P, st);
-    if (P.m <= 8) return launch_matmul<GROUP, 8>(P, st);
-    if (P.m <= 16) return launch_matmul<GROUP, 16>(P, st);
-    return launch_matmul<GROUP, 24>(P, st);
+    const Shape s = pick_shape(P.m, P.n, P.groups, GROUP);
+    switch (s.rows) {
+        case 2: return launch_matmul<GROUP, 2>(P, s.split, st);
+        case 4: return launch_matmul<GROUP, 4>(P, s.split, st);
+        case 8: return launch_matmul<GROUP, 8>(P, s.split, st);
+        case 16: return launch_matmul<GROUP, 16>(P, s.split, st);
+        default: return launch_matmul<GROUP, 24>(P, s.split, st);
+    }
 }
 
 bool group_ok(int group) { return group == 32 || group == 64 || group == 128; }
@@ -646,6 +677,13 @@ ctk_status ctk_w4_matmul_f32(const float* x, int64_t ldx, const uint32_t* packed
     P.quads = P.groups % 4 == 0 && aligned_to(scales, 16) && aligned_to(zeros, 4);
     cudaStream_t st = as_stream(stream);
     return group == 32 ? matmul_rows<32>(P, st) : group == 64 ? matmul_rows<64>(P, st) : matmul_rows<128>(P, st);
+}
+
+ctk_status ctk_w4_status(int* status) {
+    CTK_REQUIRE(status, "ctk_w4_status: null pointer");
+    CTK_CUDA(cudaDeviceSynchronize());
+    CTK_CUDA(cudaMemcpyFromSymbol(status, g_w4_status, sizeof(int)));
+    return CTK_OK;
 }
 
 }  // extern "C"

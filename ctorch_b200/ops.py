@@ -233,21 +233,40 @@ def sgd_update_split(p, g, lr, stream=None):
     return _decode_split(split, outer, inner, p)
 
 
-# ---- orthogonalised updates ---------------------------------------------------------------------------
-def _pitch(a, what):
+# ---- orthogonalised updates and 4-bit weights -----------------------------------------------------------
+# (These calls take microseconds on the device, so their way there is short: argument types are declared once, in
+# _lib, and pointers and sizes go over as plain ints.)
+_fns = {}
+
+
+def _fn(name):
+    f = _fns.get(name)
+    if f is None:
+        f = _fns[name] = getattr(lib, name)
+    return f
+
+
+def _s(stream):
+    return None if stream is None else _sh(stream)
+
+
+def _matrix(a, what):
     if len(a.shape) != 2:
         raise ValueError(f"{what}: a 2-D array expected, got shape {a.shape}")
-    return _i64(max(a.shape[1], 1))
+    return a.shape
 
 
 def orthogonalize(g, steps=5, eps=1e-7, out=None, workspace=None, stream=None):
     """NS(g): g's singular vectors with singular values near 1 (Newton-Schulz steps)."""
-    ld = _pitch(g, "orthogonalize")
-    out = out or DeviceArray(g.shape)
-    if out.shape != g.shape:
+    rows, cols = _matrix(g, "orthogonalize")
+    if out is None:
+        out = DeviceArray(g.shape)
+    elif out.shape != g.shape:
         raise ValueError(f"orthogonalize: out has shape {out.shape}, g {g.shape}")
-    check(lib.ctk_orthogonalize_f32(g.p, ld, out.p, ld, _i64(g.shape[0]), _i64(g.shape[1]), int(steps), _f(eps),
-                                    workspace.p if workspace else None, _sh(stream)))
+    ld = cols or 1
+    st = _fn("ctk_orthogonalize_f32")(g.ptr, ld, out.ptr, ld, rows, cols, steps, eps, workspace.ptr if workspace is not None else None, _s(stream))
+    if st:
+        check(st)
     return out
 
 
@@ -259,14 +278,16 @@ def orthogonalize_workspace(shape):
 def muon_update(p, g, m, lr, momentum=0.95, nesterov=True, weight_decay=0.0, scale=None, steps=5, eps=1e-7, workspace=None, stream=None):
     """One orthogonalised step of the weights p [in, out], in place, with its momentum m (updated in place too).
     scale: None for sqrt(max(1, out / in)), which keeps the step's effect on the layer's output alike for every shape."""
-    ld = _pitch(p, "muon_update")
+    rows, cols = _matrix(p, "muon_update")
     if g.shape != p.shape or m.shape != p.shape:
         raise ValueError(f"muon_update: shapes {p.shape}, {g.shape}, {m.shape} of weights, gradient and momentum differ")
-    rows, cols = p.shape
     if scale is None:
         scale = math.sqrt(max(1.0, cols / max(rows, 1)))
-    check(lib.ctk_muon_update_f32(p.p, ld, g.p, ld, m.p, ld, _i64(rows), _i64(cols), _f(lr), _f(momentum), int(bool(nesterov)),
-                                  _f(weight_decay), _f(scale), int(steps), _f(eps), workspace.p if workspace else None, _sh(stream)))
+    ld = cols or 1
+    st = _fn("ctk_muon_update_f32")(p.ptr, ld, g.ptr, ld, m.ptr, ld, rows, cols, lr, momentum, 1 if nesterov else 0, weight_decay, scale, steps, eps,
+                                    workspace.ptr if workspace is not None else None, _s(stream))
+    if st:
+        check(st)
     return p
 
 
@@ -276,15 +297,14 @@ def orthogonalize_status():
     return s.value
 
 
-# ---- 4-bit weights --------------------------------------------------------------------------------------
 class W4Weight:
     """A [k, n] weight in 4 bits: packed [n, kw] uint32, scales [n, groups], zeros [n, groups] uint8 or None."""
     __slots__ = ("packed", "scales", "zeros", "k", "n", "group")
 
     def __init__(self, packed, scales, zeros, k, n, group):
-        groups = -(-k // group) if group in (32, 64, 128) else -1
-        if groups < 0:
+        if group not in (32, 64, 128):
             raise ValueError("W4Weight: group must be 32, 64 or 128")
+        groups = -(-k // group)
         if packed.shape != (n, groups * group // 8) or scales.shape != (n, groups) or (zeros is not None and zeros.shape != (n, groups)):
             raise ValueError("W4Weight: packed, scales and zeros do not fit k, n and group")
         self.packed, self.scales, self.zeros, self.k, self.n, self.group = packed, scales, zeros, k, n, group
@@ -297,44 +317,56 @@ class W4Weight:
         return W4Weight(DeviceArray((n, groups * group // 8), np.uint32), DeviceArray((n, groups)),
                         None if symmetric else DeviceArray((n, groups), np.uint8), k, n, group)
 
-    @property
-    def _zp(self):
-        return self.zeros.p if self.zeros is not None else None
-
 
 def w4_quantize(w, group=128, symmetric=True, out=None, stream=None):
     """The 4-bit form of w [k, n] (see ctorch_b200.h for the rounding)."""
-    ld = _pitch(w, "w4_quantize")
-    out = out or W4Weight.empty(w.shape[0], w.shape[1], group, symmetric)
-    if (out.k, out.n) != w.shape or out.group != group or (out.zeros is None) != bool(symmetric):
+    k, n = _matrix(w, "w4_quantize")
+    if out is None:
+        out = W4Weight.empty(k, n, group, symmetric)
+    elif (out.k, out.n) != (k, n) or out.group != group or (out.zeros is None) != bool(symmetric):
         raise ValueError("w4_quantize: out is not a weight of this shape and form")
-    check(lib.ctk_w4_quantize_f32(w.p, ld, _i64(out.k), _i64(out.n), group, out.packed.p, out.scales.p, out._zp, _sh(stream)))
+    st = _fn("ctk_w4_quantize_f32")(w.ptr, n or 1, k, n, group, out.packed.ptr, out.scales.ptr, None if out.zeros is None else out.zeros.ptr, _s(stream))
+    if st:
+        check(st)
     return out
 
 
 def w4_dequantize(w4, out=None, stream=None):
     """The [k, n] values a 4-bit weight stands for."""
-    out = out or DeviceArray((w4.k, w4.n))
-    if out.shape != (w4.k, w4.n):
+    if out is None:
+        out = DeviceArray((w4.k, w4.n))
+    elif out.shape != (w4.k, w4.n):
         raise ValueError(f"w4_dequantize: out has shape {out.shape}, the weight {(w4.k, w4.n)}")
-    check(lib.ctk_w4_dequantize_f32(w4.packed.p, w4.scales.p, w4._zp, _i64(w4.k), _i64(w4.n), w4.group, out.p, _pitch(out, "w4_dequantize"), _sh(stream)))
+    st = _fn("ctk_w4_dequantize_f32")(w4.packed.ptr, w4.scales.ptr, None if w4.zeros is None else w4.zeros.ptr, w4.k, w4.n, w4.group, out.ptr, w4.n or 1, _s(stream))
+    if st:
+        check(st)
     return out
 
 
 def matmul_w4(x, w4, bias=None, relu=False, out=None, stream=None):
     """[relu](x . W + bias) for x [m, k] (or [k]) and W in 4 bits."""
-    m, k = _rc(x)
-    if k != w4.k or len(x.shape) > 2:
-        raise ValueError(f"matmul_w4: x has shape {x.shape}, the weight {(w4.k, w4.n)}")
-    if bias is not None and bias.size != w4.n:
-        raise ValueError(f"matmul_w4: bias of {bias.size} elements, {w4.n} columns")
-    shape = (w4.n,) if len(x.shape) == 1 else (m, w4.n)
-    out = out or DeviceArray(shape)
-    if out.shape != shape:
+    k, n, shape = w4.k, w4.n, x.shape
+    if not 1 <= len(shape) <= 2 or shape[-1] != k:
+        raise ValueError(f"matmul_w4: x has shape {shape}, the weight {(k, n)}")
+    if bias is not None and bias.size != n:
+        raise ValueError(f"matmul_w4: bias of {bias.size} elements, {n} columns")
+    m = shape[0] if len(shape) == 2 else 1
+    shape = shape[:-1] + (n,)
+    if out is None:
+        out = DeviceArray(shape)
+    elif out.shape != shape:
         raise ValueError(f"matmul_w4: out has shape {out.shape}, expected {shape}")
-    check(lib.ctk_w4_matmul_f32(x.p, _i64(max(k, 1)), w4.packed.p, w4.scales.p, w4._zp, bias.p if bias is not None else None, int(bool(relu)),
-                                out.p, _i64(max(w4.n, 1)), _i64(m), _i64(k), _i64(w4.n), w4.group, _sh(stream)))
+    st = _fn("ctk_w4_matmul_f32")(x.ptr, k or 1, w4.packed.ptr, w4.scales.ptr, None if w4.zeros is None else w4.zeros.ptr, None if bias is None else bias.ptr,
+                                  1 if relu else 0, out.ptr, n or 1, m, k, n, w4.group, _s(stream))
+    if st:
+        check(st)
     return out
+
+
+def w4_status():
+    s = ctypes.c_int()
+    check(lib.ctk_w4_status(ctypes.byref(s)))
+    return s.value
 
 
 CMP = {"gt": 0, "lt": 1, "eq": 2, "ge": 3, "le": 4, "ne": 5}

@@ -451,6 +451,8 @@ ctk_status ctk_w4_dequantize_f32(const uint32_t* packed, const float* scales, co
 ctk_status ctk_w4_matmul_f32(const float* x, int64_t ldx, const uint32_t* packed, const float* scales, const uint8_t* zeros,
                              const float* bias, int relu, float* y, int64_t ldy, int64_t m, int64_t k, int64_t n,
                              int group, void* stream);
+/* Device status word of the product's bounded waits: 0 = none ran out.  Synchronises the device. */
+ctk_status ctk_w4_status(int* status);
 
 /* ------------------------------------------------------------------------------------------- */
 /* Data-parallel gradient exchange (no counterpart in the reference, which is single-process):  */

@@ -102,7 +102,7 @@ def test_quantize_non_finite_poisons_its_group_only(cb, symmetric):
 
 
 SHAPES = [(1, 1, 1), (1, 32, 8), (1, 33, 17), (2, 128, 16), (3, 1001, 517), (1, 784, 128), (1, 128, 10), (4, 300, 65), (5, 4096, 48), (7, 513, 129),
-          (8, 256, 256), (9, 640, 40), (16, 1000, 100), (17, 333, 64), (33, 512, 72), (64, 777, 130), (65, 260, 50), (130, 384, 200), (1, 20000, 9), (2, 5, 3000)]
+          (8, 256, 256), (9, 640, 40), (16, 1000, 100), (17, 333, 64), (33, 512, 72), (64, 777, 130), (65, 260, 50), (130, 384, 200), (1, 20000, 9), (2, 5, 3000), (20, 2000, 300), (24, 1100, 129), (48, 4096, 64)]
 
 
 @pytest.mark.parametrize("symmetric", [True, False])
@@ -121,6 +121,7 @@ def test_matmul_w4(cb, m, k, n, group, symmetric):
     relu = cb.ops.matmul_w4(dx, w4, bias=db, relu=True).numpy()
     assert (np.abs(relu - np.maximum(want + b, 0)) <= bound).all()
     assert np.array_equal(cb.ops.matmul_w4(dx, w4).numpy(), got)           # the same bits again
+    assert cb.ops.w4_status() == 0
 
 
 @pytest.mark.parametrize("factor", [1e-30, 1e-6, 1e6, 1e30])
