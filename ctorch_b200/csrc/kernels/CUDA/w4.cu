@@ -5,46 +5,67 @@
 namespace {
 using namespace ctk;
 
-constexpr int W4_THREADS = 256;
+constexpr int W4_THREADS = 128;  // neighbouring columns: 512 contiguous bytes of a row of w per access (with 32 columns to a CTA quantising
+                                 // 4096 x 4096 took 59 us)
 
 // Bit position of code i of a word: the pairs (2p, 2p+1) sit 16 bits apart, so one mask takes both as the
 // two halves of a register.
 __host__ __device__ constexpr int nibble_shift(int i) { return 4 * (i >> 1) + 16 * (i & 1); }
 
 // ---- quantise ------------------------------------------------------------------------------------------
-// A thread owns one group of one column: lanes are neighbouring columns (coalesced rows of w), the group's
-// GROUP values stay in registers between the maximum and the rounding, so w is read once, with up to GROUP
-// loads in flight per thread.  Bound by w's bytes.
+// A thread owns 32 or 64 k of one column: lanes are neighbouring columns (coalesced rows of w), the values stay in registers
+// between the maximum and the rounding, so w is read once with that many loads in flight; the two halves of a group of 128
+// exchange their extremes through shared memory.  Bound by instruction issue before w's bytes, hence the rounding:
 //
-// round(w / s) exactly: with q = round(w * (1/s)) at most one step off, the remainder d = w - q s is exact in one
-// fma (|d| <= s (1/2 + tiny), a multiple of the smaller of both ulps), so comparing 2|d| with s decides the
-// rounding and its ties without a division.
-__device__ __forceinline__ float round_quotient(float w, float s, float inv) {
-    float q = rintf(w * inv);
+// round(w / s) exactly, ties to even: t = fma(w, 1/s, 1.5 * 2^23 + zero) has the code in its low bits and is at most one step
+// off; the remainder d = w - q s is exact in one fma (|d| <= s (1/2 + tiny), a multiple of the smaller of both ulps), so only
+// where |d| >= s / 2 is there anything to decide, which the word's eight codes ask about together.
+// (With a rounding, a conversion to int and three comparisons per value: 36 instructions and 50 us at 4096 x 4096,
+// this way 20 us.)
+__device__ __forceinline__ uint32_t exact_code(float w, float s, float t, float q) {
     const float d = fmaf(-q, s, w), e = 2.0f * fabsf(d);
-    if (e > s || (e == s && (static_cast<int>(q) & 1))) q += d > 0.0f ? 1.0f : -1.0f;
-    return q;
+    if (e > s || (e == s && ((__float_as_uint(q + 12582912.0f)) & 1u))) t += d > 0.0f ? 1.0f : -1.0f;
+    return __float_as_uint(fminf(fmaxf(t, 12582912.0f), 12582927.0f)) & 15u;
 }
 
 template <int GROUP, bool SYM>
-__global__ void __launch_bounds__(W4_THREADS) w4_quantize_kernel(const float* __restrict__ w, int64_t ldw, int64_t k, int64_t n, int64_t groups,
-                                                                 uint32_t* __restrict__ packed, float* __restrict__ scales, uint8_t* __restrict__ zeros) {
-    const int64_t j = static_cast<int64_t>(blockIdx.x) * 32 + (threadIdx.x & 31);
-    const int64_t grp = static_cast<int64_t>(blockIdx.y) * (W4_THREADS / 32) + (threadIdx.x >> 5);
-    if (j >= n || grp >= groups) return;
-    const int64_t k0 = grp * GROUP;
-    const int len = static_cast<int>(k - k0 < GROUP ? k - k0 : GROUP);
+__global__ void __launch_bounds__(W4_THREADS * (GROUP == 128 ? 2 : 1)) w4_quantize_kernel(const float* __restrict__ w, int64_t ldw, int64_t k, int64_t n, int64_t groups,
+                                                                                           uint32_t* __restrict__ packed, float* __restrict__ scales,
+                                                                                           uint8_t* __restrict__ zeros) {
+    constexpr int LEN = GROUP == 128 ? 64 : GROUP;  // of this thread
+    const uint32_t col_blocks = static_cast<uint32_t>((n + W4_THREADS - 1) / W4_THREADS);
+    const int lane_col = threadIdx.x % W4_THREADS, part = threadIdx.x / W4_THREADS;
+    const int64_t j = static_cast<int64_t>(blockIdx.x % col_blocks) * W4_THREADS + lane_col, grp = blockIdx.x / col_blocks;
+    const bool there = j < n;
+    const int64_t k0 = grp * GROUP + part * LEN;
+    const int len = !there || k0 >= k ? 0 : static_cast<int>(k - k0 < LEN ? k - k0 : LEN);
     const float* src = w + k0 * ldw + j;
-    float v[GROUP];
+    float v[LEN];
+    if (len == LEN) {
 #pragma unroll
-    for (int i = 0; i < GROUP; ++i) v[i] = i < len ? __ldcs(src + i * ldw) : 0.0f;
+        for (int i = 0; i < LEN; ++i) v[i] = __ldcs(src + i * ldw);
+    } else {
+#pragma unroll
+        for (int i = 0; i < LEN; ++i) v[i] = i < len ? __ldcs(src + i * ldw) : 0.0f;
+    }
     float top = 0.0f, bottom = 0.0f, poison = 0.0f;
 #pragma unroll
-    for (int i = 0; i < GROUP; ++i) {
+    for (int i = 0; i < LEN; ++i) {
         top = fmaxf(top, SYM ? fabsf(v[i]) : v[i]);
         if (!SYM) bottom = fminf(bottom, v[i]);
         poison = fmaf(v[i], 0.0f, poison);  // NaN once a value is not finite
     }
+    if constexpr (GROUP == 128) {
+        __shared__ float ends[3][2][W4_THREADS];
+        ends[0][part][lane_col] = top;
+        ends[1][part][lane_col] = bottom;
+        ends[2][part][lane_col] = poison;
+        __syncthreads();
+        top = fmaxf(ends[0][0][lane_col], ends[0][1][lane_col]);
+        bottom = fminf(ends[1][0][lane_col], ends[1][1][lane_col]);
+        poison = ends[2][0][lane_col] + ends[2][1][lane_col];
+    }
+    if (!there) return;
     // the one division of the group, in 64 bits so that the scale is the nearest fp32 number
     const float s = poison == 0.0f ? static_cast<float>(SYM ? static_cast<double>(top) / 7.0 : (static_cast<double>(top) - static_cast<double>(bottom)) / 15.0)
                                    : __int_as_float(0x7fc00000);
@@ -52,31 +73,54 @@ __global__ void __launch_bounds__(W4_THREADS) w4_quantize_kernel(const float* __
     float zero = 8.0f;
     if (!SYM) zero = live ? static_cast<float>(rint(-static_cast<double>(bottom) / static_cast<double>(s))) : 0.0f;
     if (!SYM && zero > 15.0f) zero = 15.0f;  // (subnormal scales only: the range is no longer 15 steps wide)
-    const float inv = 1.0f / s;
-    const bool plain = live && inv <= 3.0e38f;  // else s is subnormal and 1/s overflows: divide in 64 bits
-    uint32_t* dst = packed + j * (groups * (GROUP / 8)) + grp * (GROUP / 8);
-#pragma unroll
-    for (int q4 = 0; q4 < GROUP / 32; ++q4) {
-        uint4 out;
-        uint32_t* o = &out.x;
-#pragma unroll
-        for (int wd = 0; wd < 4; ++wd) {
+    const float inv = live ? 1.0f / s : 0.0f;
+    uint32_t* dst = packed + j * (groups * (GROUP / 8)) + k0 / 8;
+    if (!(inv <= 3.0e38f)) {  // a subnormal scale, 1/s overflows: divide in 64 bits, one by one (rare: no code of it in the loop below)
+#pragma unroll 1
+        for (int wd = 0; wd < LEN / 8; ++wd) {
             uint32_t word = 0;
-#pragma unroll
+#pragma unroll 1
             for (int i = 0; i < 8; ++i) {
-                const float x = v[q4 * 32 + wd * 8 + i];
-                float c = zero;
-                if (plain) c += round_quotient(x, s, inv);
-                else if (live) c += static_cast<float>(rint(static_cast<double>(x) / static_cast<double>(s)));
-                c = fminf(fmaxf(c, SYM ? 1.0f : 0.0f), 15.0f);
+                const float x = wd * 8 + i < len ? __ldg(src + (wd * 8 + i) * ldw) : 0.0f;
+                const float c = fminf(fmaxf(zero + static_cast<float>(rint(static_cast<double>(x) / static_cast<double>(s))), SYM ? 1.0f : 0.0f), 15.0f);
                 word |= static_cast<uint32_t>(c) << nibble_shift(i);
             }
-            o[wd] = word;
+            dst[wd] = word;
         }
-        *reinterpret_cast<uint4*>(dst + q4 * 4) = out;
+    } else {
+        const float base = 12582912.0f + zero, half = live ? 0.5f * s : __int_as_float(0x7f800000), step = live ? s : 0.0f;
+#pragma unroll
+        for (int q4 = 0; q4 < LEN / 32; ++q4) {
+            uint32_t out[4];
+#pragma unroll
+            for (int wd = 0; wd < 4; ++wd) {
+                uint32_t word = 0;
+                bool close = false;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float x = live ? v[q4 * 32 + wd * 8 + i] : 0.0f;
+                    float t = fmaf(x, inv, base);
+                    close |= fabsf(fmaf(base - t, step, x)) >= half;
+                    if (!SYM) t = fminf(t, 12582927.0f);  // (symmetric: 1 .. 15 by construction; the lower end as well)
+                    word |= (__float_as_uint(t) & 15u) << nibble_shift(i);
+                }
+                if (close) {
+                    word = 0;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float x = v[q4 * 32 + wd * 8 + i], t = fmaf(x, inv, base);
+                        word |= exact_code(x, s, t, t - base) << nibble_shift(i);
+                    }
+                }
+                out[wd] = word;
+            }
+            *reinterpret_cast<uint4*>(dst + q4 * 4) = make_uint4(out[0], out[1], out[2], out[3]);
+        }
     }
-    scales[j * groups + grp] = s;
-    if (!SYM) zeros[j * groups + grp] = static_cast<uint8_t>(zero);
+    if (part == 0) {
+        scales[j * groups + grp] = s;
+        if (!SYM) zeros[j * groups + grp] = static_cast<uint8_t>(zero);
+    }
 }
 
 // ---- dequantise ----------------------------------------------------------------------------------------
@@ -84,9 +128,9 @@ __global__ void __launch_bounds__(W4_THREADS) w4_quantize_kernel(const float* __
 __global__ void __launch_bounds__(W4_THREADS) w4_dequantize_kernel(const uint32_t* __restrict__ packed, const float* __restrict__ scales,
                                                                    const uint8_t* __restrict__ zeros, int64_t k, int64_t n, int group, int64_t groups,
                                                                    float* __restrict__ w, int64_t ldw) {
-    const int64_t j = static_cast<int64_t>(blockIdx.x) * 32 + (threadIdx.x & 31);
-    const int64_t k0 = (static_cast<int64_t>(blockIdx.y) * (W4_THREADS / 32) + (threadIdx.x >> 5)) * 32;
-    if (j >= n || k0 >= k) return;
+    const uint32_t col_blocks = static_cast<uint32_t>((n + W4_THREADS - 1) / W4_THREADS);
+    const int64_t j = static_cast<int64_t>(blockIdx.x % col_blocks) * W4_THREADS + threadIdx.x, k0 = static_cast<int64_t>(blockIdx.x / col_blocks) * 32;
+    if (j >= n) return;
     const int64_t grp = k0 / group;
     const uint4 c = __ldg(reinterpret_cast<const uint4*>(packed + j * (groups * (group / 8)) + k0 / 8));
     const float s = scales[j * groups + grp];
@@ -120,7 +164,9 @@ __global__ void __launch_bounds__(W4_THREADS) w4_dequantize_kernel(const uint32_
 // A hand-over between warps (an mbarrier's arrival and wait) takes some 200 clocks, the bytes of 128 columns x 128 k take 180 at
 // HBM's rate: hence the large blocks.  Before this: mma.sync with x cut into three bf16 parts (about 32 clocks an instruction on
 // this machine) 95 us for 4 x 16384 x 16384 and 46 us for 64 x 4096 x 4096; the operand in shared memory, its codes through
-// registers, 96 and 35 us (the load and store unit was the bound); blocks of 128 k, 69 and 37 us; this one LATER and LATER.
+// registers, 96 and 35 us (the load and store unit was the bound); blocks of 128 k, 69 and 37 us; this one 54 and 22 us.  (fp16 in place of e4m3
+// with x in three digits base 2048 reads back three columns per row instead of eight, but a piece of the operand in tensor
+// memory then holds half as many k, and the hand-overs cost more than that gains: 64 and 36 us.)
 constexpr int MM_COLS = 128, MM_PIECE = 128, MM_BLOCK = 256;  // columns of a CTA; k of one piece of x and of a block
 constexpr int MM_RAW_BYTES = MM_COLS * MM_BLOCK / 2;          // codes of a block
 constexpr int MM_A_COLS = MM_BLOCK / 4;                       // tensor memory columns of a block's operand
@@ -619,10 +665,9 @@ ctk_status ctk_w4_quantize_f32(const float* w, int64_t ldw, int64_t k, int64_t n
     CTK_REQUIRE(w && packed && scales, "ctk_w4_quantize_f32: null pointer");
     CTK_REQUIRE((reinterpret_cast<uintptr_t>(packed) & 15u) == 0, "ctk_w4_quantize_f32: packed must be 16-byte aligned");
     CTK_REQUIRE(aligned_to(w, 4) && aligned_to(scales, 4), "ctk_w4_quantize_f32: misaligned pointer");
-    const int64_t groups = (k + group - 1) / group, gy = (groups + W4_THREADS / 32 - 1) / (W4_THREADS / 32);
-    if (gy > 65535) return fail(CTK_ERR_LIMIT, "ctk_w4_quantize_f32: k too large");
-    const dim3 grid(static_cast<unsigned>((n + 31) / 32), static_cast<unsigned>(gy));
-    auto go = [&](auto kernel) { kernel<<<grid, W4_THREADS, 0, as_stream(stream)>>>(w, ldw, k, n, groups, packed, scales, zeros); };
+    const int64_t groups = (k + group - 1) / group, grid = groups * ((n + W4_THREADS - 1) / W4_THREADS);
+    if (grid > 0x7FFFFFFF) return fail(CTK_ERR_LIMIT, "ctk_w4_quantize_f32: too many groups");
+    auto go = [&](auto kernel) { kernel<<<static_cast<unsigned>(grid), W4_THREADS * (group == 128 ? 2 : 1), 0, as_stream(stream)>>>(w, ldw, k, n, groups, packed, scales, zeros); };
     if (zeros) group == 32 ? go(w4_quantize_kernel<32, false>) : group == 64 ? go(w4_quantize_kernel<64, false>) : go(w4_quantize_kernel<128, false>);
     else group == 32 ? go(w4_quantize_kernel<32, true>) : group == 64 ? go(w4_quantize_kernel<64, true>) : go(w4_quantize_kernel<128, true>);
     CTK_LAUNCH_CHECK("w4_quantize");
@@ -640,10 +685,9 @@ ctk_status ctk_w4_dequantize_f32(const uint32_t* packed, const float* scales, co
     CTK_REQUIRE(w && packed && scales, "ctk_w4_dequantize_f32: null pointer");
     CTK_REQUIRE((reinterpret_cast<uintptr_t>(packed) & 15u) == 0, "ctk_w4_dequantize_f32: packed must be 16-byte aligned");
     CTK_REQUIRE(aligned_to(w, 4) && aligned_to(scales, 4), "ctk_w4_dequantize_f32: misaligned pointer");
-    const int64_t groups = (k + group - 1) / group, gy = (k + 32 * (W4_THREADS / 32) - 1) / (32 * (W4_THREADS / 32));
-    if (gy > 65535) return fail(CTK_ERR_LIMIT, "ctk_w4_dequantize_f32: k too large");
-    const dim3 grid(static_cast<unsigned>((n + 31) / 32), static_cast<unsigned>(gy));
-    w4_dequantize_kernel<<<grid, W4_THREADS, 0, as_stream(stream)>>>(packed, scales, zeros, k, n, group, groups, w, ldw);
+    const int64_t groups = (k + group - 1) / group, grid = (k + 31) / 32 * ((n + W4_THREADS - 1) / W4_THREADS);
+    if (grid > 0x7FFFFFFF) return fail(CTK_ERR_LIMIT, "ctk_w4_dequantize_f32: too large");
+    w4_dequantize_kernel<<<static_cast<unsigned>(grid), W4_THREADS, 0, as_stream(stream)>>>(packed, scales, zeros, k, n, group, groups, w, ldw);
     CTK_LAUNCH_CHECK("w4_dequantize");
     return CTK_OK;
 }
