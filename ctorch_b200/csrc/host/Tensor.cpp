@@ -848,6 +848,109 @@ void Tensor::sgd_update_from_(const float* g_device, float lr) {
     cuda_check(ctk_sgd_update_f32(p, g_device, lr, static_cast<int64_t>(numel()), t_stream), "sgd_update_");
 }
 
+// ---- orthogonalised updates and 4-bit weights ----------------------------------------------------------------
+namespace {
+[[noreturn]] void refuse(ErrorType type, const std::string& what) {
+    Ctorch_Error::throwException(ErrorPlatform::kGENERAL, type, what);
+    throw std::logic_error(what);  // (throwException does not return)
+}
+void want_matrix(const Tensor& t, const char* who) {
+    if (t.device() != DeviceType::kCUDA || t.dtype() != DType::kFloat) refuse(ErrorType::DEVICE_COMPAT, std::string(who) + ": float device tensor expected");
+    if (t.sizes().size() != 2) refuse(ErrorType::DIMENSION, std::string(who) + ": 2-D tensor expected");
+    if (!t.is_contiguous()) refuse(ErrorType::DIMENSION, std::string(who) + ": contiguous tensor expected");
+}
+void want_untracked(const Tensor& t, const char* who) {
+    if (AutoDiffContext::current() && t.requires_grad()) refuse(ErrorType::DEVICE_COMPAT, std::string(who) + ": not differentiable; call it outside the tape or on a tensor that does not require grad");
+}
+int64_t extent(const Tensor& t, size_t d) { return static_cast<int64_t>(t.sizes()[d]); }
+}  // namespace
+
+Tensor Tensor::orthogonalize(int steps, float eps) const {
+    want_matrix(*this, "orthogonalize");
+    want_untracked(*this, "orthogonalize");
+    const int64_t rows = extent(*this, 0), cols = extent(*this, 1), ld = cols ? cols : 1;
+    Tensor out(ShapeTag{}, _shape, DType::kFloat, DeviceType::kCUDA, false);
+    // (the workspace comes from the block cache: a captured step keeps it, an eager one gives it back)
+    Tensor ws(ShapeTag{}, {ctk_orthogonalize_workspace_bytes(rows, cols) / sizeof(float) + 1}, DType::kFloat, DeviceType::kCUDA, false);
+    cuda_check(ctk_orthogonalize_f32(data<float>(), ld, out.data<float>(), ld, rows, cols, steps, eps, ws.data<float>(), t_stream), "orthogonalize");
+    return out;
+}
+
+void Tensor::muon_update_(const Tensor& g, Tensor& momentum, const MuonOptions& o) {
+    want_matrix(g, "muon_update_");
+    if (g.sizes() != _shape) refuse(ErrorType::DIMENSION, "muon_update_: gradient has a different shape");
+    muon_update_from_(g.data<float>(), momentum, o);
+}
+
+void Tensor::muon_update_from_(const float* g_device, Tensor& momentum, const MuonOptions& o, bool shared) {
+    want_matrix(*this, "muon_update_");
+    want_matrix(momentum, "muon_update_");
+    if (momentum.sizes() != _shape) refuse(ErrorType::DIMENSION, "muon_update_: momentum has a different shape");
+    const int64_t rows = extent(*this, 0), cols = extent(*this, 1), ld = cols ? cols : 1;
+    const float scale = o.scale >= 0.0f ? o.scale : std::sqrt(std::max(1.0f, static_cast<float>(cols) / static_cast<float>(rows ? rows : 1)));
+    float* m = momentum.data<float>();
+    float* p;
+    if (shared) {
+        p = static_cast<float*>(_storage.raw()) + _storage_offset;  // no detach: the sharers are meant to see it
+        _storage.drop_split();                                      // a split of the old values, if any, is stale now
+    } else {
+        p = data<float>();  // detaches from sharers, drops the split of the old value
+    }
+    Tensor ws(ShapeTag{}, {ctk_orthogonalize_workspace_bytes(rows, cols) / sizeof(float) + 1}, DType::kFloat, DeviceType::kCUDA, false);
+    cuda_check(ctk_muon_update_f32(p, ld, g_device, ld, m, ld, rows, cols, o.lr, o.momentum, o.nesterov ? 1 : 0, o.weight_decay, scale, o.steps, o.eps,
+                                   ws.data<float>(), t_stream),
+               "muon_update_");
+}
+
+W4Weight W4Weight::quantize(const Tensor& w, int group, bool symmetric) {
+    want_matrix(w, "W4Weight::quantize");
+    if (group != 32 && group != 64 && group != 128) refuse(ErrorType::DIMENSION, "W4Weight::quantize: group must be 32, 64 or 128");
+    if (w.numel() == 0) refuse(ErrorType::DIMENSION, "W4Weight::quantize: empty weight");
+    W4Weight q;
+    q.k_ = w.sizes()[0];
+    q.n_ = w.sizes()[1];
+    q.group_ = group;
+    q.symmetric_ = symmetric;
+    const size_t groups = (q.k_ + group - 1) / group;
+    auto make = [](std::vector<size_t> shape, DType t) { return Tensor(ShapeTag{}, shape, t, DeviceType::kCUDA, false); };
+    q.packed_ = make({q.n_, groups * group / 8}, DType::kInt);
+    q.scales_ = make({q.n_, groups}, DType::kFloat);
+    if (!symmetric) q.zeros_ = make({(q.n_ * groups + 3) / 4}, DType::kInt);
+    cuda_check(ctk_w4_quantize_f32(w.data<float>(), static_cast<int64_t>(q.n_), static_cast<int64_t>(q.k_), static_cast<int64_t>(q.n_), group,
+                                   reinterpret_cast<uint32_t*>(q.packed_.data<int32_t>()), q.scales_.data<float>(),
+                                   symmetric ? nullptr : reinterpret_cast<uint8_t*>(q.zeros_.data<int32_t>()), current_stream()),
+               "W4Weight::quantize");
+    return q;
+}
+
+Tensor W4Weight::dequantize() const {
+    if (!n_) refuse(ErrorType::DIMENSION, "W4Weight::dequantize: no weight");
+    Tensor w(ShapeTag{}, {k_, n_}, DType::kFloat, DeviceType::kCUDA, false);
+    cuda_check(ctk_w4_dequantize_f32(packed(), scales(), zeros(), static_cast<int64_t>(k_), static_cast<int64_t>(n_), group_, w.data<float>(),
+                                     static_cast<int64_t>(n_), current_stream()),
+               "W4Weight::dequantize");
+    return w;
+}
+
+Tensor Tensor::linear_w4(const W4Weight& W, const Tensor* bias, bool relu) const {
+    if (_device != DeviceType::kCUDA || _dtype != DType::kFloat) refuse(ErrorType::DEVICE_COMPAT, "linear_w4: float device tensor expected");
+    if (_shape.empty() || _shape.size() > 2 || _shape.back() != W.k() || !W.n()) refuse(ErrorType::DIMENSION, "linear_w4: the input's last extent is not the weight's");
+    if (!is_contiguous()) refuse(ErrorType::DIMENSION, "linear_w4: contiguous tensor expected");
+    want_untracked(*this, "linear_w4");
+    if (bias) {
+        if (bias->device() != DeviceType::kCUDA || bias->dtype() != DType::kFloat) refuse(ErrorType::DEVICE_COMPAT, "linear_w4: float device bias expected");
+        if (bias->numel() != W.n() || !bias->is_contiguous()) refuse(ErrorType::DIMENSION, "linear_w4: one bias per column expected");
+    }
+    std::vector<size_t> shape = _shape;
+    shape.back() = W.n();
+    Tensor y(ShapeTag{}, shape, DType::kFloat, DeviceType::kCUDA, false);
+    const int64_t m = _shape.size() == 2 ? static_cast<int64_t>(_shape[0]) : 1, k = static_cast<int64_t>(W.k()), n = static_cast<int64_t>(W.n());
+    cuda_check(ctk_w4_matmul_f32(data<float>(), k, W.packed(), W.scales(), W.zeros(), bias ? bias->data<float>() : nullptr, relu ? 1 : 0, y.data<float>(), n, m, k,
+                                 n, W.group(), t_stream),
+               "linear_w4");
+    return y;
+}
+
 // ---- free functions (src/Tensor.cpp:1373-1453) ---------------------------------------------------------------
 void backward(Tensor& root) {
     if (AutoDiffContext::current()) AutoDiffContext::current()->backward(root);

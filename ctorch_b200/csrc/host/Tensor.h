@@ -22,6 +22,17 @@
 
 namespace ctorch {
 
+class W4Weight;
+
+// An orthogonalised step (Tensor::muon_update_): momentum, look-ahead, decay, Newton-Schulz steps.
+struct MuonOptions {
+    float lr = 0.02f, momentum = 0.95f, weight_decay = 0.0f;
+    bool nesterov = true;
+    int steps = 5;
+    float eps = 1e-7f;
+    float scale = -1.0f;  // of the step; negative: sqrt(max(1, columns / rows)) of an [in, out] weight
+};
+
 class Tensor {
     static std::atomic<size_t> global_tensor_id;
 
@@ -184,7 +195,41 @@ public:
     // the updated weights.  Opt-in, no counterpart in the reference.
     void sgd_update_shared_(const Tensor& g, float lr);
 
+    // ---- orthogonalised updates and 4-bit weights (no counterpart in the reference) ----
+    // These are not recorded on the tape; a tensor whose gradient the current tape would follow is refused.
+    // This 2-D contiguous float device tensor with singular values near 1 (ctk_orthogonalize_f32).
+    Tensor orthogonalize(int steps = 5, float eps = 1e-7f) const;
+    // One orthogonalised step of this weight matrix, in place, next to sgd_update_: momentum is a tensor of the same shape,
+    // updated in place.  The form with a raw pointer takes a gradient that lives in a communicator's buffer; shared: the
+    // update is seen by every tensor that shares this buffer (as sgd_update_shared_).
+    void muon_update_(const Tensor& g, Tensor& momentum, const MuonOptions& options);
+    void muon_update_from_(const float* g_device, Tensor& momentum, const MuonOptions& options, bool shared = false);
+    // [relu](this . W + bias) with W in 4 bits; this [m, k] or [k].
+    Tensor linear_w4(const W4Weight& W, const Tensor* bias, bool relu) const;
+
     friend class AutoDiff;
+};
+
+// A [k, n] weight in 4 bits with a scale (and optionally a zero point) per group of k: see ctorch_b200.h for the layout and
+// the rounding.
+class W4Weight {
+    Tensor packed_, scales_, zeros_;  // words, fp32, bytes four to a word
+    size_t k_ = 0, n_ = 0;
+    int group_ = 128;
+    bool symmetric_ = true;
+
+public:
+    W4Weight() = default;
+    // w: 2-D float device tensor [k, n]; group 32, 64 or 128.
+    static W4Weight quantize(const Tensor& w, int group = 128, bool symmetric = true);
+    Tensor dequantize() const;
+    size_t k() const { return k_; }
+    size_t n() const { return n_; }
+    int group() const { return group_; }
+    bool symmetric() const { return symmetric_; }
+    const uint32_t* packed() const { return reinterpret_cast<const uint32_t*>(packed_.data<int32_t>()); }
+    const float* scales() const { return scales_.data<float>(); }
+    const uint8_t* zeros() const { return symmetric_ ? nullptr : reinterpret_cast<const uint8_t*>(zeros_.data<int32_t>()); }
 };
 
 void backward(Tensor& root);

@@ -167,6 +167,71 @@ public:
         }
     }
 
+    // Orthogonalised steps for the weight matrices (no counterpart in the reference; off by default).  Biases keep
+    // the SGD step with the trainer's lr, and with hidden_only so do the first and the last layer's weights.
+    struct Muon {
+        bool on = false, hidden_only = false;
+        MuonOptions options;
+        std::vector<Tensor> momentum;  // per layer
+    } muon;
+    void set_muon(bool on, const MuonOptions& o, bool hidden_only) {
+        if (on && dp_mode == DP_SHARDED) throw std::runtime_error("cth_mlp_set_muon: a sharded update owns parts of a matrix, an orthogonalised step needs all of it; use another data-parallel mode");
+        if (on && (!(o.steps >= 1 && o.steps <= 64) || !(o.eps > 0.0f) || !(o.momentum >= 0.0f && o.momentum < 1.0f)))
+            throw std::runtime_error("cth_mlp_set_muon: steps in [1, 64], eps > 0 and momentum in [0, 1) expected");
+        release_graph();  // a recorded step holds the old rule
+        muon.on = on;
+        muon.options = o;
+        muon.hidden_only = hidden_only;
+        if (on && muon.momentum.empty()) {
+            for (Tensor& w : W) {
+                muon.momentum.emplace_back(ShapeTag{}, w.sizes(), DType::kFloat, DeviceType::kCUDA, true);
+                muon.momentum.back().data<float>();
+            }
+            cuda_check(ctk_device_sync(), "set_muon sync");
+        }
+        if (!on) muon.momentum.clear();
+    }
+    bool muon_param(int p) const {
+        if (!muon.on || p % 2) return false;
+        const size_t l = static_cast<size_t>(p / 2);
+        return !muon.hidden_only || (l > 0 && l + 1 < W.size());
+    }
+    // The momentum of every weight matrix, packed in layer order, for a checkpoint.
+    void muon_state(float* out, const float* in) {
+        if (!muon.on) throw std::runtime_error("cth_mlp_*_muon_state: switch orthogonalised steps on first");
+        finish_exchange();
+        cuda_check(ctk_device_sync(), "muon_state sync");
+        for (Tensor& m : muon.momentum) {
+            if (out) { m.copy_to_host(out, m.numel()); out += m.numel(); }
+            else { m.copy_from_host(in, m.numel()); in += m.numel(); }
+        }
+    }
+
+    // The weights in 4 bits, for predict_w4 (no counterpart in the reference): a snapshot, later steps do not change it.
+    std::vector<W4Weight> W4;
+    std::vector<Tensor> b4;
+    void quantize_w4(int group, bool symmetric) {
+        finish_exchange();
+        AutoDiffContext::Guard guard(nullptr);
+        std::vector<W4Weight> q;
+        for (const Tensor& w : W) q.push_back(W4Weight::quantize(w, group, symmetric));
+        // (copies, not shared buffers: a replayed step writes its parameters in place, past any copy-on-write)
+        std::vector<Tensor> bias;
+        for (const Tensor& t : b) {
+            bias.emplace_back(ShapeTag{}, t.sizes(), DType::kFloat, DeviceType::kCUDA, false);
+            cuda_check(ctk_memcpy_d2d(bias.back().data<float>(), t.data<float>(), t.numel() * sizeof(float), current_stream()), "bias copy");
+        }
+        W4 = std::move(q);
+        b4 = std::move(bias);
+    }
+    Tensor predict_w4(const Tensor& x) {
+        if (W4.empty()) throw std::runtime_error("cth_mlp_predict_w4: quantise the weights first (cth_mlp_quantize_w4)");
+        AutoDiffContext::Guard guard(nullptr);
+        Tensor h = x;
+        for (size_t l = 0; l < W4.size(); ++l) h = h.linear_w4(W4[l], &b4[l], l + 1 < W4.size());
+        return h.softmax(static_cast<int>(h.sizes().size()) - 1);
+    }
+
     int64_t n_params() const {
         int64_t n = 0;
         for (size_t l = 0; l + 1 < dims.size(); ++l) n += dims[l] * dims[l + 1] + dims[l + 1];
@@ -191,6 +256,7 @@ public:
     void set_dp_mode(int mode) {
         if (mode < DP_INPLACE || mode > DP_SHARDED) throw std::runtime_error("cth_mlp_set_dp_mode: 0 in place, 1 registered buffer, 2 one all-reduce after backward, 3 sharded update");
         if (comm) throw std::runtime_error("cth_mlp_set_dp_mode: choose the mode before cth_mlp_set_comm");
+        if (mode == DP_SHARDED && muon.on) throw std::runtime_error("cth_mlp_set_dp_mode: the sharded update cannot take orthogonalised steps (cth_mlp_set_muon)");
         dp_mode = mode;
     }
 
@@ -358,7 +424,13 @@ public:
                     cuda_check(ctk_event_record(event_in(ev_ag, p), comm_stream), "record");
                     return;
                 }
-                t.sgd_update_from_(slot, lr);
+                if (muon_param(p)) t.muon_update_from_(slot, muon.momentum[p / 2], muon.options, fresh_weights);
+                else t.sgd_update_from_(slot, lr);
+                return;
+            }
+            if (muon_param(p)) {
+                const Tensor g = grad(t);
+                t.muon_update_from_(g.data<float>(), muon.momentum[p / 2], muon.options, fresh_weights);
                 return;
             }
             if (fresh_weights) t.sgd_update_shared_(grad(t), lr);
@@ -668,8 +740,8 @@ public:
     // calculate_accuracy of mnist/mnist.cpp:134-158: per row the first class whose probability exceeds
     // -1 and every earlier one, compared with (int)label; correct / total in float.  Runs on the
     // device; one float comes back.
-    float accuracy(const Tensor& x, const Tensor& labels) {
-        const Tensor probs = predict(x);
+    float accuracy(const Tensor& x, const Tensor& labels, bool w4 = false) {
+        const Tensor probs = w4 ? predict_w4(x) : predict(x);
         const int64_t rows = static_cast<int64_t>(probs.sizes()[0]), classes = static_cast<int64_t>(probs.sizes()[1]);
         if (static_cast<int64_t>(labels.numel()) != rows) throw std::runtime_error("accuracy: one label per row expected");
         void* st = current_stream();
@@ -1008,7 +1080,62 @@ int cth_sgd_update(void* p, void* g, float lr) {
     return guarded([&] { T(p)->sgd_update_(*T(g), lr); });
 }
 
+// ---- orthogonalised updates and 4-bit weights ----
+int cth_orthogonalize(void* t, int steps, float eps, void** out) {
+    return guarded([&] { *out = new Tensor(T(t)->orthogonalize(steps, eps)); });
+}
+int cth_muon_update(void* p, void* g, void* momentum, float lr, float mu, int nesterov, float weight_decay, float scale, int steps, float eps) {
+    return guarded([&] {
+        MuonOptions o;
+        o.lr = lr; o.momentum = mu; o.nesterov = nesterov != 0; o.weight_decay = weight_decay; o.scale = scale; o.steps = steps; o.eps = eps;
+        T(p)->muon_update_(*T(g), *T(momentum), o);
+    });
+}
+int cth_w4_quantize(void* w, int group, int symmetric, void** out) {
+    return guarded([&] { *out = new W4Weight(W4Weight::quantize(*T(w), group, symmetric != 0)); });
+}
+int cth_w4_free(void* w4) {
+    return guarded([&] { delete static_cast<W4Weight*>(w4); });
+}
+int cth_w4_info(void* w4, int64_t* k, int64_t* n, int* group, int* symmetric) {
+    return guarded([&] {
+        const W4Weight& q = *static_cast<W4Weight*>(w4);
+        if (k) *k = static_cast<int64_t>(q.k());
+        if (n) *n = static_cast<int64_t>(q.n());
+        if (group) *group = q.group();
+        if (symmetric) *symmetric = q.symmetric() ? 1 : 0;
+    });
+}
+int cth_w4_dequantize(void* w4, void** out) {
+    return guarded([&] { *out = new Tensor(static_cast<W4Weight*>(w4)->dequantize()); });
+}
+int cth_linear_w4(void* x, void* w4, void* bias_or_null, int relu, void** out) {
+    return guarded([&] { *out = new Tensor(T(x)->linear_w4(*static_cast<W4Weight*>(w4), bias_or_null ? T(bias_or_null) : nullptr, relu != 0)); });
+}
+
 // ---- MLP trainer ----
+int cth_mlp_set_muon(void* m, int on, float lr, float mu, int nesterov, float weight_decay, float scale, int steps, float eps, int hidden_only) {
+    return guarded([&] {
+        MuonOptions o;
+        o.lr = lr; o.momentum = mu; o.nesterov = nesterov != 0; o.weight_decay = weight_decay; o.scale = scale; o.steps = steps; o.eps = eps;
+        static_cast<MlpTrainer*>(m)->set_muon(on != 0, o, hidden_only != 0);
+    });
+}
+int cth_mlp_get_muon_state(void* m, float* out) {
+    return guarded([&] { static_cast<MlpTrainer*>(m)->muon_state(out, nullptr); });
+}
+int cth_mlp_set_muon_state(void* m, const float* in) {
+    return guarded([&] { static_cast<MlpTrainer*>(m)->muon_state(nullptr, in); });
+}
+int cth_mlp_quantize_w4(void* m, int group, int symmetric) {
+    return guarded([&] { static_cast<MlpTrainer*>(m)->quantize_w4(group, symmetric != 0); });
+}
+int cth_mlp_predict_w4(void* m, void* x, void** probs) {
+    return guarded([&] { *probs = new Tensor(static_cast<MlpTrainer*>(m)->predict_w4(*T(x))); });
+}
+int cth_mlp_accuracy_w4(void* m, void* x, void* labels, float* accuracy) {
+    return guarded([&] { *accuracy = static_cast<MlpTrainer*>(m)->accuracy(*T(x), *T(labels), true); });
+}
 int cth_mlp_create(int n_layers, const int64_t* dims, const float* params, float lr, void** out) {
     return guarded([&] {
         if (n_layers < 1) throw std::runtime_error("cth_mlp_create: need at least one layer");

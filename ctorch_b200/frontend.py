@@ -218,10 +218,55 @@ class Tensor:
     def sgd_update_(self, g, lr):
         _chk(lib.cth_sgd_update(self.h, g.h, ctypes.c_float(lr)))
 
+    def orthogonalize(self, steps=5, eps=1e-7):
+        """This matrix with singular values near 1 (Newton-Schulz steps)."""
+        h = _vp()
+        _chk(lib.cth_orthogonalize(self.h, int(steps), ctypes.c_float(eps), ctypes.byref(h)))
+        return Tensor(h)
+
+    def muon_update_(self, g, momentum, lr, mu=0.95, nesterov=True, weight_decay=0.0, scale=None, steps=5, eps=1e-7):
+        """One orthogonalised step of this weight matrix [in, out]; momentum is updated in place."""
+        f = ctypes.c_float
+        _chk(lib.cth_muon_update(self.h, g.h, momentum.h, f(lr), f(mu), 1 if nesterov else 0, f(weight_decay), f(-1.0 if scale is None else scale), int(steps),
+                                 f(eps)))
+
+    def linear_w4(self, w4, bias=None, relu=False):
+        """[relu](self . W + bias) with W in 4 bits."""
+        h = _vp()
+        _chk(lib.cth_linear_w4(self.h, w4.h, bias.h if bias is not None else None, 1 if relu else 0, ctypes.byref(h)))
+        return Tensor(h)
+
     def __del__(self):
         try:
             if self.h:
                 lib.cth_tensor_free(self.h)
+        except Exception:
+            pass
+
+
+class W4Weight:
+    """A weight matrix in 4 bits: codes, a scale (and, unless symmetric, a zero point) per group of `group` inputs."""
+
+    def __init__(self, w, group=128, symmetric=True):
+        self.h = None
+        h = _vp()
+        _chk(lib.cth_w4_quantize(w.h, int(group), 1 if symmetric else 0, ctypes.byref(h)))
+        self.h = h
+
+    def info(self):
+        k, n, g, s = ctypes.c_int64(), ctypes.c_int64(), ctypes.c_int(), ctypes.c_int()
+        _chk(lib.cth_w4_info(self.h, ctypes.byref(k), ctypes.byref(n), ctypes.byref(g), ctypes.byref(s)))
+        return dict(shape=(k.value, n.value), group=g.value, symmetric=bool(s.value))
+
+    def dequantize(self):
+        h = _vp()
+        _chk(lib.cth_w4_dequantize(self.h, ctypes.byref(h)))
+        return Tensor(h)
+
+    def __del__(self):
+        try:
+            if self.h:
+                lib.cth_w4_free(self.h)
         except Exception:
             pass
 
@@ -354,6 +399,42 @@ class MlpTrainer:
         h = _vp()
         _chk(lib.cth_mlp_predict(self.h, x.h, ctypes.byref(h)))
         return Tensor(h)
+
+    def set_muon(self, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, scale=None, steps=5, eps=1e-7, hidden_only=False, on=True):
+        """Orthogonalised steps for the weight matrices (biases keep SGD; hidden_only: the first and the last layer too)."""
+        f = ctypes.c_float
+        _chk(lib.cth_mlp_set_muon(self.h, 1 if on else 0, f(lr), f(momentum), 1 if nesterov else 0, f(weight_decay), f(-1.0 if scale is None else scale), int(steps),
+                                  f(eps), 1 if hidden_only else 0))
+
+    def _n_weights(self):
+        return sum(i * o for i, o in zip(self.dims[:-1], self.dims[1:]))
+
+    def muon_state(self):
+        """The momenta of the weight matrices, packed in layer order."""
+        out = np.empty(self._n_weights(), np.float32)
+        _chk(lib.cth_mlp_get_muon_state(self.h, out.ctypes.data_as(_vp)))
+        return out
+
+    def load_muon_state(self, state):
+        state = np.require(state, dtype=np.float32, requirements="C")
+        if state.size != self._n_weights():
+            raise ValueError(f"load_muon_state: {state.size} values, {self._n_weights()} weights")
+        _chk(lib.cth_mlp_set_muon_state(self.h, state.ctypes.data_as(_vp)))
+
+    def quantize_w4(self, group=128, symmetric=True):
+        """Takes the current weights in 4 bits, for predict_w4 / accuracy_w4."""
+        _chk(lib.cth_mlp_quantize_w4(self.h, int(group), 1 if symmetric else 0))
+
+    def predict_w4(self, x):
+        """Class probabilities from the 4-bit weights."""
+        h = _vp()
+        _chk(lib.cth_mlp_predict_w4(self.h, x.h, ctypes.byref(h)))
+        return Tensor(h)
+
+    def accuracy_w4(self, x, labels):
+        a = ctypes.c_float()
+        _chk(lib.cth_mlp_accuracy_w4(self.h, x.h, labels.h, ctypes.byref(a)))
+        return a.value
 
     def accuracy(self, x, labels):
         """calculate_accuracy on the device: fraction of rows whose first-maximum class equals the label."""

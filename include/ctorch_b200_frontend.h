@@ -93,6 +93,20 @@ int cth_grad(void* tensor, void** out);                /* free grad(t), src/Tens
 int cth_linear(void* x, void* w, void* bias, int relu, void** out);
 int cth_sgd_update(void* param, void* grad, float lr); /* p -= g*lr on the device (mnist/mnist.cpp:80-92) */
 
+/* ---- orthogonalised updates and 4-bit weights (no counterpart in the reference) ----
+ * Not recorded on the tape: a tensor that requires grad while a context is current is refused. */
+int cth_orthogonalize(void* tensor, int steps, float eps, void** out);   /* ctk_orthogonalize_f32 of a 2-D tensor */
+/* One orthogonalised step of a weight matrix [in, out] in place, next to cth_sgd_update; momentum: a tensor of the same
+ * shape, updated in place.  scale < 0: sqrt(max(1, out / in)). */
+int cth_muon_update(void* param, void* grad, void* momentum, float lr, float mu, int nesterov, float weight_decay,
+                    float scale, int steps, float eps);
+/* A 4-bit weight is a handle of its own.  group: 32, 64 or 128 (ctk_w4_quantize_f32). */
+int cth_w4_quantize(void* tensor, int group, int symmetric, void** w4);
+int cth_w4_free(void* w4);
+int cth_w4_info(void* w4, int64_t* k, int64_t* n, int* group, int* symmetric);
+int cth_w4_dequantize(void* w4, void** tensor);
+int cth_linear_w4(void* x, void* w4, void* bias_or_null, int relu, void** out);   /* [relu](x W + bias), x [m, k] or [k] */
+
 /* ---- the MLP training step of mnist/mnist.cpp:44-92 for any layer list ----
  * dims[0..n_layers]; params packed W1,b1,W2,b2,... (W row-major [in,out]).  A step is
  * make_leaf/requires_grad/zero_grad, forward (matmul + bias, ReLU between layers), one-hot
@@ -171,6 +185,21 @@ int cth_mlp_train_epoch(void* mlp, void* images, void* labels, int64_t batch_siz
 int cth_mnist_load(const char* dir, const char* image_file, const char* label_file, int device, void** images, void** labels);
 /* Rows [start, start+count) as a view of the same buffer (the batch of get_batch, :160-188, without its copy). */
 int cth_tensor_narrow_rows(void* tensor, int64_t start, int64_t count, void** out);
+/* Orthogonalised steps for the trainer's weight matrices instead of SGD (no counterpart in the reference; off by default).
+ * lr is theirs; biases, and with hidden_only the first and the last layer's weights, keep SGD with the trainer's lr.
+ * on == 0 returns to SGD and drops the momentum.  Works in the eager, the graph and the data-parallel step except the sharded
+ * update (mode 3), which is refused; an already recorded graph is released.  get / set_muon_state: the momenta, packed in
+ * layer order (the sizes of the weights), for a checkpoint. */
+int cth_mlp_set_muon(void* mlp, int on, float lr, float mu, int nesterov, float weight_decay, float scale, int steps,
+                     float eps, int hidden_only);
+int cth_mlp_get_muon_state(void* mlp, float* out);
+int cth_mlp_set_muon_state(void* mlp, const float* in);
+/* Quantises the current weights to 4 bits (a snapshot: later steps leave it as it is; quantise again to follow them), for
+ * cth_mlp_predict_w4 and cth_mlp_accuracy_w4, which read it in place of the fp32 weights.  Made for few rows; large batches are
+ * faster through cth_mlp_predict. */
+int cth_mlp_quantize_w4(void* mlp, int group, int symmetric);
+int cth_mlp_predict_w4(void* mlp, void* x, void** probs);
+int cth_mlp_accuracy_w4(void* mlp, void* x, void* labels, float* accuracy);
 int cth_mlp_n_params(void* mlp, int64_t* n);
 int cth_mlp_get_params(void* mlp, float* out);
 int cth_mlp_get_grads(void* mlp, float* out);         /* gradients of the last step (after the all-reduce) */

@@ -120,3 +120,12 @@ def test_python_face_checks_shapes():
         cb.ops.w4_quantize(fake((32, 8)), group=32, symmetric=False, out=w)
     with pytest.raises(ValueError):
         cb.ops.w4_dequantize(w, out=fake((8, 32)))
+
+
+def test_front_end_refuses_host_tensors():
+    from ctorch_b200 import frontend as F
+    F.set_quiet(True)
+    t = F.Tensor.from_numpy(np.ones((4, 8), np.float32), device=F.CPU)
+    for call in (lambda: t.orthogonalize(), lambda: t.muon_update_(t, t.copy(), 0.1), lambda: F.W4Weight(t)):
+        with pytest.raises(F.FrontendError):
+            call()
