@@ -202,6 +202,8 @@ struct Params {
     int m, n;                 // extents of the product's result
     int tiles_m, tiles_n, units, num_kb;
     int split;                // medium matrices: CTAs that share a tile's k-blocks
+    int slabs;                // GRAM of a long, thin matrix: clusters that share a tile, each with its part of k
+    float* slab_sums;         // [slab][tile][row][column] of them, taken up by ns_join_kernel
     Pair src;                 // POLY: A; APPLY: X before the step
     Pair dst;                 // GRAM: A; POLY: B; APPLY: X after the step (unless last)
     const float* coef;        // this step's {b, c, f}
@@ -520,7 +522,7 @@ __device__ __forceinline__ void join8(const uint4& hi, const uint4& lo, float (&
 // because at these sizes straight-line code spends its time on instruction fetches (the persistent kernel's unrolled
 // epilogue took 10 us for its one tile).
 constexpr int MID_THREADS = 576;  // warp 0 loads, warp 1 multiplies, warps 2-17: 4 per quarter of the rows, 32 columns each
-constexpr int MID_MAX_CTAS = 160;
+constexpr int MID_MAX_CTAS = 160, MAX_SLABS = 16;
 constexpr int MID_SMEM = STAGES * STAGE_BYTES + 1024;
 constexpr int MID_PITCH = 129;
 
@@ -540,8 +542,9 @@ __global__ void __launch_bounds__(MID_THREADS, 1) ns_tile_kernel(const __grid_co
     auto tfull_bar = [&](int a) { return bar0 + 8u * (2 * STAGES + a); };
     auto tempty_bar = [&](int a) { return bar0 + 8u * (2 * STAGES + 2 + a); };
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int split = P.split, rank = static_cast<int>(cluster_ctarank()), unit = blockIdx.x / split;
-    const int kb0 = P.num_kb * rank / split, kb1 = P.num_kb * (rank + 1) / split;
+    const int split = P.split, rank = static_cast<int>(cluster_ctarank()), cluster = blockIdx.x / split, slab = cluster / P.units, unit = cluster % P.units;
+    const int share = slab * split + rank, shares = P.slabs * split;
+    const int kb0 = static_cast<int>(static_cast<int64_t>(P.num_kb) * share / shares), kb1 = static_cast<int>(static_cast<int64_t>(P.num_kb) * (share + 1) / shares);
     int tm, tn;
     unit_tile<MODE>(unit, P, tm, tn);
 
@@ -647,7 +650,7 @@ __global__ void __launch_bounds__(MID_THREADS, 1) ns_tile_kernel(const __grid_co
         cluster_sync_all();
         for (int t = tid; t < (cols / 4) * BM; t += MID_THREADS) {
             const int c = t / BM, i = t % BM;
-            const float4* in = partial + (static_cast<int64_t>(unit) * split * 32 + rank * (cols / 4) + c) * BM + i;
+            const float4* in = partial + (static_cast<int64_t>(cluster) * split * 32 + rank * (cols / 4) + c) * BM + i;
             float4 sum = make_float4(0.f, 0.f, 0.f, 0.f), p[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
@@ -671,6 +674,12 @@ __global__ void __launch_bounds__(MID_THREADS, 1) ns_tile_kernel(const __grid_co
     if (warp == 1) {
         fence_after();
         tmem_dealloc<1>(tmem, 256);
+    }
+
+    if (MODE == GRAM && P.slabs > 1) {  // a part of the sum: the join kernel has the epilogue
+        float* to = P.slab_sums + (static_cast<int64_t>(slab) * P.units + unit) * BM * BM + rank * cols;
+        for (int t = tid; t < cols * BM; t += MID_THREADS) to[t / cols * BM + t % cols] = E[t / cols * MID_PITCH + t % cols];
+        return;
     }
 
     // ---- the epilogue, 8 columns of a row at a time ----
@@ -722,6 +731,35 @@ __global__ void __launch_bounds__(MID_THREADS, 1) ns_tile_kernel(const __grid_co
             *reinterpret_cast<uint4*>(d) = hi;
             *reinterpret_cast<uint4*>(d + P.dst.lo) = lo;
         }
+    }
+}
+
+// A = X X^T from the slabs' sums, added in slab order: a thread per 8 columns of a row and, for the mirror place, 8 rows of a
+// column of its tile (the other triangle is read transposed: long, thin matrices have one to a few tiles).
+__global__ void __launch_bounds__(256) ns_join_kernel(const Params P) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int unit = blockIdx.x;
+    int tm, tn;
+    unit_tile<GRAM>(unit, P, tm, tn);
+    const float* in = P.slab_sums + static_cast<int64_t>(unit) * BM * BM;
+    const int64_t next = static_cast<int64_t>(P.units) * BM * BM;
+    const int sides = tm == tn ? 1 : 2;
+    for (int t = blockIdx.y * 256 + threadIdx.x; t < sides * BM * (BM / 8); t += gridDim.y * 256) {
+        const bool mirror = t >= BM * (BM / 8);
+        const int i = (t / (BM / 8)) % BM, c = t % (BM / 8) * 8;  // of the place written to: row, first of 8 columns
+        const int64_t row = (mirror ? tn : tm) * BM + i, col = (mirror ? tm : tn) * BM + c;
+        if (row >= P.m || col >= P.n) continue;
+        float x[8] = {};
+        for (int s = 0; s < P.slabs; ++s)
+#pragma unroll
+            for (int q = 0; q < 8; ++q) x[q] += __ldcg(in + s * next + (mirror ? (c + q) * BM + i : i * BM + c + q));
+#pragma unroll
+        for (int q = 0; q < 8; ++q) x[q] *= 1.0f / 32768.0f;
+        uint4 hi, lo;
+        split8(x, hi, lo);
+        __half* d = P.dst.hi + row * P.dst.pitch + col;
+        *reinterpret_cast<uint4*>(d) = hi;
+        *reinterpret_cast<uint4*>(d + P.dst.lo) = lo;
     }
 }
 
@@ -1131,6 +1169,10 @@ ctk_status launch_tile(const CUtensorMap& a, const CUtensorMap& b, Params P, flo
     // as many CTAs to a tile as the SMs hold at once, each with a k-block at least
     P.split = 1;
     while (P.split < 8 && P.units * P.split * 2 <= MID_MAX_CTAS && P.units * P.split * 2 <= ctk::sm_count() && P.split * 2 <= P.num_kb) P.split *= 2;
+    // a long, thin matrix has few tiles and very many k-blocks: several clusters to a tile (128 x 50000: LATER us a step)
+    P.slabs = 1;
+    if (MODE == GRAM && P.split == 8)
+        while (P.slabs < MAX_SLABS && P.units * 8 * P.slabs * 2 <= MID_MAX_CTAS && P.units * 8 * P.slabs * 2 <= ctk::sm_count() && P.num_kb >= 8 * P.slabs * 8) P.slabs *= 2;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -1139,7 +1181,7 @@ ctk_status launch_tile(const CUtensorMap& a, const CUtensorMap& b, Params P, flo
     attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.gridDim = dim3(static_cast<unsigned>(P.units * P.split));
+    cfg.gridDim = dim3(static_cast<unsigned>(P.units * P.slabs * P.split));
     cfg.blockDim = dim3(MID_THREADS);
     cfg.dynamicSmemBytes = MID_SMEM;
     cfg.stream = st;
@@ -1147,11 +1189,20 @@ ctk_status launch_tile(const CUtensorMap& a, const CUtensorMap& b, Params P, flo
     cfg.numAttrs = 2;
     CTK_CUDA(cudaLaunchKernelEx(&cfg, kernel, a, b, P, partial));
     CTK_LAUNCH_CHECK("ns_tile_kernel");
+    if (P.slabs > 1) {
+        cfg.gridDim = dim3(static_cast<unsigned>(P.units), 8u);
+        cfg.blockDim = dim3(256);
+        cfg.dynamicSmemBytes = 0;
+        cfg.attrs = attr + 1;
+        cfg.numAttrs = 1;
+        CTK_CUDA(cudaLaunchKernelEx(&cfg, ns_join_kernel, P));
+        CTK_LAUNCH_CHECK("ns_join_kernel");
+    }
     return CTK_OK;
 }
 
 struct Layout {
-    size_t partial, coef, x[2], a, b, sums, total;
+    size_t partial, coef, x[2], a, b, sums, slabs, total;
     int64_t pitch_x, pitch_d;
 };
 constexpr int MAX_PARTS = 1024, MAX_STEPS = 64;
@@ -1170,6 +1221,7 @@ Layout layout_for(int64_t rows, int64_t cols) {
     L.a = take(static_cast<size_t>(d) * L.pitch_d * 4);
     L.b = take(static_cast<size_t>(d) * L.pitch_d * 4);
     L.sums = take(d > MID_SIDE ? 0 : static_cast<size_t>(MID_MAX_CTAS) * BM * BM * 4);
+    L.slabs = take(d > MID_SIDE ? 0 : static_cast<size_t>(MID_MAX_CTAS / 8) * BM * BM * 4);  // (slabs x tiles <= MID_MAX_CTAS / 8)
     L.total = at;
     return L;
 }
@@ -1201,6 +1253,7 @@ ctk_status run_steps(const Layout& L, char* ws, int64_t rows, int64_t cols, Sink
         P.m = P.n = static_cast<int>(d);
         P.num_kb = blocks(tall ? rows : cols);
         P.dst = A;
+        P.slab_sums = reinterpret_cast<float*>(ws + L.slabs);
         if (medium) rc = tall ? launch_tile<GRAM, true, true>(mx_mn[at], mx_mn[at], P, sums, st) : launch_tile<GRAM, false, false>(mx_k[at], mx_k[at], P, sums, st);
         else rc = tall ? launch_product<2, GRAM, true, true>(mx_mn[at], mx_mn[at], P, st) : launch_product<2, GRAM, false, false>(mx_k[at], mx_k[at], P, st);
         if (rc) return rc;

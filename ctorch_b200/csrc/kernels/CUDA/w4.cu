@@ -1,5 +1,7 @@
 // 4-bit weights with group scales: quantising, the values they stand for, and y = [relu](x W + bias).
 // The layout is described in ctorch_b200.h.
+#include <algorithm>
+
 #include "tcgen05.cuh"
 
 namespace {
@@ -219,9 +221,10 @@ template <int GROUP, int ROWS>
 __global__ void __launch_bounds__(128) w4_digits_kernel(const float* __restrict__ x, int64_t ldx, int64_t m, int64_t k, int64_t pieces, uint8_t* __restrict__ image) {
     using C = MmCfg<GROUP, ROWS>;
     const int lane = threadIdx.x & 31;
-    const int64_t piece = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-    const int row_block = blockIdx.y / ROWS, r = blockIdx.y % ROWS;
-    const int64_t row = blockIdx.y, k0 = piece * MM_PIECE + lane * 4;
+    const int64_t piece = static_cast<int64_t>(blockIdx.y) * 4 + (threadIdx.x >> 5);
+    const int64_t row = blockIdx.x, row_block = row / ROWS;
+    const int r = static_cast<int>(row - row_block * ROWS);
+    const int64_t k0 = piece * MM_PIECE + lane * 4;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (the main kernel starts with what does not depend on this one)
     if (piece >= pieces) return;
     uint8_t* const out = image + (row_block * pieces + piece) * C::X_BYTES;
@@ -560,14 +563,14 @@ ctk_status launch_matmul(MmArgs P, int split, cudaStream_t st) {
     if (attr_set.first()) CTK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
     const int64_t col_blocks = (P.n + MM_COLS - 1) / MM_COLS, row_blocks = (P.m + ROWS - 1) / ROWS, pieces = (P.groups + C::GPP - 1) / C::GPP;
     P.split = split;
-    if (col_blocks * P.split > 0x7FFFFFFF || row_blocks * ROWS > 65535) return fail(CTK_ERR_LIMIT, "ctk_w4_matmul_f32: too many rows or columns");
+    if (col_blocks * P.split > 0x7FFFFFFF || row_blocks > 65535 || (pieces + 3) / 4 > 65535) return fail(CTK_ERR_LIMIT, "ctk_w4_matmul_f32: k or n too large");
     StreamScratch scratch;
     if (pieces) {
         ctk_status rc = scratch.get(static_cast<size_t>(row_blocks * pieces) * C::X_BYTES, st);
         if (rc) return rc;
         uint8_t* image = static_cast<uint8_t*>(scratch.p);
         P.image = image;
-        w4_digits_kernel<GROUP, ROWS><<<dim3(static_cast<unsigned>((pieces + 3) / 4), static_cast<unsigned>(row_blocks * ROWS)), 128, 0, st>>>(P.x, P.ldx, P.m, P.k, pieces, image);
+        w4_digits_kernel<GROUP, ROWS><<<dim3(static_cast<unsigned>(row_blocks * ROWS), static_cast<unsigned>((pieces + 3) / 4)), 128, 0, st>>>(P.x, P.ldx, P.m, P.k, pieces, image);
         CTK_LAUNCH_CHECK("w4_digits");
     }
     // the codes as a matrix of 32-bit words, 128 columns x 32 words a copy; what lies past its extents reads as zero
@@ -720,7 +723,17 @@ ctk_status ctk_w4_matmul_f32(const float* x, int64_t ldx, const uint32_t* packed
     P.relu = relu;
     P.quads = P.groups % 4 == 0 && aligned_to(scales, 16) && aligned_to(zeros, 4);
     cudaStream_t st = as_stream(stream);
-    return group == 32 ? matmul_rows<32>(P, st) : group == 64 ? matmul_rows<64>(P, st) : matmul_rows<128>(P, st);
+    // x's digits take about 8.2 bytes per element of x: many rows go in slabs of 512 MB of them (a multiple of every kernel's rows)
+    const int64_t per_row = P.groups * group * 9 + 1, slab = std::min<int64_t>(65520, std::max<int64_t>(48, (int64_t(512) << 20) / per_row / 48 * 48));
+    for (int64_t r = 0; r < m; r += slab) {
+        MmArgs Q = P;
+        Q.m = m - r < slab ? m - r : slab;
+        Q.x = x + r * ldx;
+        Q.y = y + r * ldy;
+        const ctk_status rc = group == 32 ? matmul_rows<32>(Q, st) : group == 64 ? matmul_rows<64>(Q, st) : matmul_rows<128>(Q, st);
+        if (rc) return rc;
+    }
+    return CTK_OK;
 }
 
 ctk_status ctk_w4_status(int* status) {

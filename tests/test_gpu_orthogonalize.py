@@ -242,3 +242,13 @@ def test_sizes_around_the_one_launch_limit(cb, shape):
     assert np.linalg.norm(dp.numpy() - (p - 0.5 * o)) <= 0.5 * np.linalg.norm(o) * (ns_tol(5) + 3 * 2.0 ** -24) + 3 * 2.0 ** -24 * np.linalg.norm(p)
     assert (np.abs(dm.numpy() - m64) <= 2.0 ** -23 * (np.abs(0.5 * m) + np.abs(g)) + 1e-38).all()
     assert cb.ops.orthogonalize_status() == 0
+
+
+@pytest.mark.parametrize("shape", [(3, 20000), (128, 9000), (30011, 100), (130, 16000), (16001, 200), (300, 12345)])
+def test_long_thin_matrices(cb, shape):
+    g = grad_like(np.random.default_rng(shape[0]), *shape)
+    d = cb.to_device(g)
+    o = cb.ops.orthogonalize(d).numpy()
+    assert rel(o, ns64(g)) <= ns_tol(5)
+    assert np.array_equal(cb.ops.orthogonalize(d).numpy(), o)
+    assert cb.ops.orthogonalize_status() == 0

@@ -229,3 +229,11 @@ def test_matmul_w4_one_row_of_many_sizes(cb):
     largest = np.abs(x).reshape(2, -1, 128).max(-1).repeat(128, axis=1).astype(np.float64)
     bound = (64 + 8 + 40) * 2.0 ** -23 * (np.abs(x).astype(np.float64) @ np.abs(w)) + 2.0 ** -31 * (largest @ np.abs(w))
     assert (np.abs(cb.ops.matmul_w4(cb.to_device(x), w4).numpy() - x.astype(np.float64) @ w) <= bound).all()
+
+
+def test_matmul_w4_more_rows_than_one_launch_takes(cb):
+    rng = np.random.default_rng(91)
+    w4, w = random_weight(cb, rng, 40, 8, 32, False)
+    x = rng.standard_normal((140001, 40)).astype(np.float32)
+    bound = (32 + 2 + 40) * 2.0 ** -23 * (np.abs(x).astype(np.float64) @ np.abs(w))
+    assert (np.abs(cb.ops.matmul_w4(cb.to_device(x), w4).numpy() - x.astype(np.float64) @ w) <= bound).all()
