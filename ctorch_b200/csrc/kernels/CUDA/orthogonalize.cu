@@ -515,7 +515,7 @@ __device__ __forceinline__ void join8(const uint4& hi, const uint4& lo, float (&
 }
 
 // ---- products of medium matrices -------------------------------------------------------------------------
-// A 128 x 128 tile per cluster of `split` CTAs, each with its share of the k-blocks: with d <= 1024 there are few tiles,
+// A 128 x 128 tile per cluster of `split` CTAs, each with its share of the k-blocks: with d up to 2048 there are few tiles,
 // and a CTA alone takes its operands from L2 at one SM's rate (64 KB a k-block, about 0.9 us).  The CTAs' sums meet in L2
 // (fp32, [column quad][row], so that a warp's store is one run); after a cluster barrier each CTA adds 128 / split
 // columns over all of them, in rank order, and takes these through the epilogue from shared memory -- compact loops,
@@ -772,7 +772,8 @@ __global__ void __launch_bounds__(256) ns_join_kernel(const Params P) {
 //   writes A's hi and lo as shared memory has them -> global | cluster barrier | one bulk copy per array brings A back |
 //   A A, B and B X in each CTA for itself.
 // Everything a product reads is there before it starts, so the small terms go first; an accumulator takes half of K.
-// What bounds it is latency: at 784 x 128 a step is LATER us.  (The exchange through the other CTAs' shared memory
+// What bounds it is latency: at 784 x 128 a step is 12 us, half of it
+// hand-overs between the CTAs.  (The exchange through the other CTAs' shared memory
 // instead of L2 took 18000 of 37000 clocks a step there: 64 KB in and out of every CTA at 7 bytes a clock.)
 constexpr int CL_THREADS = 512;                    // 4 warps per quarter of the accumulator's rows, 32 columns each
 constexpr int CL_SIDE = 128;                       // largest d, widest slab
@@ -1169,7 +1170,7 @@ ctk_status launch_tile(const CUtensorMap& a, const CUtensorMap& b, Params P, flo
     // as many CTAs to a tile as the SMs hold at once, each with a k-block at least
     P.split = 1;
     while (P.split < 8 && P.units * P.split * 2 <= MID_MAX_CTAS && P.units * P.split * 2 <= ctk::sm_count() && P.split * 2 <= P.num_kb) P.split *= 2;
-    // a long, thin matrix has few tiles and very many k-blocks: several clusters to a tile (128 x 50000: LATER us a step)
+    // a long, thin matrix has few tiles and very many k-blocks: several clusters to a tile (128 x 50000: 336 us in all)
     P.slabs = 1;
     if (MODE == GRAM && P.split == 8)
         while (P.slabs < MAX_SLABS && P.units * 8 * P.slabs * 2 <= MID_MAX_CTAS && P.units * 8 * P.slabs * 2 <= ctk::sm_count() && P.num_kb >= 8 * P.slabs * 8) P.slabs *= 2;
@@ -1206,7 +1207,9 @@ struct Layout {
     int64_t pitch_x, pitch_d;
 };
 constexpr int MAX_PARTS = 1024, MAX_STEPS = 64;
-constexpr int64_t MID_SIDE = 1024;  // short sides up to this take the medium kernels
+// Short sides up to this take the medium kernels (with / without: 1100 x 1100 255 / 575 us, 2048 x 2048 597 / 922, 2048 x 4096
+// 1019 / 1248, 2500 x 2500 1454 / 1253).
+constexpr int64_t MID_SIDE = 2048;
 Layout layout_for(int64_t rows, int64_t cols) {
     Layout L;
     const int64_t d = rows < cols ? rows : cols;
