@@ -155,8 +155,8 @@ __global__ void __launch_bounds__(W4_THREADS) w4_dequantize_kernel(const uint32_
 // eight digits joined in fp32, one fma per group with the scale.
 //
 // A first, small kernel writes x's digits (w4_digits_kernel: a warp per row and 128 k) piece by piece as the main kernel's
-// shared memory wants them.  A CTA of the main kernel takes 128 columns of W and, in blocks of 256 k, its share of k (a cluster
-// of `split` CTAs shares the whole):
+// shared memory wants them; where x is small, every CTA makes its own.  A CTA of the main kernel takes 128 columns of W and, in
+// blocks of 256 k, its share of k (a cluster of `split` CTAs shares the whole):
 //   2 warps     loads: the block's codes (one TMA copy, 128 columns x 128 bytes, RAW blocks in flight, the first of them before
 //               x's digits are there) and x's digits, their sums and x's steps (one bulk copy);
 //   4 warps     a thread per column: its 128 bytes of codes, masked, into the operand's place in tensor memory;
@@ -194,6 +194,8 @@ struct MmCfg {
     static constexpr int RC = ROWS <= 8 ? 2 : 4;     // rows joined at a time
     static constexpr int U = GPB < 4 ? GPB : 4;      // groups whose scales are read together
     static constexpr int THREADS = (DRAIN + 4 + 3) * 32;
+    static constexpr int QUAD = GPP >= 4 ? 1 : 4 / GPP;  // pieces of four groups
+    static __host__ __device__ int64_t share_begin(int64_t pieces, int rank, int split) { return rank == split ? pieces : pieces * rank / split / QUAD * QUAD; }
     static_assert(USED_COLS <= 512 && SMEM * PER_SM <= 225 * 1024 && MINE % 2 == 0 && GPB % BATCH == 0 && BATCH <= 4, "");
 };
 
@@ -211,27 +213,22 @@ struct MmArgs {
     int64_t m, k, n, groups;
     int relu, split;
     int quads;             // scales and zero points can be read four at a time
-    const uint8_t* image;  // x's digits, [row block][piece][X_BYTES]
+    const uint8_t* image;  // x's digits, [row block][piece][X_BYTES]; nullptr: each CTA makes its own
 };
 
-// x's digits.  A warp takes one row's 128 k of a piece, lane l the k 4l .. 4l+3.  Rows past m give zeros.
-// The order of a word's codes in the operand's bytes: the masks leave the even nibbles, then the odd ones,
-// nibbles 0 2 4 6 = codes 0 4 1 5 and nibbles 1 3 5 7 = codes 2 6 3 7; x's digits are stored in that order.
+// x's digits.  A warp takes one row's 128 k of a piece, lane l the k 4l .. 4l+3 (load_x; rows past m give zeros), and writes
+// row r of the piece at `out` (global memory, or a stage of the main kernel).
+__device__ __forceinline__ float4 load_x(const float* __restrict__ x, int64_t ldx, int64_t m, int64_t k, int64_t row, int64_t k0) {
+    const float* p = x + row * ldx + k0;
+    const bool here = row < m;
+    return make_float4(here && k0 < k ? __ldg(p) : 0.0f, here && k0 + 1 < k ? __ldg(p + 1) : 0.0f, here && k0 + 2 < k ? __ldg(p + 2) : 0.0f,
+                       here && k0 + 3 < k ? __ldg(p + 3) : 0.0f);
+}
 template <int GROUP, int ROWS>
-__global__ void __launch_bounds__(128) w4_digits_kernel(const float* __restrict__ x, int64_t ldx, int64_t m, int64_t k, int64_t pieces, uint8_t* __restrict__ image) {
+__device__ __forceinline__ void write_digits(float4 x, int r, int lane, uint8_t* out) {
     using C = MmCfg<GROUP, ROWS>;
-    const int lane = threadIdx.x & 31;
-    const int64_t piece = static_cast<int64_t>(blockIdx.y) * 4 + (threadIdx.x >> 5);
-    const int64_t row = blockIdx.x, row_block = row / ROWS;
-    const int r = static_cast<int>(row - row_block * ROWS);
-    const int64_t k0 = piece * MM_PIECE + lane * 4;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (the main kernel starts with what does not depend on this one)
-    if (piece >= pieces) return;
-    uint8_t* const out = image + (row_block * pieces + piece) * C::X_BYTES;
     float* const sums = reinterpret_cast<float*>(out + C::B_BYTES);
-    float v[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = row < m && k0 + e < k ? __ldg(x + row * ldx + k0 + e) : 0.0f;
+    const float v[4] = {x.x, x.y, x.z, x.w};
     // the largest exponent (as bits, so that an infinity or a NaN wins)
     uint32_t top = max(max(__float_as_uint(v[0]) & 0x7FFFFFFFu, __float_as_uint(v[1]) & 0x7FFFFFFFu), max(__float_as_uint(v[2]) & 0x7FFFFFFFu, __float_as_uint(v[3]) & 0x7FFFFFFFu));
     top = __reduce_max_sync(0xffffffffu, top);
@@ -267,6 +264,16 @@ __global__ void __launch_bounds__(128) w4_digits_kernel(const float* __restrict_
     // what one unit of digit 0 stands for, times 2^18
     if (lane == 0) sums[C::GPP * ROWS * 4 + r] = __uint_as_float(bad ? 0x7FC00000u : static_cast<uint32_t>(127 + ex - 156 + 18) << 23);
 }
+template <int GROUP, int ROWS>
+__global__ void __launch_bounds__(128) w4_digits_kernel(const float* __restrict__ x, int64_t ldx, int64_t m, int64_t k, int64_t pieces, uint8_t* __restrict__ image) {
+    const int lane = threadIdx.x & 31;
+    const int64_t piece = static_cast<int64_t>(blockIdx.y) * 4 + (threadIdx.x >> 5);
+    const int64_t row = blockIdx.x, row_block = row / ROWS;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (the main kernel starts with what does not depend on this one)
+    if (piece >= pieces) return;
+    write_digits<GROUP, ROWS>(load_x(x, ldx, m, k, row, piece * MM_PIECE + lane * 4), static_cast<int>(row - row_block * ROWS), lane,
+                              image + (row_block * pieces + piece) * MmCfg<GROUP, ROWS>::X_BYTES);
+}
 
 template <int GROUP, int ROWS>
 __global__ void __launch_bounds__((MmCfg<GROUP, ROWS>::THREADS), (MmCfg<GROUP, ROWS>::PER_SM))
@@ -295,9 +302,7 @@ w4_matmul_kernel(const __grid_constant__ CUtensorMap codes, const MmArgs P) {
     const int rows = static_cast<int>(P.m - row_base < ROWS ? P.m - row_base : ROWS);
     // this CTA's share: pieces of 128 k, groups, blocks
     // (a share starts at a multiple of four groups, so that their scales can be read together)
-    constexpr int QUAD = C::GPP >= 4 ? 1 : 4 / C::GPP;
-    const int64_t all_pieces = (P.groups + C::GPP - 1) / C::GPP, p_begin = all_pieces * rank / split / QUAD * QUAD;
-    const int64_t p_end = rank + 1 == split ? all_pieces : all_pieces * (rank + 1) / split / QUAD * QUAD;
+    const int64_t all_pieces = (P.groups + C::GPP - 1) / C::GPP, p_begin = C::share_begin(all_pieces, rank, split), p_end = C::share_begin(all_pieces, rank + 1, split);
     const int pieces = static_cast<int>(p_end - p_begin), blocks = (pieces + 1) / 2;
     const int groups = static_cast<int>((p_end * C::GPP < P.groups ? p_end * C::GPP : P.groups) - p_begin * C::GPP);
 
@@ -308,12 +313,27 @@ w4_matmul_kernel(const __grid_constant__ CUtensorMap codes, const MmArgs P) {
         for (int s = 0; s < C::STAGES; ++s) { mbar_init(op_full(s), 4); mbar_init(op_empty(s), 1); }
         for (int a = 0; a < 2; ++a) { mbar_init(acc_full(a), 1); mbar_init(acc_empty(a), C::DRAIN); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        if (!P.image) {  // the first codes set off before x's digits are made
+            for (int b = 0; b < blocks && b < C::RAW; ++b) {
+                mbar_expect_tx(raw_full(b), MM_RAW_BYTES);
+                tma_load_2d(base + RAW_AT + b * MM_RAW_BYTES, &codes, raw_full(b), static_cast<int>(p_begin * (MM_PIECE / 8)) + b * (MM_BLOCK / 8), static_cast<int>(col_base));
+            }
+        }
+    }
+    if (!P.image) {  // all of this CTA's x fits its ring: every warp makes a share of the digits, here and once
+        for (int t = warp; t < pieces * ROWS; t += C::THREADS / 32) {
+            const int p = t / ROWS, r = t - p * ROWS;
+            write_digits<GROUP, ROWS>(load_x(P.x, P.ldx, P.m, P.k, row_base + r, (p_begin + p) * MM_PIECE + lane * 4), r, lane, smem + p * C::X_BYTES);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     if (warp == W_MMA) tmem_alloc<1>(smem_u32(&tmem_slot), C::TMEM_COLS);
     fence_before();
     __syncthreads();
     fence_after();
     const uint32_t tmem = tmem_slot, op_tmem = tmem + 2 * C::BATCH * C::N;
+    if (!P.image && tid == 0)
+        for (int b = 0; b < blocks; ++b) mbar_arrive(x_full(b));
 
     float result[C::MINE];
 #pragma unroll
@@ -322,7 +342,7 @@ w4_matmul_kernel(const __grid_constant__ CUtensorMap codes, const MmArgs P) {
     if (warp == W_CODES) {
         // ------------------------------ codes: global -> shared ------------------------------
         if (lane == 0) {
-            for (int b = 0; b < blocks; ++b) {
+            for (int b = P.image ? 0 : C::RAW; b < blocks; ++b) {
                 const int i = b % C::RAW;
                 if (!mbar_wait(raw_empty(i), ((b / C::RAW) & 1) ^ 1u, &abort_flag, &g_w4_status, 0x100 | i)) break;
                 mbar_expect_tx(raw_full(i), MM_RAW_BYTES);
@@ -331,7 +351,7 @@ w4_matmul_kernel(const __grid_constant__ CUtensorMap codes, const MmArgs P) {
         }
     } else if (warp == W_X) {
         // ------------------------------ x: global -> shared ------------------------------
-        if (lane == 0) {
+        if (lane == 0 && P.image) {
             asm volatile("griddepcontrol.wait;" ::: "memory");  // x's digits are there
             const uint8_t* from = P.image + (blockIdx.y * all_pieces + p_begin) * C::X_BYTES;
             for (int b = 0; b < blocks; ++b) {
@@ -564,8 +584,16 @@ ctk_status launch_matmul(MmArgs P, int split, cudaStream_t st) {
     const int64_t col_blocks = (P.n + MM_COLS - 1) / MM_COLS, row_blocks = (P.m + ROWS - 1) / ROWS, pieces = (P.groups + C::GPP - 1) / C::GPP;
     P.split = split;
     if (col_blocks * P.split > 0x7FFFFFFF || row_blocks > 65535 || (pieces + 3) / 4 > 65535) return fail(CTK_ERR_LIMIT, "ctk_w4_matmul_f32: k or n too large");
+    // Where a CTA's share of x is small it makes the digits itself, the same ones in every CTA of the row of column blocks: no
+    // first kernel, no scratch.  3 x 1001 x 517 g32: 8.2 us a call against 10.1, 5.7 against 6.1 in a graph; 8 x 1024 x 4096 g64:
+    // 19 us from the call to its end against 21, but 7.8 against 7.4 in a graph.  With shares of 8 pieces the first kernel wins
+    // there by more (1 x 4096 x 4096 g128: 6.9 us against 7.6).
     StreamScratch scratch;
-    if (pieces) {
+    int64_t share = 0;  // the longest one, in pieces
+    for (int r = 0; r < split; ++r) share = std::max(share, C::share_begin(pieces, r + 1, split) - C::share_begin(pieces, r, split));
+    const bool alone = share <= 4 && share * ROWS <= 16;
+    static_assert(2 * C::XS >= 4, "a share fits the ring");
+    if (pieces && !alone) {
         ctk_status rc = scratch.get(static_cast<size_t>(row_blocks * pieces) * C::X_BYTES, st);
         if (rc) return rc;
         uint8_t* image = static_cast<uint8_t*>(scratch.p);
@@ -599,7 +627,7 @@ ctk_status launch_matmul(MmArgs P, int split, cudaStream_t st) {
     cfg.dynamicSmemBytes = C::SMEM;
     cfg.stream = st;
     cfg.attrs = attr;
-    cfg.numAttrs = pieces ? 2 : 1;  // (without k there is nothing in front of it to wait for in the kernel)
+    cfg.numAttrs = P.image ? 2 : 1;  // (without the first kernel there is nothing to wait for in the kernel)
     CTK_CUDA(cudaLaunchKernelEx(&cfg, kernel, codes, P));
     CTK_LAUNCH_CHECK("w4_matmul");
     return CTK_OK;
