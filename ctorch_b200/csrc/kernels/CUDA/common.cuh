@@ -35,12 +35,17 @@ struct StreamScratch {
 };
 
 inline bool aligned_to(const void* p, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
-// Whether two [rows, cols] fp32 arrays of row pitch lda / ldb share a byte between their first and last element.
+// Whether two [rows, cols] fp32 arrays of row pitch lda / ldb overlap: share a byte between their first and last element, unless
+// both are columns of one buffer (the same pitch) that lie side by side.
 inline bool spans_overlap(const void* a, int64_t rows_a, int64_t cols_a, int64_t lda, const void* b, int64_t rows_b, int64_t cols_b, int64_t ldb) {
     if (rows_a <= 0 || cols_a <= 0 || rows_b <= 0 || cols_b <= 0) return false;
     const uintptr_t a0 = reinterpret_cast<uintptr_t>(a), b0 = reinterpret_cast<uintptr_t>(b);
     const uintptr_t a1 = a0 + 4 * static_cast<uintptr_t>((rows_a - 1) * lda + cols_a), b1 = b0 + 4 * static_cast<uintptr_t>((rows_b - 1) * ldb + cols_b);
-    return a0 < b1 && b0 < a1;
+    if (a0 >= b1 || b0 >= a1) return false;
+    if (lda != ldb || (a0 - b0) % 4) return true;
+    // side by side in the rows of one buffer
+    const int64_t shift = static_cast<int64_t>(b0 > a0 ? (b0 - a0) / 4 : (a0 - b0) / 4) % lda, first = b0 > a0 ? cols_a : cols_b, second = b0 > a0 ? cols_b : cols_a;
+    return shift < first || shift + second > lda;
 }
 
 inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s); }
@@ -66,6 +71,21 @@ struct PerDeviceOnce {
         if (done[dev]) return false;
         done[dev] = true;
         return true;
+    }
+};
+
+// The same where threads may make their first calls at once: every thread that finds the set-up missing does it (it is
+// idempotent) before it launches, and only a set-up that succeeded is marked.
+struct PerDeviceReady {
+    std::atomic<bool> done[64];
+    template <typename F>
+    ctk_status ensure(F&& set_up) {
+        int dev = 0;
+        const bool known = cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64;
+        if (known && done[dev].load(std::memory_order_acquire)) return CTK_OK;
+        const ctk_status st = set_up();
+        if (!st && known) done[dev].store(true, std::memory_order_release);
+        return st;
     }
 };
 

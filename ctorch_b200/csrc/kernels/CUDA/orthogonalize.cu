@@ -193,8 +193,9 @@ constexpr int STAGES = 3;
 // k-blocks of 64 terms summed in TMEM before they move to registers.  Relative error of NS(G) against 64 bits at 784 x 128
 // with 1 / 2 / 4 / 8 blocks: 1.8 / 3.1 / 3.4 / 4.0e-6, at 4096 x 4096 0.7 / 0.9 / 1.6 / 3.0e-6 (fp32 library products: 1.4 and
 // 3.8e-6).  A drain of the 128 x 256 accumulator costs the tensor pipe about 0.6 us (4096 x 4096 APPLY: 350 / 335 / 315 us
-// with 2 / 4 / 8 blocks, 293 without drains), so large products take 4 and small ones, which are not bound by the pipe, 1.
-__host__ __device__ constexpr int chunk_kb(int group) { return group == 2 ? 4 : 1; }
+// with 2 / 4 / 8 blocks, 293 without drains), so the pairs' product takes 4 and the kernels of smaller matrices, which are not
+// bound by the pipe, 1.
+constexpr int CHUNK_KB = 4;
 constexpr int OUT_PITCH = 33;
 constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_WARPS * 32 * OUT_PITCH * 4 + 1024;
 
@@ -321,21 +322,20 @@ __device__ __forceinline__ void emit_block(const Params& P, bool mirror, int row
     }
 }
 
-// D = A B^T over k, persistent.  GROUP 2: a pair of CTAs per 256 x 256 tile, each with 128 rows of A and 128 columns
-// of B; GROUP 1: a CTA per 128 x 128 tile.  A stage is one box of hi and lo per operand (K-major), or two, one per 64
-// columns (MN-major).  Two accumulators: the next chunk is multiplied while the epilogue warps add the last one.
-template <int GROUP, int MODE, bool A_MN, bool B_MN>
+// D = A B^T over k, persistent.  A pair of CTAs per 256 x 256 tile, each with 128 rows of A and 128 columns of B.
+// A stage is one box of hi and lo per operand (K-major), or two, one per 64 columns (MN-major).  Two accumulators: the next
+// chunk is multiplied while the epilogue warps add the last one.
+template <int MODE, bool A_MN, bool B_MN>
 __global__ void __launch_bounds__(THREADS, 1) ns_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Params P) {
     using namespace t5;
-    constexpr int BN = 128 * GROUP;
-    constexpr int CHUNK_KB = chunk_kb(GROUP);
+    constexpr int BN = 256;
     constexpr int TMEM_COLS = 2 * BN;
     constexpr int BLOCKS = BN / 64;  // 32-column blocks per epilogue warp: two warps share a row quarter
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t bars[2 * STAGES + 4];
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int abort_flag;
-    const uint32_t rank = GROUP == 2 ? cluster_ctarank() : 0;
+    const uint32_t rank = cluster_ctarank();
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint32_t* out_stage = reinterpret_cast<uint32_t*>(smem_raw + (smem_base - smem_u32(smem_raw)) + STAGES * STAGE_BYTES);
     const uint32_t bar0 = smem_u32(bars);
@@ -343,24 +343,24 @@ __global__ void __launch_bounds__(THREADS, 1) ns_product_kernel(const __grid_con
     auto empty_bar = [&](int s) { return bar0 + 8u * (STAGES + s); };
     auto tfull_bar = [&](int a) { return bar0 + 8u * (2 * STAGES + a); };
     auto tempty_bar = [&](int a) { return bar0 + 8u * (2 * STAGES + 2 + a); };
-    const uint32_t peer_abort = GROUP == 2 ? map_to_cta(smem_u32(const_cast<int*>(&abort_flag)), rank ^ 1u) : 0u;
+    const uint32_t peer_abort = map_to_cta(smem_u32(const_cast<int*>(&abort_flag)), rank ^ 1u);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
         abort_flag = 0;
         for (int s = 0; s < STAGES; ++s) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
-        for (int a = 0; a < 2; ++a) { mbar_init(tfull_bar(a), 1); mbar_init(tempty_bar(a), EPI_WARPS * GROUP); }
+        for (int a = 0; a < 2; ++a) { mbar_init(tfull_bar(a), 1); mbar_init(tempty_bar(a), EPI_WARPS * 2); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         prefetch_tmap(&map_a);
         prefetch_tmap(&map_b);
     }
-    if (warp == 1) tmem_alloc<GROUP>(smem_u32(&tmem_slot), TMEM_COLS);
+    if (warp == 1) tmem_alloc<2>(smem_u32(&tmem_slot), TMEM_COLS);
     fence_before();
     __syncthreads();
-    if (GROUP == 2) cluster_sync_all();  // the peer's barriers exist before anything is signalled across
+    cluster_sync_all();  // the peer's barriers exist before anything is signalled across
     fence_after();
     const uint32_t tmem_base = tmem_slot;
-    const int first_unit = blockIdx.x / GROUP, unit_step = gridDim.x / GROUP;
+    const int first_unit = blockIdx.x / 2, unit_step = gridDim.x / 2;
 
     if (warp == 0) {
         if (lane == 0) {
@@ -370,24 +370,24 @@ __global__ void __launch_bounds__(THREADS, 1) ns_product_kernel(const __grid_con
             for (int u = first_unit; u < P.units && ok; u += unit_step) {
                 int tm, tn;
                 unit_tile<MODE>(u, P, tm, tn);
-                const int m0 = (tm * GROUP + static_cast<int>(rank)) * BM, n0 = tn * BN + static_cast<int>(rank) * BM;
+                const int m0 = (tm * 2 + static_cast<int>(rank)) * BM, n0 = tn * BN + static_cast<int>(rank) * BM;
                 for (int kb = 0; kb < P.num_kb; ++kb) {
                     if (!mbar_wait(empty_bar(stage), phase ^ 1u, &abort_flag, &g_ns_status, 0x100 | stage)) { ok = false; break; }
-                    if (rank == 0) mbar_expect_tx(full_bar(stage), GROUP * STAGE_BYTES);
-                    const uint32_t fb = GROUP == 2 ? map_to_cta(full_bar(stage), 0) : full_bar(stage);
+                    if (rank == 0) mbar_expect_tx(full_bar(stage), 2 * STAGE_BYTES);
+                    const uint32_t fb = map_to_cta(full_bar(stage), 0);
                     const uint32_t base = smem_base + stage * STAGE_BYTES;
                     const int k0 = kb * BK;
                     if (A_MN) {
-                        tma_load_3d<GROUP>(base, &map_a, fb, m0, k0, 0);
-                        tma_load_3d<GROUP>(base + STAGE_BYTES / 4, &map_a, fb, m0 + 64, k0, 0);
+                        tma_load_3d<2>(base, &map_a, fb, m0, k0, 0);
+                        tma_load_3d<2>(base + STAGE_BYTES / 4, &map_a, fb, m0 + 64, k0, 0);
                     } else {
-                        tma_load_3d<GROUP>(base, &map_a, fb, k0, m0, 0);
+                        tma_load_3d<2>(base, &map_a, fb, k0, m0, 0);
                     }
                     if (B_MN) {
-                        tma_load_3d<GROUP>(base + STAGE_BYTES / 2, &map_b, fb, n0, k0, 0);
-                        tma_load_3d<GROUP>(base + 3 * (STAGE_BYTES / 4), &map_b, fb, n0 + 64, k0, 0);
+                        tma_load_3d<2>(base + STAGE_BYTES / 2, &map_b, fb, n0, k0, 0);
+                        tma_load_3d<2>(base + 3 * (STAGE_BYTES / 4), &map_b, fb, n0 + 64, k0, 0);
                     } else {
-                        tma_load_3d<GROUP>(base + STAGE_BYTES / 2, &map_b, fb, k0, n0, 0);
+                        tma_load_3d<2>(base + STAGE_BYTES / 2, &map_b, fb, k0, n0, 0);
                     }
                     ++issued;
                     if (++stage == STAGES) { stage = 0; phase ^= 1u; }
@@ -402,13 +402,13 @@ __global__ void __launch_bounds__(THREADS, 1) ns_product_kernel(const __grid_con
                 if (++stage == STAGES) { stage = 0; phase ^= 1u; }
             }
             if (!ok) {
-                if (GROUP == 2) st_cluster_u32(peer_abort, 1u);
+                st_cluster_u32(peer_abort, 1u);
                 for (int i = 0; i < 2048; ++i) __nanosleep(1000);
             }
         }
     } else if (warp == 1) {
         if (rank == 0) {
-            constexpr uint32_t idesc = make_idesc(BM * GROUP, BN, A_MN, B_MN);
+            constexpr uint32_t idesc = make_idesc(BM * 2, BN, A_MN, B_MN);
             // hi and lo of a K-major tile lie half an operand apart; of an MN-major one a quarter, inside each column group
             // (descriptors hold addresses in units of 16 bytes: every step is an addition of a constant)
             constexpr uint64_t a_lo = (A_MN ? STAGE_BYTES / 8 : STAGE_BYTES / 4) >> 4, b_lo = (B_MN ? STAGE_BYTES / 8 : STAGE_BYTES / 4) >> 4;
@@ -430,24 +430,24 @@ __global__ void __launch_bounds__(THREADS, 1) ns_product_kernel(const __grid_con
                         if (elect_one()) {
 #pragma unroll
                             for (int ks = 0; ks < BK / 16; ++ks) {  // the small terms first, while the accumulator is small
-                                mma_f16<GROUP>(d, a + a_lo + ks * a_step, b + ks * b_step, idesc, kb > c0 || ks > 0);
-                                mma_f16<GROUP>(d, a + ks * a_step, b + b_lo + ks * b_step, idesc, 1u);
+                                mma_f16<2>(d, a + a_lo + ks * a_step, b + ks * b_step, idesc, kb > c0 || ks > 0);
+                                mma_f16<2>(d, a + ks * a_step, b + b_lo + ks * b_step, idesc, 1u);
                             }
 #pragma unroll
-                            for (int ks = 0; ks < BK / 16; ++ks) mma_f16<GROUP>(d, a + ks * a_step, b + ks * b_step, idesc, 1u);
-                            commit<GROUP>(empty_bar(stage));
-                            if (kb + 1 == c1) commit<GROUP>(tfull_bar(acc));
+                            for (int ks = 0; ks < BK / 16; ++ks) mma_f16<2>(d, a + ks * a_step, b + ks * b_step, idesc, 1u);
+                            commit<2>(empty_bar(stage));
+                            if (kb + 1 == c1) commit<2>(tfull_bar(acc));
                         }
                         if (++stage == STAGES) { stage = 0; phase ^= 1u; }
                     }
                     if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
                 }
             }
-            if (!ok && GROUP == 2 && lane == 0) st_cluster_u32(peer_abort, 1u);
+            if (!ok && lane == 0) st_cluster_u32(peer_abort, 1u);
         }
     } else {
         const int quarter = warp & 3, side = (warp - 2) >> 2;  // rows 32 quarter.., columns BN/2 side..
-        const uint32_t te0 = GROUP == 2 ? map_to_cta(tempty_bar(0), 0) : tempty_bar(0), te1 = GROUP == 2 ? map_to_cta(tempty_bar(1), 0) : tempty_bar(1);
+        const uint32_t te0 = map_to_cta(tempty_bar(0), 0), te1 = map_to_cta(tempty_bar(1), 0);
         const float cf[3] = {__ldg(P.coef), __ldg(P.coef + 1), __ldg(P.coef + 2)};
         uint32_t* stage = out_stage + (warp - 2) * 32 * OUT_PITCH;
         int acc = 0;
@@ -481,20 +481,20 @@ __global__ void __launch_bounds__(THREADS, 1) ns_product_kernel(const __grid_con
                 if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
             }
             if (!ok) break;
-            const int row_base = (tm * GROUP + static_cast<int>(rank)) * BM + quarter * 32;
+            const int row_base = (tm * 2 + static_cast<int>(rank)) * BM + quarter * 32;
 #pragma unroll
             for (int b = 0; b < BLOCKS; ++b)
                 emit_block<MODE>(P, MODE != APPLY && tm != tn, row_base, lane, tn * BN + side * (BN / 2) + b * 32, sum[b], stage, cf);
         }
-        if (!ok && GROUP == 2 && lane == 0) st_cluster_u32(peer_abort, 1u);
+        if (!ok && lane == 0) st_cluster_u32(peer_abort, 1u);
     }
 
     fence_before();
     __syncthreads();
-    if (GROUP == 2) cluster_sync_all();  // neither CTA leaves (or frees TMEM) while the other may still signal it
+    cluster_sync_all();  // neither CTA leaves (or frees TMEM) while the other may still signal it
     if (warp == 1) {
         fence_after();
-        tmem_dealloc<GROUP>(tmem_base, TMEM_COLS);
+        tmem_dealloc<2>(tmem_base, TMEM_COLS);
     }
 }
 
@@ -1122,17 +1122,17 @@ ctk_status make_map(CUtensorMap* map, const Pair& p, int64_t inner, int64_t oute
     return CTK_OK;
 }
 
-template <int GROUP, int MODE, bool A_MN, bool B_MN>
+template <int MODE, bool A_MN, bool B_MN>
 ctk_status launch_product(const CUtensorMap& a, const CUtensorMap& b, Params P, cudaStream_t st) {
-    auto kernel = ns_product_kernel<GROUP, MODE, A_MN, B_MN>;
-    static int resident[64] = {0};  // tiles in flight on a device
+    auto kernel = ns_product_kernel<MODE, A_MN, B_MN>;
+    static std::atomic<int> resident[64];  // tiles in flight on a device
     int dev = 0;
     CTK_CUDA(cudaGetDevice(&dev));
     CTK_REQUIRE(dev >= 0 && dev < 64, "device ordinal out of range");
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = GROUP;
+    attr[0].val.clusterDim.x = 2;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     cfg.blockDim = dim3(THREADS);
@@ -1140,19 +1140,19 @@ ctk_status launch_product(const CUtensorMap& a, const CUtensorMap& b, Params P, 
     cfg.stream = st;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (!resident[dev]) {
+    int at_once = resident[dev];
+    if (!at_once) {
         CTK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES));
-        cfg.gridDim = dim3(static_cast<unsigned>(GROUP * ctk::sm_count()));
-        int n = 0;
-        CTK_CUDA(cudaOccupancyMaxActiveClusters(&n, kernel, &cfg));
-        CTK_REQUIRE(n > 0, "the device cannot hold the orthogonalisation kernel");
-        resident[dev] = n;
+        cfg.gridDim = dim3(static_cast<unsigned>(2 * ctk::sm_count()));
+        CTK_CUDA(cudaOccupancyMaxActiveClusters(&at_once, kernel, &cfg));
+        CTK_REQUIRE(at_once > 0, "the device cannot hold the orthogonalisation kernel");
+        resident[dev] = at_once;
     }
-    constexpr int T = BM * GROUP;
+    constexpr int T = BM * 2;
     P.tiles_m = (P.m + T - 1) / T;
     P.tiles_n = (P.n + T - 1) / T;
     P.units = MODE == APPLY ? P.tiles_m * P.tiles_n : P.tiles_n * (P.tiles_n + 1) / 2;
-    cfg.gridDim = dim3(static_cast<unsigned>(GROUP * (P.units < resident[dev] ? P.units : resident[dev])));
+    cfg.gridDim = dim3(static_cast<unsigned>(2 * (P.units < at_once ? P.units : at_once)));
     CTK_CUDA(cudaLaunchKernelEx(&cfg, kernel, a, b, P));
     CTK_LAUNCH_CHECK("ns_product_kernel");
     return CTK_OK;
@@ -1162,8 +1162,12 @@ ctk_status launch_product(const CUtensorMap& a, const CUtensorMap& b, Params P, 
 template <int MODE, bool A_MN, bool B_MN>
 ctk_status launch_tile(const CUtensorMap& a, const CUtensorMap& b, Params P, float4* partial, cudaStream_t st) {
     auto kernel = ns_tile_kernel<MODE, A_MN, B_MN>;
-    static ctk::PerDeviceOnce attr_set;
-    if (attr_set.first()) CTK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MID_SMEM));
+    static ctk::PerDeviceReady ready;
+    const ctk_status rc = ready.ensure([&]() -> ctk_status {
+        CTK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MID_SMEM));
+        return CTK_OK;
+    });
+    if (rc) return rc;
     P.tiles_m = (P.m + BM - 1) / BM;
     P.tiles_n = (P.n + BM - 1) / BM;
     P.units = MODE == APPLY ? P.tiles_m * P.tiles_n : P.tiles_n * (P.tiles_n + 1) / 2;
@@ -1258,12 +1262,12 @@ ctk_status run_steps(const Layout& L, char* ws, int64_t rows, int64_t cols, Sink
         P.dst = A;
         P.slab_sums = reinterpret_cast<float*>(ws + L.slabs);
         if (medium) rc = tall ? launch_tile<GRAM, true, true>(mx_mn[at], mx_mn[at], P, sums, st) : launch_tile<GRAM, false, false>(mx_k[at], mx_k[at], P, sums, st);
-        else rc = tall ? launch_product<2, GRAM, true, true>(mx_mn[at], mx_mn[at], P, st) : launch_product<2, GRAM, false, false>(mx_k[at], mx_k[at], P, st);
+        else rc = tall ? launch_product<GRAM, true, true>(mx_mn[at], mx_mn[at], P, st) : launch_product<GRAM, false, false>(mx_k[at], mx_k[at], P, st);
         if (rc) return rc;
         P.num_kb = blocks(d);
         P.src = A;
         P.dst = B;
-        rc = medium ? launch_tile<POLY, false, false>(ma, ma, P, sums, st) : launch_product<2, POLY, false, false>(ma, ma, P, st);
+        rc = medium ? launch_tile<POLY, false, false>(ma, ma, P, sums, st) : launch_product<POLY, false, false>(ma, ma, P, st);
         if (rc) return rc;
         P.m = static_cast<int>(rows);
         P.n = static_cast<int>(cols);
@@ -1271,7 +1275,7 @@ ctk_status run_steps(const Layout& L, char* ws, int64_t rows, int64_t cols, Sink
         P.dst = X[at ^ 1];
         P.last = s + 1 == steps;
         if (medium) rc = tall ? launch_tile<APPLY, false, false>(mx_k[at], mb, P, sums, st) : launch_tile<APPLY, false, true>(mb, mx_mn[at], P, sums, st);
-        else rc = tall ? launch_product<2, APPLY, false, false>(mx_k[at], mb, P, st) : launch_product<2, APPLY, false, true>(mb, mx_mn[at], P, st);
+        else rc = tall ? launch_product<APPLY, false, false>(mx_k[at], mb, P, st) : launch_product<APPLY, false, true>(mb, mx_mn[at], P, st);
     }
     return rc;
 }
@@ -1279,11 +1283,13 @@ ctk_status run_steps(const Layout& L, char* ws, int64_t rows, int64_t cols, Sink
 template <int V, bool MOMENTUM>
 ctk_status launch_cluster(const ClusterArgs& P, int ctas, cudaStream_t st) {
     auto kernel = ns_cluster_kernel<V, MOMENTUM>;
-    static ctk::PerDeviceOnce attr_set;
-    if (attr_set.first()) {
+    static ctk::PerDeviceReady ready;
+    const ctk_status rc = ready.ensure([&]() -> ctk_status {
         CTK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, CL_SMEM));
         CTK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    }
+        return CTK_OK;
+    });
+    if (rc) return rc;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;

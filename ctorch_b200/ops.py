@@ -250,10 +250,27 @@ def _s(stream):
     return None if stream is None else _sh(stream)
 
 
+_F32 = np.dtype(np.float32)
+_workspaces = {}
+
+
 def _matrix(a, what):
     if len(a.shape) != 2:
         raise ValueError(f"{what}: a 2-D array expected, got shape {a.shape}")
+    if a.dtype != _F32:
+        raise ValueError(f"{what}: a float32 array expected, got {a.dtype}")
     return a.shape
+
+
+def _workspace(a, shape, what):
+    if a is None:
+        return None
+    need = _workspaces.get(shape)
+    if need is None:
+        need = _workspaces[shape] = int(lib.ctk_orthogonalize_workspace_bytes(_i64(shape[0]), _i64(shape[1])))
+    if a.nbytes < need:
+        raise ValueError(f"{what}: a workspace of {a.nbytes} bytes, {need} needed")
+    return a.ptr
 
 
 def orthogonalize(g, steps=5, eps=1e-7, out=None, workspace=None, stream=None):
@@ -261,10 +278,10 @@ def orthogonalize(g, steps=5, eps=1e-7, out=None, workspace=None, stream=None):
     rows, cols = _matrix(g, "orthogonalize")
     if out is None:
         out = DeviceArray(g.shape)
-    elif out.shape != g.shape:
-        raise ValueError(f"orthogonalize: out has shape {out.shape}, g {g.shape}")
+    elif out.shape != g.shape or out.dtype != _F32:
+        raise ValueError(f"orthogonalize: out has shape {out.shape} and type {out.dtype}, g {g.shape}")
     ld = cols or 1
-    st = _fn("ctk_orthogonalize_f32")(g.ptr, ld, out.ptr, ld, rows, cols, steps, eps, workspace.ptr if workspace is not None else None, _s(stream))
+    st = _fn("ctk_orthogonalize_f32")(g.ptr, ld, out.ptr, ld, rows, cols, steps, eps, _workspace(workspace, g.shape, "orthogonalize"), _s(stream))
     if st:
         check(st)
     return out
@@ -281,11 +298,13 @@ def muon_update(p, g, m, lr, momentum=0.95, nesterov=True, weight_decay=0.0, sca
     rows, cols = _matrix(p, "muon_update")
     if g.shape != p.shape or m.shape != p.shape:
         raise ValueError(f"muon_update: shapes {p.shape}, {g.shape}, {m.shape} of weights, gradient and momentum differ")
+    if g.dtype != _F32 or m.dtype != _F32:
+        raise ValueError(f"muon_update: float32 arrays expected, got {g.dtype} and {m.dtype}")
     if scale is None:
         scale = math.sqrt(max(1.0, cols / max(rows, 1)))
     ld = cols or 1
     st = _fn("ctk_muon_update_f32")(p.ptr, ld, g.ptr, ld, m.ptr, ld, rows, cols, lr, momentum, 1 if nesterov else 0, weight_decay, scale, steps, eps,
-                                    workspace.ptr if workspace is not None else None, _s(stream))
+                                    _workspace(workspace, p.shape, "muon_update"), _s(stream))
     if st:
         check(st)
     return p
@@ -307,6 +326,8 @@ class W4Weight:
         groups = -(-k // group)
         if packed.shape != (n, groups * group // 8) or scales.shape != (n, groups) or (zeros is not None and zeros.shape != (n, groups)):
             raise ValueError("W4Weight: packed, scales and zeros do not fit k, n and group")
+        if packed.dtype not in (np.uint32, np.int32) or scales.dtype != _F32 or (zeros is not None and zeros.dtype != np.uint8):
+            raise ValueError("W4Weight: packed is uint32, scales float32, zeros uint8")
         self.packed, self.scales, self.zeros, self.k, self.n, self.group = packed, scales, zeros, k, n, group
 
     @staticmethod
@@ -335,8 +356,8 @@ def w4_dequantize(w4, out=None, stream=None):
     """The [k, n] values a 4-bit weight stands for."""
     if out is None:
         out = DeviceArray((w4.k, w4.n))
-    elif out.shape != (w4.k, w4.n):
-        raise ValueError(f"w4_dequantize: out has shape {out.shape}, the weight {(w4.k, w4.n)}")
+    elif out.shape != (w4.k, w4.n) or out.dtype != _F32:
+        raise ValueError(f"w4_dequantize: out has shape {out.shape} and type {out.dtype}, the weight {(w4.k, w4.n)}")
     st = _fn("ctk_w4_dequantize_f32")(w4.packed.ptr, w4.scales.ptr, None if w4.zeros is None else w4.zeros.ptr, w4.k, w4.n, w4.group, out.ptr, w4.n or 1, _s(stream))
     if st:
         check(st)
@@ -348,14 +369,16 @@ def matmul_w4(x, w4, bias=None, relu=False, out=None, stream=None):
     k, n, shape = w4.k, w4.n, x.shape
     if not 1 <= len(shape) <= 2 or shape[-1] != k:
         raise ValueError(f"matmul_w4: x has shape {shape}, the weight {(k, n)}")
-    if bias is not None and bias.size != n:
-        raise ValueError(f"matmul_w4: bias of {bias.size} elements, {n} columns")
+    if x.dtype != _F32:
+        raise ValueError(f"matmul_w4: float32 x expected, got {x.dtype}")
+    if bias is not None and (bias.size != n or bias.dtype != _F32):
+        raise ValueError(f"matmul_w4: bias of {bias.size} elements ({bias.dtype}), {n} columns")
     m = shape[0] if len(shape) == 2 else 1
     shape = shape[:-1] + (n,)
     if out is None:
         out = DeviceArray(shape)
-    elif out.shape != shape:
-        raise ValueError(f"matmul_w4: out has shape {out.shape}, expected {shape}")
+    elif out.shape != shape or out.dtype != _F32:
+        raise ValueError(f"matmul_w4: out has shape {out.shape} and type {out.dtype}, expected {shape}")
     st = _fn("ctk_w4_matmul_f32")(x.ptr, k or 1, w4.packed.ptr, w4.scales.ptr, None if w4.zeros is None else w4.zeros.ptr, None if bias is None else bias.ptr,
                                   1 if relu else 0, out.ptr, n or 1, m, k, n, w4.group, _s(stream))
     if st:

@@ -446,8 +446,10 @@ ctk_status ctk_w4_dequantize_f32(const uint32_t* packed, const float* scales, co
                                  int group, float* w, int64_t ldw, void* stream);
 /* y = [relu](x W + bias): x [m, k] with row pitch ldx, y [m, n] with row pitch ldy, bias n floats or NULL.
  * Made for few rows (the weight's bytes are the bound up to about 8 rows); any m is taken.  fp32-level accuracy:
- * codes are exact in the products, x enters with its 24 bits, sums are fp32 per group and across groups, in
- * an order that depends on the sizes only.  x must not overlap y. */
+ * x enters rounded to within 2^-38 of the largest |x| among the 128 consecutive k (from a multiple of 128) of its
+ * row that hold it, the sums within a group are exact, and the groups' sums are joined in fp32 in an order that
+ * depends on the sizes only.  A row of x that holds an infinity or a NaN gives NaN.  x must not overlap y.
+ * x's digits, about 8.2 bytes per element, come from the device's pool in the stream's order where x is not small. */
 ctk_status ctk_w4_matmul_f32(const float* x, int64_t ldx, const uint32_t* packed, const float* scales, const uint8_t* zeros,
                              const float* bias, int relu, float* y, int64_t ldy, int64_t m, int64_t k, int64_t n,
                              int group, void* stream);

@@ -252,3 +252,52 @@ def test_long_thin_matrices(cb, shape):
     assert rel(o, ns64(g)) <= ns_tol(5)
     assert np.array_equal(cb.ops.orthogonalize(d).numpy(), o)
     assert cb.ops.orthogonalize_status() == 0
+
+
+@pytest.mark.parametrize("shape", [(70, 90), (300, 210)])
+def test_orthogonalize_columns_of_one_buffer(cb, shape):
+    """g and out side by side in the rows of one buffer, in both orders."""
+    rows, cols = shape
+    rng = np.random.default_rng(rows)
+    ld = 2 * cols + 3
+    g = grad_like(rng, rows, cols)
+    want = cb.ops.orthogonalize(cb.to_device(g)).numpy()
+    for at_g, at_out in ((0, cols + 3), (cols, 0)):
+        host = rng.standard_normal((rows, ld)).astype(np.float32)
+        host[:, at_g:at_g + cols] = g
+        buf = cb.to_device(host)
+        cb.check(cb.lib.ctk_orthogonalize_f32(buf.view(at_g, (1,)).p, i64(ld), buf.view(at_out, (1,)).p, i64(ld), i64(rows), i64(cols), 5, f32(1e-7), None, None))
+        got = buf.numpy()
+        # (which loads are taken four at a time depends on the alignment, not what they add up to)
+        assert rel(got[:, at_out:at_out + cols], want) <= ns_tol(5)
+        host[:, at_out:at_out + cols] = got[:, at_out:at_out + cols]
+        assert np.array_equal(got, host)
+
+
+def test_orthogonalize_from_several_threads(cb):
+    """Calls from four threads at once, each on a stream of its own, give what they give alone."""
+    import threading
+    rng = np.random.default_rng(77)
+    shapes = [(64, 300), (400, 250), (129, 40), (300, 2000)]
+    gs = [cb.to_device(grad_like(rng, *s)) for s in shapes]
+    outs = [cb.empty(s) for s in shapes]
+    errors = []
+    cb.synchronize()
+
+    def work(i):
+        try:
+            st = cb.Stream()
+            for _ in range(5):
+                cb.ops.orthogonalize(gs[i], out=outs[i], stream=st)
+            st.sync()
+        except Exception as e:
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(shapes))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    for g, o in zip(gs, outs):
+        assert np.array_equal(o.numpy(), cb.ops.orthogonalize(g).numpy())

@@ -221,7 +221,7 @@ def test_matmul_w4_whole_numbers_are_exact(cb, m, group):
 
 
 def test_matmul_w4_one_row_of_many_sizes(cb):
-    """A row with elements of very different sizes: each block of 128 k is taken to 31 bits below its largest."""
+    """A row with elements of very different sizes: each block of 128 k is taken to 38 bits below its largest."""
     rng = np.random.default_rng(55)
     k, n = 512, 70
     w4, w = random_weight(cb, rng, k, n, 64, False)
@@ -237,3 +237,47 @@ def test_matmul_w4_more_rows_than_one_launch_takes(cb):
     x = rng.standard_normal((140001, 40)).astype(np.float32)
     bound = (32 + 2 + 40) * 2.0 ** -23 * (np.abs(x).astype(np.float64) @ np.abs(w))
     assert (np.abs(cb.ops.matmul_w4(cb.to_device(x), w4).numpy() - x.astype(np.float64) @ w) <= bound).all()
+
+
+@pytest.mark.parametrize("m", [1, 3, 12])
+def test_matmul_w4_outliers_where_the_weight_is_zero(cb, m):
+    """Single elements of x a million times the others: columns whose weight is zero there keep what the others give.  x enters
+    within 2^-38 of the largest of its 128 neighbours, which adds that much per unit of weight to the tolerance."""
+    rng = np.random.default_rng(40 + m)
+    k, n, group = 640, 300, 64
+    packed = pack(rng.integers(0, 16, (n, k)))
+    codes = unpack(packed).reshape(n, k)
+    codes[:, 5::128] = 8                                                # zero of the symmetric form
+    packed = pack(codes)
+    scales = rng.uniform(0.5, 1.5, (n, k // group)).astype(np.float32)
+    w = values64(packed, scales, None, k, group)
+    x = rng.standard_normal((m, k)).astype(np.float32)
+    x[:, 5::128] *= 1e6
+    w4 = cb.ops.W4Weight(cb.to_device(packed, np.uint32), cb.to_device(scales), None, k, n, group)
+    y = cb.ops.matmul_w4(cb.to_device(x), w4).numpy()
+    top = np.abs(x).reshape(m, -1, 128).max(axis=2).repeat(128, axis=1).astype(np.float64)
+    bound = (group + k // group + 40) * 2.0 ** -23 * (np.abs(x).astype(np.float64) @ np.abs(w)) + 2.0 ** -38 * (top @ np.abs(w))
+    assert (np.abs(y - x.astype(np.float64) @ w) <= bound).all()
+
+
+def test_matmul_w4_input_and_result_in_one_buffer(cb):
+    """x and y as columns of one buffer, side by side in its rows."""
+    rng = np.random.default_rng(8)
+    m, k, n, ld = 5, 96, 40, 140
+    w4, w = random_weight(cb, rng, k, n, 32, True)
+    host = rng.standard_normal((m, ld)).astype(np.float32)
+    want = cb.ops.matmul_w4(cb.to_device(host[:, :k]), w4).numpy()
+    for at_x, at_y in ((0, k), (n + 4, 0)):
+        buf = cb.to_device(host)
+        if at_x:
+            host2 = host.copy()
+            host2[:, at_x:at_x + k] = host[:, :k]
+            buf = cb.to_device(host2)
+        before = buf.numpy()
+        cb.check(cb.lib.ctk_w4_matmul_f32(buf.view(at_x, (1,)).p, i64(ld), w4.packed.p, w4.scales.p, None, None, 0, buf.view(at_y, (1,)).p, i64(ld), i64(m), i64(k),
+                                          i64(n), 32, None))
+        after = buf.numpy()
+        assert np.array_equal(after[:, at_y:at_y + n], want)
+        keep = np.ones(ld, bool)
+        keep[at_y:at_y + n] = False
+        assert np.array_equal(after[:, keep], before[:, keep])

@@ -129,3 +129,35 @@ def test_front_end_refuses_host_tensors():
     for call in (lambda: t.orthogonalize(), lambda: t.muon_update_(t, t.copy(), 0.1), lambda: F.W4Weight(t)):
         with pytest.raises(F.FrontendError):
             call()
+
+
+def test_columns_of_one_buffer_must_not_cross(L):
+    # 8 columns from column 0, 8 more from column 7 or (round the row's end) from column 13 of rows of 20
+    assert ortho(L, ldg=20, ldo=20, out=P((1 << 20) + 4 * 7)) == INVALID
+    assert ortho(L, ldg=20, ldo=20, out=P((1 << 20) + 4 * 13)) == INVALID
+    assert ortho(L, ldg=20, ldo=21, out=P((1 << 20) + 4 * 10)) == INVALID  # different pitches: not side by side throughout
+    assert product(L, ldx=80, ldy=80, y=P((1 << 20) + 4 * 60)) == INVALID
+    assert product(L, ldx=80, ldy=80, y=P((1 << 20) + 4 * 75)) == INVALID
+
+
+def test_python_face_checks_types_and_workspace():
+    import ctorch_b200 as cb
+
+    def fake(shape, dtype=np.float32):
+        return cb.DeviceArray(shape, dtype, _ptr=1 << 20)
+
+    g, d = fake((300, 200)), fake((300, 200), np.float64)
+    small = fake((1024,), np.uint8)
+    for call in (lambda: cb.ops.orthogonalize(d), lambda: cb.ops.orthogonalize(g, out=d), lambda: cb.ops.muon_update(g, d, g, lr=0.1),
+                 lambda: cb.ops.muon_update(g, g, d, lr=0.1), lambda: cb.ops.orthogonalize(g, out=g, workspace=small),
+                 lambda: cb.ops.muon_update(g, g, g, lr=0.1, workspace=small), lambda: cb.ops.w4_quantize(d, group=32),
+                 lambda: cb.ops.W4Weight(fake((8, 4)), fake((8, 1)), None, 32, 8, 32),
+                 lambda: cb.ops.W4Weight(fake((8, 4), np.uint32), fake((8, 1), np.float64), None, 32, 8, 32),
+                 lambda: cb.ops.W4Weight(fake((8, 4), np.uint32), fake((8, 1)), fake((8, 1)), 32, 8, 32)):
+        with pytest.raises(ValueError):
+            call()
+    w = cb.ops.W4Weight(fake((8, 4), np.uint32), fake((8, 1)), None, 32, 8, 32)
+    for call in (lambda: cb.ops.matmul_w4(fake((2, 32), np.float64), w), lambda: cb.ops.matmul_w4(fake((2, 32)), w, bias=fake((8,), np.float64)),
+                 lambda: cb.ops.matmul_w4(fake((2, 32)), w, out=fake((2, 8), np.float64)), lambda: cb.ops.w4_dequantize(w, out=fake((32, 8), np.float64))):
+        with pytest.raises(ValueError):
+            call()
