@@ -243,68 +243,72 @@ __device__ __forceinline__ void emit_block(const Params& P, bool mirror, int row
     if (col0 >= P.n || row_base >= P.m) return;  // the whole warp
     const int sub = lane >> 3, c4 = (lane & 7) * 4;
     const int64_t col = col0 + c4;
-    uint2 h4[8], l4[8];
-    if (MODE != GRAM) {  // all of the block's reads in flight before anything waits
-        const __half* xp = P.src.hi + (row_base + sub) * P.src.pitch + col;  // (pitches are multiples of 8: four elements never leave the row)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            h4[i] = l4[i] = make_uint2(0u, 0u);
-            if (row_base + i * 4 + sub < P.m && col < P.n) {
-                h4[i] = __ldcg(reinterpret_cast<const uint2*>(xp + i * 4 * P.src.pitch));
-                l4[i] = __ldcg(reinterpret_cast<const uint2*>(xp + i * 4 * P.src.pitch + P.src.lo));
-            }
-        }
-    }
 #pragma unroll
     for (int i = 0; i < 32; ++i) stage[lane * OUT_PITCH + i] = __float_as_uint(v[i]);
     __syncwarp();
+    constexpr int HALF = 4;  // rows of a lane at a time (2500 x 2500 with 8: 1130 us, 4: 1097, 2: the same)
+#pragma unroll 1
+    for (int r0 = 0; r0 < 32; r0 += 4 * HALF) {
+        uint2 h4[HALF], l4[HALF];
+        if (MODE != GRAM) {  // all of these reads in flight before anything waits
+            const __half* xp = P.src.hi + (row_base + r0 + sub) * P.src.pitch + col;  // (pitches are multiples of 8: four elements never leave the row)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int r = i * 4 + sub;
-        uint32_t* s = stage + r * OUT_PITCH + c4;
-        const __half2 h0 = *reinterpret_cast<const __half2*>(&h4[i].x), h1 = *reinterpret_cast<const __half2*>(&h4[i].y);
-        const __half2 l0 = *reinterpret_cast<const __half2*>(&l4[i].x), l1 = *reinterpret_cast<const __half2*>(&l4[i].y);
-        const float src[4] = {__low2float(h0) + __low2float(l0), __high2float(h0) + __high2float(l0), __low2float(h1) + __low2float(l1),
-                              __high2float(h1) + __high2float(l1)};
-        float o[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float d = __uint_as_float(s[e]);
-            if (MODE == GRAM) o[e] = d * (1.0f / 32768.0f);
-            if (MODE == POLY) o[e] = fmaf(cf[0] * 0.5f, src[e], cf[1] * (1.0f / 65536.0f) * d);
-            if (MODE == APPLY) o[e] = cf[2] * fmaf(kA, src[e], d * (1.0f / 16384.0f));
-        }
-        const bool inside = row_base + r < P.m && col < P.n;
-        if (MODE == APPLY && P.last) {
-            if (!inside) continue;
-            float* out = P.sink.out + (row_base + r) * P.sink.ldo + col;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] *= 1.0f / kScaleX;
-            if (P.sink.vec && col + 4 <= P.n) {
-                float4 old = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (P.sink.update) old = *reinterpret_cast<const float4*>(out);
-                *reinterpret_cast<float4*>(out) = make_float4(sink_value(P.sink, o[0], old.x), sink_value(P.sink, o[1], old.y), sink_value(P.sink, o[2], old.z),
-                                                              sink_value(P.sink, o[3], old.w));
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (col + e < P.n) out[e] = sink_value(P.sink, o[e], P.sink.update ? out[e] : 0.0f);
+            for (int i = 0; i < HALF; ++i) {
+                h4[i] = l4[i] = make_uint2(0u, 0u);
+                if (row_base + r0 + i * 4 + sub < P.m && col < P.n) {
+                    h4[i] = __ldcg(reinterpret_cast<const uint2*>(xp + i * 4 * P.src.pitch));
+                    l4[i] = __ldcg(reinterpret_cast<const uint2*>(xp + i * 4 * P.src.pitch + P.src.lo));
+                }
             }
-            continue;
         }
-        uint2 hi, lo;
-        split2(o[0], o[1], hi.x, lo.x);
-        split2(o[2], o[3], hi.y, lo.y);
-        if (inside) {
-            __half* d = P.dst.hi + (row_base + r) * P.dst.pitch + col;
-            *reinterpret_cast<uint2*>(d) = hi;
-            *reinterpret_cast<uint2*>(d + P.dst.lo) = lo;
-        }
-        if (MODE != APPLY && mirror) {  // {hi, lo} of one element in one word
-            s[0] = __byte_perm(hi.x, lo.x, 0x5410);
-            s[1] = __byte_perm(hi.x, lo.x, 0x7632);
-            s[2] = __byte_perm(hi.y, lo.y, 0x5410);
-            s[3] = __byte_perm(hi.y, lo.y, 0x7632);
+#pragma unroll
+        for (int i = 0; i < HALF; ++i) {
+            const int r = r0 + i * 4 + sub;
+            uint32_t* s = stage + r * OUT_PITCH + c4;
+            const __half2 h0 = *reinterpret_cast<const __half2*>(&h4[i].x), h1 = *reinterpret_cast<const __half2*>(&h4[i].y);
+            const __half2 l0 = *reinterpret_cast<const __half2*>(&l4[i].x), l1 = *reinterpret_cast<const __half2*>(&l4[i].y);
+            const float src[4] = {__low2float(h0) + __low2float(l0), __high2float(h0) + __high2float(l0), __low2float(h1) + __low2float(l1),
+                                  __high2float(h1) + __high2float(l1)};
+            float o[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float d = __uint_as_float(s[e]);
+                if (MODE == GRAM) o[e] = d * (1.0f / 32768.0f);
+                if (MODE == POLY) o[e] = fmaf(cf[0] * 0.5f, src[e], cf[1] * (1.0f / 65536.0f) * d);
+                if (MODE == APPLY) o[e] = cf[2] * fmaf(kA, src[e], d * (1.0f / 16384.0f));
+            }
+            const bool inside = row_base + r < P.m && col < P.n;
+            if (MODE == APPLY && P.last) {
+                if (!inside) continue;
+                float* out = P.sink.out + (row_base + r) * P.sink.ldo + col;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] *= 1.0f / kScaleX;
+                if (P.sink.vec && col + 4 <= P.n) {
+                    float4 old = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (P.sink.update) old = *reinterpret_cast<const float4*>(out);
+                    *reinterpret_cast<float4*>(out) = make_float4(sink_value(P.sink, o[0], old.x), sink_value(P.sink, o[1], old.y), sink_value(P.sink, o[2], old.z),
+                                                                  sink_value(P.sink, o[3], old.w));
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (col + e < P.n) out[e] = sink_value(P.sink, o[e], P.sink.update ? out[e] : 0.0f);
+                }
+                continue;
+            }
+            uint2 hi, lo;
+            split2(o[0], o[1], hi.x, lo.x);
+            split2(o[2], o[3], hi.y, lo.y);
+            if (inside) {
+                __half* d = P.dst.hi + (row_base + r) * P.dst.pitch + col;
+                *reinterpret_cast<uint2*>(d) = hi;
+                *reinterpret_cast<uint2*>(d + P.dst.lo) = lo;
+            }
+            if (MODE != APPLY && mirror) {  // {hi, lo} of one element in one word
+                s[0] = __byte_perm(hi.x, lo.x, 0x5410);
+                s[1] = __byte_perm(hi.x, lo.x, 0x7632);
+                s[2] = __byte_perm(hi.y, lo.y, 0x5410);
+                s[3] = __byte_perm(hi.y, lo.y, 0x7632);
+            }
         }
     }
     __syncwarp();
@@ -360,6 +364,8 @@ __global__ void __launch_bounds__(THREADS, 1) ns_product_kernel(const __grid_con
     cluster_sync_all();  // the peer's barriers exist before anything is signalled across
     fence_after();
     const uint32_t tmem_base = tmem_slot;
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // what the kernel before wrote is there
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int first_unit = blockIdx.x / 2, unit_step = gridDim.x / 2;
 
     if (warp == 0) {
@@ -467,24 +473,34 @@ __global__ void __launch_bounds__(THREADS, 1) ns_product_kernel(const __grid_con
                 const uint32_t t = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * BN + side * (BN / 2));
 #pragma unroll
                 for (int b = 0; b < BLOCKS; ++b) {
-                    uint32_t r[32];
-                    tmem_ld32(t + b * 32, r);
-                    tmem_ld_wait();
-                    if (b == BLOCKS - 1) {  // read completely: the next but one chunk may go there
-                        fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive_cluster(acc ? te1 : te0);
-                    }
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) sum[b][i] += __uint_as_float(r[i]);
+                    for (int h = 0; h < 2; ++h) {  // 16 columns at a time: with 32 the sums spill (2500 x 2500: 1087 us, this way 1069)
+                        uint32_t r[16];
+                        tmem_ld_cols(t + b * 32 + h * 16, r);
+                        tmem_ld_wait();
+                        if (b == BLOCKS - 1 && h == 1) {  // read completely: the next but one chunk may go there
+                            fence_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive_cluster(acc ? te1 : te0);
+                        }
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) sum[b][h * 16 + i] += __uint_as_float(r[i]);
+                    }
                 }
                 if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
             }
             if (!ok) break;
             const int row_base = (tm * 2 + static_cast<int>(rank)) * BM + quarter * 32;
+            // one copy of the code, the blocks moved through its registers: unrolled four times, instruction fetch was most of an
+            // epilogue's time (2500 x 2500: 1247 us unrolled, 1137 this way)
+#pragma unroll 1
+            for (int b = 0; b < BLOCKS; ++b) {
+                emit_block<MODE>(P, MODE != APPLY && tm != tn, row_base, lane, tn * BN + side * (BN / 2) + b * 32, sum[0], stage, cf);
 #pragma unroll
-            for (int b = 0; b < BLOCKS; ++b)
-                emit_block<MODE>(P, MODE != APPLY && tm != tn, row_base, lane, tn * BN + side * (BN / 2) + b * 32, sum[b], stage, cf);
+                for (int c = 0; c + 1 < BLOCKS; ++c)
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) sum[c][i] = sum[c + 1][i];
+            }
         }
         if (!ok && lane == 0) st_cluster_u32(peer_abort, 1u);
     }
@@ -1130,11 +1146,13 @@ ctk_status launch_product(const CUtensorMap& a, const CUtensorMap& b, Params P, 
     CTK_CUDA(cudaGetDevice(&dev));
     CTK_REQUIRE(dev >= 0 && dev < 64, "device ordinal out of range");
     cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 2;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.blockDim = dim3(THREADS);
     cfg.dynamicSmemBytes = SMEM_BYTES;
     cfg.stream = st;
@@ -1153,6 +1171,7 @@ ctk_status launch_product(const CUtensorMap& a, const CUtensorMap& b, Params P, 
     P.tiles_n = (P.n + T - 1) / T;
     P.units = MODE == APPLY ? P.tiles_m * P.tiles_n : P.tiles_n * (P.tiles_n + 1) / 2;
     cfg.gridDim = dim3(static_cast<unsigned>(2 * (P.units < at_once ? P.units : at_once)));
+    cfg.numAttrs = 2;
     CTK_CUDA(cudaLaunchKernelEx(&cfg, kernel, a, b, P));
     CTK_LAUNCH_CHECK("ns_product_kernel");
     return CTK_OK;
@@ -1211,8 +1230,8 @@ struct Layout {
     int64_t pitch_x, pitch_d;
 };
 constexpr int MAX_PARTS = 1024, MAX_STEPS = 64;
-// Short sides up to this take the medium kernels (with / without: 1100 x 1100 255 / 575 us, 2048 x 2048 597 / 922, 2048 x 4096
-// 1019 / 1248, 2500 x 2500 1454 / 1253).
+// Short sides up to this take the medium kernels (with / without: 1300 x 1300 302 / 533 us, 2048 x 2048 544 / 729, 2048 x 4096
+// 863 / 1084, 2500 x 2500 1454 / 1253 before the pairs' epilogue was made shorter).
 constexpr int64_t MID_SIDE = 2048;
 Layout layout_for(int64_t rows, int64_t cols) {
     Layout L;
@@ -1250,6 +1269,9 @@ ctk_status run_steps(const Layout& L, char* ws, int64_t rows, int64_t cols, Sink
     if (!rc) rc = make_map(&mb, B, d, d, 128);
     const float* coef = reinterpret_cast<const float*>(ws + L.coef);
     const bool medium = d <= MID_SIDE;
+    // B X of a medium matrix that has more 128 x 128 tiles than SMs: the pairs' 256 x 256 tiles take half the operand traffic and
+    // no second round (with / without: 784 x 4096 283 / 300 us, 2048 x 2048 533 / 593, 2048 x 4096 843 / 988)
+    const int64_t apply_tiles = ((rows + BM - 1) / BM) * ((cols + BM - 1) / BM);
     float4* sums = reinterpret_cast<float4*>(ws + L.sums);
     auto blocks = [](int64_t k) { return static_cast<int>((k + BK - 1) / BK); };
     for (int s = 0; s < steps && !rc; ++s) {
@@ -1274,7 +1296,7 @@ ctk_status run_steps(const Layout& L, char* ws, int64_t rows, int64_t cols, Sink
         P.src = X[at];
         P.dst = X[at ^ 1];
         P.last = s + 1 == steps;
-        if (medium) rc = tall ? launch_tile<APPLY, false, false>(mx_k[at], mb, P, sums, st) : launch_tile<APPLY, false, true>(mb, mx_mn[at], P, sums, st);
+        if (medium && apply_tiles <= ctk::sm_count()) rc = tall ? launch_tile<APPLY, false, false>(mx_k[at], mb, P, sums, st) : launch_tile<APPLY, false, true>(mb, mx_mn[at], P, sums, st);
         else rc = tall ? launch_product<APPLY, false, false>(mx_k[at], mb, P, st) : launch_product<APPLY, false, true>(mb, mx_mn[at], P, st);
     }
     return rc;
