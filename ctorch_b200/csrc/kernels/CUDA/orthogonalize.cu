@@ -1270,8 +1270,10 @@ ctk_status run_steps(const Layout& L, char* ws, int64_t rows, int64_t cols, Sink
     const float* coef = reinterpret_cast<const float*>(ws + L.coef);
     const bool medium = d <= MID_SIDE;
     // B X of a medium matrix that has more 128 x 128 tiles than SMs: the pairs' 256 x 256 tiles take half the operand traffic and
-    // no second round (with / without: 784 x 4096 283 / 300 us, 2048 x 2048 533 / 593, 2048 x 4096 843 / 988)
-    const int64_t apply_tiles = ((rows + BM - 1) / BM) * ((cols + BM - 1) / BM);
+    // no second round (with / without: 784 x 4096 283 / 300 us, 2048 x 2048 533 / 593, 2048 x 4096 843 / 988) -- unless too much
+    // of them lies past the edges (300 x 20000 389 / 370, 50000 x 128 384 / 336, 20 x 100000 558 / 387)
+    const int64_t apply_tiles = ((rows + BM - 1) / BM) * ((cols + BM - 1) / BM), pair_tiles = ((rows + 2 * BM - 1) / (2 * BM)) * ((cols + 2 * BM - 1) / (2 * BM));
+    const bool apply_pairs = !medium || (apply_tiles > ctk::sm_count() && 16 * pair_tiles <= 5 * apply_tiles);
     float4* sums = reinterpret_cast<float4*>(ws + L.sums);
     auto blocks = [](int64_t k) { return static_cast<int>((k + BK - 1) / BK); };
     for (int s = 0; s < steps && !rc; ++s) {
@@ -1296,7 +1298,7 @@ ctk_status run_steps(const Layout& L, char* ws, int64_t rows, int64_t cols, Sink
         P.src = X[at];
         P.dst = X[at ^ 1];
         P.last = s + 1 == steps;
-        if (medium && apply_tiles <= ctk::sm_count()) rc = tall ? launch_tile<APPLY, false, false>(mx_k[at], mb, P, sums, st) : launch_tile<APPLY, false, true>(mb, mx_mn[at], P, sums, st);
+        if (!apply_pairs) rc = tall ? launch_tile<APPLY, false, false>(mx_k[at], mb, P, sums, st) : launch_tile<APPLY, false, true>(mb, mx_mn[at], P, sums, st);
         else rc = tall ? launch_product<APPLY, false, false>(mx_k[at], mb, P, st) : launch_product<APPLY, false, true>(mb, mx_mn[at], P, st);
     }
     return rc;
