@@ -535,8 +535,9 @@ __device__ __forceinline__ void join8(const uint4& hi, const uint4& lo, float (&
 // and a CTA alone takes its operands from L2 at one SM's rate (64 KB a k-block, about 0.9 us).  The CTAs' sums meet in L2
 // (fp32, [column quad][row], so that a warp's store is one run); after a cluster barrier each CTA adds 128 / split
 // columns over all of them, in rank order, and takes these through the epilogue from shared memory -- compact loops,
-// because at these sizes straight-line code spends its time on instruction fetches (the persistent kernel's unrolled
-// epilogue took 10 us for its one tile).
+// because at these sizes straight-line code spends its time on instruction fetches.  What bounds it up to d of about 600 is
+// latency, 6.7 - 8.5 us a launch: 1.4 us from one launch to the next, 1.4 to the first accumulator, 3 for the sums to meet, 1 for
+// the epilogue.
 constexpr int MID_THREADS = 576;  // warp 0 loads, warp 1 multiplies, warps 2-17: 4 per quarter of the rows, 32 columns each
 constexpr int MID_MAX_CTAS = 160, MAX_SLABS = 16;
 constexpr int MID_SMEM = STAGES * STAGE_BYTES + 1024;
@@ -789,8 +790,7 @@ __global__ void __launch_bounds__(256) ns_join_kernel(const Params P) {
 //   A A, B and B X in each CTA for itself.
 // Everything a product reads is there before it starts, so the small terms go first; an accumulator takes half of K.
 // What bounds it is latency: at 784 x 128 a step is 12 us, half of it
-// hand-overs between the CTAs.  (The exchange through the other CTAs' shared memory
-// instead of L2 took 18000 of 37000 clocks a step there: 64 KB in and out of every CTA at 7 bytes a clock.)
+// hand-overs between the CTAs.  (The exchange through the other CTAs' shared memory instead of L2 took 18000 of 37000 clocks a step there: 64 KB in and out of every CTA at 7 bytes a clock.)
 constexpr int CL_THREADS = 512;                    // 4 warps per quarter of the accumulator's rows, 32 columns each
 constexpr int CL_SIDE = 128;                       // largest d, widest slab
 constexpr int CL_GROUP = CL_SIDE * 128;            // bytes of a 64-wide column group of a matrix of 128 rows
@@ -1190,9 +1190,10 @@ ctk_status launch_tile(const CUtensorMap& a, const CUtensorMap& b, Params P, flo
     P.tiles_m = (P.m + BM - 1) / BM;
     P.tiles_n = (P.n + BM - 1) / BM;
     P.units = MODE == APPLY ? P.tiles_m * P.tiles_n : P.tiles_n * (P.tiles_n + 1) / 2;
-    // as many CTAs to a tile as the SMs hold at once, each with a k-block at least
+    // as many CTAs to a tile as the SMs hold at once, each with a k-block at least, where four k-blocks or more pay for the
+    // hand-over (130 x 140, three of them: 116 us in one CTA, 136 in two; 256 x 256, four: 144 and 116 us in four)
     P.split = 1;
-    while (P.split < 8 && P.units * P.split * 2 <= MID_MAX_CTAS && P.units * P.split * 2 <= ctk::sm_count() && P.split * 2 <= P.num_kb) P.split *= 2;
+    while (P.split < 8 && P.num_kb >= 4 && P.units * P.split * 2 <= MID_MAX_CTAS && P.units * P.split * 2 <= ctk::sm_count() && P.split * 2 <= P.num_kb) P.split *= 2;
     // a long, thin matrix has few tiles and very many k-blocks: several clusters to a tile (128 x 50000: 336 us in all)
     P.slabs = 1;
     if (MODE == GRAM && P.split == 8)
