@@ -403,7 +403,7 @@ ctk_status ctk_matmul_status(int* status);
  * (A = X^T X and X on the left where rows > cols), (a, b, c) = (3.4445, -4.7750, 2.0315).
  * g is [rows, cols] with row pitch ldg >= cols, out with row pitch ldo >= cols (elements; any 4-byte
  * aligned pointers); out == g with the same pitch is allowed, other overlaps are not.  fp32-level accuracy: the products
- * take both operands as 22-bit fixed-precision pairs of fp16 and are summed in fp32 with rounding.  A
+ * take both operands as pairs of fp16 (22 bits, and no finer than 2^-39) and are summed in fp32 with rounding.  A
  * non-finite element of g makes every element of out NaN; g == 0 gives 0.  The same bits from call to call.
  * workspace: ctk_orthogonalize_workspace_bytes(rows, cols) bytes of device memory, 256-byte aligned, that
  * no other running call uses, or NULL: taken from the device's pool for the duration of the call, in
