@@ -14,6 +14,13 @@ constexpr int W4_THREADS = 128;  // neighbouring columns: 512 contiguous bytes o
 // two halves of a register.
 __host__ __device__ constexpr int nibble_shift(int i) { return 4 * (i >> 1) + 16 * (i & 1); }
 
+// the larger one, a NaN if either is one
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
 // ---- quantise ------------------------------------------------------------------------------------------
 // A thread owns 32 or 64 k of one column: lanes are neighbouring columns (coalesced rows of w), the values stay in registers
 // between the maximum and the rounding, so w is read once with that many loads in flight; the two halves of a group of 128
@@ -23,7 +30,8 @@ __host__ __device__ constexpr int nibble_shift(int i) { return 4 * (i >> 1) + 16
 // off; the remainder d = w - q s is exact in one fma (|d| <= s (1/2 + tiny), a multiple of the smaller of both ulps), so only
 // where |d| >= s / 2 is there anything to decide, which the word's eight codes ask about together.
 // (With a rounding, a conversion to int and three comparisons per value: 36 instructions and 50 us at 4096 x 4096,
-// this way 20 us.)
+// this way 20 us.  The codes are added up shifted, with the bits above them, and those taken off once a word: 256 against 234 us
+// for 16384 x 16384 g128.)
 __device__ __forceinline__ uint32_t exact_code(float w, float s, float t, float q) {
     const float d = fmaf(-q, s, w), e = 2.0f * fabsf(d);
     if (e > s || (e == s && ((__float_as_uint(q + 12582912.0f)) & 1u))) t += d > 0.0f ? 1.0f : -1.0f;
@@ -50,27 +58,25 @@ __global__ void __launch_bounds__(W4_THREADS * (GROUP == 128 ? 2 : 1)) w4_quanti
 #pragma unroll
         for (int i = 0; i < LEN; ++i) v[i] = i < len ? __ldcs(src + i * ldw) : 0.0f;
     }
-    float top = 0.0f, bottom = 0.0f, poison = 0.0f;
+    float top = 0.0f, bottom = 0.0f;  // (a NaN stays in top, an infinity in either)
 #pragma unroll
     for (int i = 0; i < LEN; ++i) {
-        top = fmaxf(top, SYM ? fabsf(v[i]) : v[i]);
+        top = max_nan(top, SYM ? fabsf(v[i]) : v[i]);
         if (!SYM) bottom = fminf(bottom, v[i]);
-        poison = fmaf(v[i], 0.0f, poison);  // NaN once a value is not finite
     }
     if constexpr (GROUP == 128) {
-        __shared__ float ends[3][2][W4_THREADS];
+        __shared__ float ends[2][2][W4_THREADS];
         ends[0][part][lane_col] = top;
         ends[1][part][lane_col] = bottom;
-        ends[2][part][lane_col] = poison;
         __syncthreads();
-        top = fmaxf(ends[0][0][lane_col], ends[0][1][lane_col]);
+        top = max_nan(ends[0][0][lane_col], ends[0][1][lane_col]);
         bottom = fminf(ends[1][0][lane_col], ends[1][1][lane_col]);
-        poison = ends[2][0][lane_col] + ends[2][1][lane_col];
     }
     if (!there) return;
     // the one division of the group, in 64 bits so that the scale is the nearest fp32 number
-    const float s = poison == 0.0f ? static_cast<float>(SYM ? static_cast<double>(top) / 7.0 : (static_cast<double>(top) - static_cast<double>(bottom)) / 15.0)
-                                   : __int_as_float(0x7fc00000);
+    const bool finite = top < __int_as_float(0x7f800000) && bottom > __int_as_float(0xff800000);
+    const float s = finite ? static_cast<float>(SYM ? static_cast<double>(top) / 7.0 : (static_cast<double>(top) - static_cast<double>(bottom)) / 15.0)
+                           : __int_as_float(0x7fc00000);
     const bool live = s > 0.0f;  // false for a group of zeros and for NaN
     float zero = 8.0f;
     if (!SYM) zero = live ? static_cast<float>(rint(-static_cast<double>(bottom) / static_cast<double>(s))) : 0.0f;
@@ -89,23 +95,27 @@ __global__ void __launch_bounds__(W4_THREADS * (GROUP == 128 ? 2 : 1)) w4_quanti
             }
             dst[wd] = word;
         }
+    } else if (!live) {  // zeros, or a value that is not finite: every code the zero point
+#pragma unroll
+        for (int wd = 0; wd < LEN / 8; ++wd) dst[wd] = SYM ? 0x88888888u : 0u;
     } else {
-        const float base = 12582912.0f + zero, half = live ? 0.5f * s : __int_as_float(0x7f800000), step = live ? s : 0.0f;
+        const float base = 12582912.0f + zero, half = 0.5f * s;
 #pragma unroll
         for (int q4 = 0; q4 < LEN / 32; ++q4) {
             uint32_t out[4];
 #pragma unroll
             for (int wd = 0; wd < 4; ++wd) {
-                uint32_t word = 0;
+                uint32_t word = 0;  // t's bits are 0x4B400000 + code: added up shifted, the constants taken off once
                 bool close = false;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const float x = live ? v[q4 * 32 + wd * 8 + i] : 0.0f;
+                    const float x = v[q4 * 32 + wd * 8 + i];
                     float t = fmaf(x, inv, base);
-                    close |= fabsf(fmaf(base - t, step, x)) >= half;
+                    close |= fabsf(fmaf(base - t, s, x)) >= half;
                     if (!SYM) t = fminf(t, 12582927.0f);  // (symmetric: 1 .. 15 by construction; the lower end as well)
-                    word |= (__float_as_uint(t) & 15u) << nibble_shift(i);
+                    word += __float_as_uint(t) << nibble_shift(i);
                 }
+                word -= 0x4B400000u * 0x11111111u;
                 if (close) {
                     word = 0;
 #pragma unroll
@@ -126,7 +136,8 @@ __global__ void __launch_bounds__(W4_THREADS * (GROUP == 128 ? 2 : 1)) w4_quanti
 }
 
 // ---- dequantise ----------------------------------------------------------------------------------------
-// A thread takes 32 k of one column: one 16-byte load of codes, 32 coalesced stores (lanes are columns).
+// A thread takes 32 k of one column: one 16-byte load of codes, 32 coalesced stores (lanes are columns).  16384 x 16384 g64 206 us,
+// 5.6 TB/s (with a shift and a conversion to float per value 233).
 __global__ void __launch_bounds__(W4_THREADS) w4_dequantize_kernel(const uint32_t* __restrict__ packed, const float* __restrict__ scales,
                                                                    const uint8_t* __restrict__ zeros, int64_t k, int64_t n, int group, int64_t groups,
                                                                    float* __restrict__ w, int64_t ldw) {
@@ -139,10 +150,24 @@ __global__ void __launch_bounds__(W4_THREADS) w4_dequantize_kernel(const uint32_
     const float zero = zeros ? static_cast<float>(zeros[j * groups + grp]) : 8.0f;
     const uint32_t word[4] = {c.x, c.y, c.z, c.w};
     float* dst = w + k0 * ldw + j;
-    const int len = static_cast<int>(k - k0 < 32 ? k - k0 : 32);
+    // the nibble at bit 4p under an exponent of 23 - 4p is the number 2^(23 - 4p) + code: no conversion, no shift
+    float base[4];
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
-        if (i < len) __stcs(dst + i * ldw, (static_cast<float>((word[i >> 3] >> nibble_shift(i & 7)) & 15u) - zero) * s);
+    for (int p = 0; p < 4; ++p) base[p] = static_cast<float>(1 << (23 - 4 * p)) + zero;
+    auto value = [&](int i) {
+        const int p = (i & 7) >> 1;
+        const uint32_t half = i & 1 ? word[i >> 3] >> 16 : word[i >> 3];
+        return (__uint_as_float((half & (15u << (4 * p))) | (static_cast<uint32_t>(150 - 4 * p) << 23)) - base[p]) * s;
+    };
+    if (k - k0 >= 32) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) __stcs(dst + i * ldw, value(i));
+    } else {
+        const int len = static_cast<int>(k - k0);
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+            if (i < len) __stcs(dst + i * ldw, value(i));
+    }
 }
 
 // ---- y = [relu](x W + bias) ------------------------------------------------------------------------------
