@@ -38,16 +38,19 @@ __device__ __forceinline__ uint32_t exact_code(float w, float s, float t, float 
     return __float_as_uint(fminf(fmaxf(t, 12582912.0f), 12582927.0f)) & 15u;
 }
 
+// Threads that share a column of a CTA: 4 groups of 32, one of 64 (two of them: 262 us for 16384 x 16384 with zero points, 232
+// alone), or the halves of one of 128.
+__host__ __device__ constexpr int quantize_parts(int group) { return group == 32 ? 4 : group == 64 ? 1 : 2; }
 template <int GROUP, bool SYM>
-__global__ void __launch_bounds__(W4_THREADS * (GROUP == 128 ? 2 : 1)) w4_quantize_kernel(const float* __restrict__ w, int64_t ldw, int64_t k, int64_t n, int64_t groups,
+__global__ void __launch_bounds__(W4_THREADS * quantize_parts(GROUP)) w4_quantize_kernel(const float* __restrict__ w, int64_t ldw, int64_t k, int64_t n, int64_t groups,
                                                                                            uint32_t* __restrict__ packed, float* __restrict__ scales,
-                                                                                           uint8_t* __restrict__ zeros) {
-    constexpr int LEN = GROUP == 128 ? 64 : GROUP;  // of this thread
+                                                                                           uint8_t* __restrict__ zeros, bool wide) {
+    constexpr int LEN = GROUP == 128 ? 64 : GROUP, PARTS = quantize_parts(GROUP), GROUPS = PARTS * LEN / GROUP;  // k of a thread; threads and groups of a column
     const uint32_t col_blocks = static_cast<uint32_t>((n + W4_THREADS - 1) / W4_THREADS);
     const int lane_col = threadIdx.x % W4_THREADS, part = threadIdx.x / W4_THREADS;
-    const int64_t j = static_cast<int64_t>(blockIdx.x % col_blocks) * W4_THREADS + lane_col, grp = blockIdx.x / col_blocks;
-    const bool there = j < n;
-    const int64_t k0 = grp * GROUP + part * LEN;
+    const int64_t j = static_cast<int64_t>(blockIdx.x % col_blocks) * W4_THREADS + lane_col, first = blockIdx.x / col_blocks * GROUPS;
+    const int64_t k0 = first * GROUP + part * LEN;
+    const bool there = j < n && k0 < groups * GROUP;
     const int len = !there || k0 >= k ? 0 : static_cast<int>(k - k0 < LEN ? k - k0 : LEN);
     const float* src = w + k0 * ldw + j;
     float v[LEN];
@@ -72,7 +75,6 @@ __global__ void __launch_bounds__(W4_THREADS * (GROUP == 128 ? 2 : 1)) w4_quanti
         top = max_nan(ends[0][0][lane_col], ends[0][1][lane_col]);
         bottom = fminf(ends[1][0][lane_col], ends[1][1][lane_col]);
     }
-    if (!there) return;
     // the one division of the group, in 64 bits so that the scale is the nearest fp32 number
     const bool finite = top < __int_as_float(0x7f800000) && bottom > __int_as_float(0xff800000);
     const float s = finite ? static_cast<float>(SYM ? static_cast<double>(top) / 7.0 : (static_cast<double>(top) - static_cast<double>(bottom)) / 15.0)
@@ -83,7 +85,8 @@ __global__ void __launch_bounds__(W4_THREADS * (GROUP == 128 ? 2 : 1)) w4_quanti
     if (!SYM && zero > 15.0f) zero = 15.0f;  // (subnormal scales only: the range is no longer 15 steps wide)
     const float inv = live ? 1.0f / s : 0.0f;
     uint32_t* dst = packed + j * (groups * (GROUP / 8)) + k0 / 8;
-    if (!(inv <= 3.0e38f)) {  // a subnormal scale, 1/s overflows: divide in 64 bits, one by one (rare: no code of it in the loop below)
+    if (!there) {
+    } else if (!(inv <= 3.0e38f)) {  // a subnormal scale, 1/s overflows: divide in 64 bits, one by one (rare: no code of it in the loop below)
 #pragma unroll 1
         for (int wd = 0; wd < LEN / 8; ++wd) {
             uint32_t word = 0;
@@ -129,9 +132,29 @@ __global__ void __launch_bounds__(W4_THREADS * (GROUP == 128 ? 2 : 1)) w4_quanti
             *reinterpret_cast<uint4*>(dst + q4 * 4) = make_uint4(out[0], out[1], out[2], out[3]);
         }
     }
-    if (part == 0) {
-        scales[j * groups + grp] = s;
-        if (!SYM) zeros[j * groups + grp] = static_cast<uint8_t>(zero);
+    if constexpr (GROUPS == 1) {
+        if (part == 0 && there) {
+            scales[j * groups + first] = s;
+            if (!SYM) zeros[j * groups + first] = static_cast<uint8_t>(zero);
+        }
+    } else {  // a column's four groups together: one by one, each store is a sector of its own (16384 x 16384 308 us, this way 263)
+        __shared__ float group_scales[GROUPS][W4_THREADS];
+        __shared__ uint8_t group_zeros[GROUPS][W4_THREADS];
+        group_scales[part][lane_col] = s;
+        group_zeros[part][lane_col] = static_cast<uint8_t>(zero);
+        __syncthreads();
+        if (part != 0 || j >= n) return;
+        const int64_t at = j * groups + first;
+        if (wide && groups % 4 == 0) {
+            *reinterpret_cast<float4*>(scales + at) = make_float4(group_scales[0][lane_col], group_scales[1][lane_col], group_scales[2][lane_col], group_scales[3][lane_col]);
+            if (!SYM)
+                *reinterpret_cast<uchar4*>(zeros + at) = make_uchar4(group_zeros[0][lane_col], group_zeros[1][lane_col], group_zeros[2][lane_col], group_zeros[3][lane_col]);
+            return;
+        }
+        for (int g = 0; g < GROUPS && first + g < groups; ++g) {
+            scales[at + g] = group_scales[g][lane_col];
+            if (!SYM) zeros[at + g] = group_zeros[g][lane_col];
+        }
     }
 }
 
@@ -730,9 +753,11 @@ ctk_status ctk_w4_quantize_f32(const float* w, int64_t ldw, int64_t k, int64_t n
     CTK_REQUIRE(w && packed && scales, "ctk_w4_quantize_f32: null pointer");
     CTK_REQUIRE((reinterpret_cast<uintptr_t>(packed) & 15u) == 0, "ctk_w4_quantize_f32: packed must be 16-byte aligned");
     CTK_REQUIRE(aligned_to(w, 4) && aligned_to(scales, 4), "ctk_w4_quantize_f32: misaligned pointer");
-    const int64_t groups = (k + group - 1) / group, grid = groups * ((n + W4_THREADS - 1) / W4_THREADS);
+    const int64_t groups = (k + group - 1) / group, per_cta = group == 32 ? quantize_parts(32) : 1;
+    const int64_t grid = (groups + per_cta - 1) / per_cta * ((n + W4_THREADS - 1) / W4_THREADS);
     if (grid > 0x7FFFFFFF) return fail(CTK_ERR_LIMIT, "ctk_w4_quantize_f32: too many groups");
-    auto go = [&](auto kernel) { kernel<<<static_cast<unsigned>(grid), W4_THREADS * (group == 128 ? 2 : 1), 0, as_stream(stream)>>>(w, ldw, k, n, groups, packed, scales, zeros); };
+    const bool wide = aligned_to(scales, 16) && aligned_to(zeros, 4);
+    auto go = [&](auto kernel) { kernel<<<static_cast<unsigned>(grid), W4_THREADS * quantize_parts(group), 0, as_stream(stream)>>>(w, ldw, k, n, groups, packed, scales, zeros, wide); };
     if (zeros) group == 32 ? go(w4_quantize_kernel<32, false>) : group == 64 ? go(w4_quantize_kernel<64, false>) : go(w4_quantize_kernel<128, false>);
     else group == 32 ? go(w4_quantize_kernel<32, true>) : group == 64 ? go(w4_quantize_kernel<64, true>) : go(w4_quantize_kernel<128, true>);
     CTK_LAUNCH_CHECK("w4_quantize");

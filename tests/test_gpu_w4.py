@@ -281,3 +281,24 @@ def test_matmul_w4_input_and_result_in_one_buffer(cb):
         keep = np.ones(ld, bool)
         keep[at_y:at_y + n] = False
         assert np.array_equal(after[:, keep], before[:, keep])
+
+
+@pytest.mark.parametrize("group", [32, 128])
+def test_scales_and_zeros_at_odd_addresses(cb, group):
+    """Scales 4 bytes and zero points 1 byte past an aligned address: the same bits, nothing around them written."""
+    rng = np.random.default_rng(group)
+    k, n, m = 4 * group, 150, 3
+    groups = k // group
+    w = cb.to_device(rng.standard_normal((k, n)).astype(np.float32))
+    want = cb.ops.w4_quantize(w, group=group, symmetric=False)
+    scales = cb.to_device(np.full(n * groups + 2, -1.0, np.float32))
+    zeros = cb.to_device(np.full(n * groups + 2, 77, np.uint8), np.uint8)
+    odd = cb.ops.W4Weight(cb.empty((n, k // 8), np.uint32), scales.view(1, (n, groups)), zeros.view(1, (n, groups)), k, n, group)
+    cb.ops.w4_quantize(w, group=group, symmetric=False, out=odd)
+    assert np.array_equal(odd.packed.numpy(), want.packed.numpy())
+    s, z = scales.numpy(), zeros.numpy()
+    assert np.array_equal(s[1:-1].reshape(n, groups), want.scales.numpy()) and s[0] == -1.0 and s[-1] == -1.0
+    assert np.array_equal(z[1:-1].reshape(n, groups), want.zeros.numpy()) and z[0] == 77 and z[-1] == 77
+    x = cb.to_device(rng.standard_normal((m, k)).astype(np.float32))
+    assert np.array_equal(cb.ops.w4_dequantize(odd).numpy(), cb.ops.w4_dequantize(want).numpy())
+    assert np.array_equal(cb.ops.matmul_w4(x, odd).numpy(), cb.ops.matmul_w4(x, want).numpy())
