@@ -24,7 +24,7 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 // ---- quantise ------------------------------------------------------------------------------------------
 // A thread owns 32 or 64 k of one column: lanes are neighbouring columns (coalesced rows of w), the values stay in registers
 // between the maximum and the rounding, so w is read once with that many loads in flight; the two halves of a group of 128
-// exchange their extremes through shared memory.  Bound by instruction issue before w's bytes, hence the rounding:
+// exchange their extremes through shared memory.  Bound by instruction issue until the rounding became what it is:
 //
 // round(w / s) exactly, ties to even: t = fma(w, 1/s, 1.5 * 2^23 + zero) has the code in its low bits and is at most one step
 // off; the remainder d = w - q s is exact in one fma (|d| <= s (1/2 + tiny), a multiple of the smaller of both ulps), so only
