@@ -789,13 +789,14 @@ __global__ void __launch_bounds__(256) ns_join_kernel(const Params P) {
 //   writes A's hi and lo as shared memory has them -> global | cluster barrier | one bulk copy per array brings A back |
 //   A A, B and B X in each CTA for itself.
 // Everything a product reads is there before it starts, so the small terms go first; an accumulator takes half of K.
-// What bounds it is latency: at 784 x 128 a step is 12 us, half of it
-// hand-overs between the CTAs.  (The exchange through the other CTAs' shared memory instead of L2 took 18000 of 37000 clocks a step there: 64 KB in and out of every CTA at 7 bytes a clock.)
+// What bounds it is latency: at 784 x 128 a step is 10 us, half of it
+// hand-overs between the CTAs, and what comes before and after the steps 11.  (The exchange through the other CTAs' shared memory instead of L2 took 18000 of 37000 clocks a step there: 64 KB in and out of every CTA at 7 bytes a clock.)
 constexpr int CL_THREADS = 512;                    // 4 warps per quarter of the accumulator's rows, 32 columns each
 constexpr int CL_SIDE = 128;                       // largest d, widest slab
 constexpr int CL_GROUP = CL_SIDE * 128;            // bytes of a 64-wide column group of a matrix of 128 rows
 constexpr int CL_MATRIX = 4 * CL_GROUP;            // hi: 2 groups, lo: 2 groups
-constexpr int CL_PITCH = 132;                      // floats per row of the fp32 buffer
+constexpr int CL_PITCH = 132, CL_PITCH_TALL = 129;  // floats per row of the fp32 buffer, which a tall G enters and leaves down its
+                                                    // columns (784 x 128 with 132: 65.4 us, with 129: 60.5)
 constexpr int CL_MAX = 16;                         // CTAs of a cluster
 constexpr int CL_SMEM = 2 * CL_MATRIX + CL_SIDE * CL_PITCH * 4 + 1024;
 constexpr int CL_PARTIAL = CL_SIDE * CL_SIDE * 4;  // bytes of one CTA's X X^T
@@ -808,14 +809,14 @@ struct ClusterArgs {
     Source S;
     Sink K;
     int d, length, slab;  // short side, long side, columns of the long side per CTA (a multiple of 16)
-    int tall, steps;
+    int steps;
     float eps;
     float4* partial;      // [C][32 column quads][128 rows]
     uint8_t* image;       // A as it lies in shared memory
 };
 
 // V elements of the long (wide G) or the short side (tall G), whichever is contiguous, at a time.
-template <int V, bool MOMENTUM>
+template <int V, bool MOMENTUM, bool TALL>
 __global__ void __launch_bounds__(CL_THREADS, 1) ns_cluster_kernel(const ClusterArgs P) {
     using namespace t5;
     extern __shared__ uint8_t smem_raw[];
@@ -833,6 +834,7 @@ __global__ void __launch_bounds__(CL_THREADS, 1) ns_cluster_kernel(const Cluster
     const int d = P.d, d16 = (d + 15) & ~15, w16 = P.slab, n0 = rank * P.slab;
     const int width = P.length - n0 < P.slab ? (P.length - n0 > 0 ? P.length - n0 : 0) : P.slab;  // this CTA's part that exists
 
+    constexpr int pitch = TALL ? CL_PITCH_TALL : CL_PITCH;
     if (tid == 0) {
         abort_flag = 0;
         mbar_init(bar, 1);
@@ -843,11 +845,11 @@ __global__ void __launch_bounds__(CL_THREADS, 1) ns_cluster_kernel(const Cluster
     // every operand byte a product may touch is defined: rows and columns past d and the slab are zero
     for (int i = tid; i < 2 * CL_MATRIX / 16; i += CL_THREADS) *reinterpret_cast<uint4*>(smem + i * 16) = make_uint4(0u, 0u, 0u, 0u);
     if (width < w16)
-        for (int t = tid; t < d * (w16 - width); t += CL_THREADS) E[(t % d) * CL_PITCH + width + t / d] = 0.0f;
+        for (int t = tid; t < d * (w16 - width); t += CL_THREADS) E[(t % d) * pitch + width + t / d] = 0.0f;
 
     // ---- U into E, the momentum update, the norm ----
     const Source& S = P.S;
-    const int fast = (P.tall ? d : width) / V, total = (P.tall ? width : d) * fast;  // accesses of V elements
+    const int fast = (TALL ? d : width) / V, total = (TALL ? width : d) * fast;  // accesses of V elements
     constexpr int U = 4;                                                           // of them in flight per thread
     double acc = 0.0;
     for (int t0 = tid; t0 < total; t0 += U * CL_THREADS) {
@@ -859,7 +861,7 @@ __global__ void __launch_bounds__(CL_THREADS, 1) ns_cluster_kernel(const Cluster
             sl[k] = t / fast;
             fa[k] = (t - sl[k] * fast) * V;
             if (t >= total) continue;
-            const int64_t r = P.tall ? n0 + sl[k] : sl[k], c = P.tall ? fa[k] : n0 + fa[k];
+            const int64_t r = TALL ? n0 + sl[k] : sl[k], c = TALL ? fa[k] : n0 + fa[k];
             u[k] = load_vec<V>(S.g + r * S.ldg + c);
             if (MOMENTUM) m[k] = load_vec<V>(S.momentum + r * S.ldm + c);
         }
@@ -872,12 +874,12 @@ __global__ void __launch_bounds__(CL_THREADS, 1) ns_cluster_kernel(const Cluster
                     m[k].v[q] = fmaf(S.mu, m[k].v[q], u[k].v[q]);
                     u[k].v[q] = S.nesterov ? fmaf(S.mu, m[k].v[q], u[k].v[q]) : m[k].v[q];
                 }
-                *reinterpret_cast<Vec<V>*>(S.momentum + (P.tall ? n0 + sl[k] : sl[k]) * S.ldm + (P.tall ? fa[k] : n0 + fa[k])) = m[k];
+                *reinterpret_cast<Vec<V>*>(S.momentum + (TALL ? n0 + sl[k] : sl[k]) * S.ldm + (TALL ? fa[k] : n0 + fa[k])) = m[k];
             }
 #pragma unroll
             for (int q = 0; q < V; ++q) {
                 acc = fma(static_cast<double>(u[k].v[q]), static_cast<double>(u[k].v[q]), acc);
-                E[(P.tall ? fa[k] + q : sl[k]) * CL_PITCH + (P.tall ? sl[k] : fa[k] + q)] = u[k].v[q];
+                E[(TALL ? fa[k] + q : sl[k]) * pitch + (TALL ? sl[k] : fa[k] + q)] = u[k].v[q];
             }
         }
     }
@@ -900,7 +902,7 @@ __global__ void __launch_bounds__(CL_THREADS, 1) ns_cluster_kernel(const Cluster
         const int i = t / (w16 / 8), c = t % (w16 / 8);
         float x[8];
 #pragma unroll
-        for (int q = 0; q < 8; ++q) x[q] = (E[i * CL_PITCH + c * 8 + q] * N.p2) * (N.rest * kScaleX);
+        for (int q = 0; q < 8; ++q) x[q] = (E[i * pitch + c * 8 + q] * N.p2) * (N.rest * kScaleX);
         uint4 hi, lo;
         split8(x, hi, lo);
         *reinterpret_cast<uint4*>(X + cl_chunk(i, c)) = hi;
@@ -1079,9 +1081,14 @@ __global__ void __launch_bounds__(CL_THREADS, 1) ns_cluster_kernel(const Cluster
 #pragma unroll
                 for (int k = 0; k < 8; ++k) x[k] = f * fmaf(kA, x[k], v[q * 8 + k] * (1.0f / 16384.0f));
                 if (last) {
-                    float4* out = reinterpret_cast<float4*>(E + row * CL_PITCH + c0 + q * 8);
-                    out[0] = make_float4(x[0], x[1], x[2], x[3]);
-                    out[1] = make_float4(x[4], x[5], x[6], x[7]);
+                    float* out = E + row * pitch + c0 + q * 8;
+                    if constexpr (TALL) {
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) out[k] = x[k];
+                    } else {
+                        reinterpret_cast<float4*>(out)[0] = make_float4(x[0], x[1], x[2], x[3]);
+                        reinterpret_cast<float4*>(out)[1] = make_float4(x[4], x[5], x[6], x[7]);
+                    }
                 } else {
                     split8(x, hi, lo);
                     *chunk_of(X, q, 0) = hi;
@@ -1101,7 +1108,7 @@ __global__ void __launch_bounds__(CL_THREADS, 1) ns_cluster_kernel(const Cluster
 #pragma unroll
         for (int k = 0; k < U; ++k) {
             const int t = t0 + k * CL_THREADS, sl = t / fast, fa = (t - sl * fast) * V;
-            at[k] = P.K.out + (P.tall ? n0 + sl : sl) * P.K.ldo + (P.tall ? fa : n0 + fa);
+            at[k] = P.K.out + (TALL ? n0 + sl : sl) * P.K.ldo + (TALL ? fa : n0 + fa);
             if (P.K.update && t < total) old[k] = load_vec<V>(at[k]);
         }
 #pragma unroll
@@ -1111,7 +1118,7 @@ __global__ void __launch_bounds__(CL_THREADS, 1) ns_cluster_kernel(const Cluster
             Vec<V> o;
 #pragma unroll
             for (int q = 0; q < V; ++q)
-                o.v[q] = sink_value(P.K, E[(P.tall ? fa + q : sl) * CL_PITCH + (P.tall ? sl : fa + q)] * (1.0f / kScaleX), P.K.update ? old[k].v[q] : 0.0f);
+                o.v[q] = sink_value(P.K, E[(TALL ? fa + q : sl) * pitch + (TALL ? sl : fa + q)] * (1.0f / kScaleX), P.K.update ? old[k].v[q] : 0.0f);
             *reinterpret_cast<Vec<V>*>(at[k]) = o;
         }
     }
@@ -1305,9 +1312,9 @@ ctk_status run_steps(const Layout& L, char* ws, int64_t rows, int64_t cols, Sink
     return rc;
 }
 
-template <int V, bool MOMENTUM>
+template <int V, bool MOMENTUM, bool TALL>
 ctk_status launch_cluster(const ClusterArgs& P, int ctas, cudaStream_t st) {
-    auto kernel = ns_cluster_kernel<V, MOMENTUM>;
+    auto kernel = ns_cluster_kernel<V, MOMENTUM, TALL>;
     static ctk::PerDeviceReady ready;
     const ctk_status rc = ready.ensure([&]() -> ctk_status {
         CTK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, CL_SMEM));
@@ -1362,15 +1369,18 @@ ctk_status newton_schulz(const Source& S, Sink K, int steps, float eps, void* wo
         P.d = static_cast<int>(d);
         P.length = static_cast<int>(length);
         P.slab = static_cast<int>((length + ctas - 1) / ctas + 15) / 16 * 16;
-        P.tall = S.rows > S.cols;
         P.steps = steps;
         P.eps = eps;
         P.partial = static_cast<float4*>(workspace);
         P.image = static_cast<uint8_t*>(workspace) + static_cast<size_t>(ctas) * CL_PARTIAL;
         const bool v4 = vec && K.vec;
         cudaStream_t st = as_stream(stream);
-        if (S.momentum) return v4 ? launch_cluster<4, true>(P, ctas, st) : launch_cluster<1, true>(P, ctas, st);
-        return v4 ? launch_cluster<4, false>(P, ctas, st) : launch_cluster<1, false>(P, ctas, st);
+        if (S.rows > S.cols) {
+            if (S.momentum) return v4 ? launch_cluster<4, true, true>(P, ctas, st) : launch_cluster<1, true, true>(P, ctas, st);
+            return v4 ? launch_cluster<4, false, true>(P, ctas, st) : launch_cluster<1, false, true>(P, ctas, st);
+        }
+        if (S.momentum) return v4 ? launch_cluster<4, true, false>(P, ctas, st) : launch_cluster<1, true, false>(P, ctas, st);
+        return v4 ? launch_cluster<4, false, false>(P, ctas, st) : launch_cluster<1, false, false>(P, ctas, st);
     }
     const Layout L = layout_for(S.rows, S.cols);
     char* ws = static_cast<char*>(workspace);
