@@ -789,8 +789,9 @@ __global__ void __launch_bounds__(256) ns_join_kernel(const Params P) {
 //   writes A's hi and lo as shared memory has them -> global | cluster barrier | one bulk copy per array brings A back |
 //   A A, B and B X in each CTA for itself.
 // Everything a product reads is there before it starts, so the small terms go first; an accumulator takes half of K.
-// What bounds it is latency: at 784 x 128 a step is 10 us, half of it
-// hand-overs between the CTAs, and what comes before and after the steps 11.  (The exchange through the other CTAs' shared memory instead of L2 took 18000 of 37000 clocks a step there: 64 KB in and out of every CTA at 7 bytes a clock.)
+// What bounds it is latency: at 784 x 128 a step is 10 us, half of it hand-overs between the CTAs, and what comes before and
+// after the steps 11.  (The exchange through the other CTAs' shared memory instead of L2 took 18000 of 37000 clocks a step there:
+// 64 KB in and out of every CTA at 7 bytes a clock.)
 constexpr int CL_THREADS = 512;                    // 4 warps per quarter of the accumulator's rows, 32 columns each
 constexpr int CL_SIDE = 128;                       // largest d, widest slab
 constexpr int CL_GROUP = CL_SIDE * 128;            // bytes of a 64-wide column group of a matrix of 128 rows
