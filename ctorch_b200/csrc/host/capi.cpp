@@ -546,11 +546,11 @@ public:
     }
 
     void release_graph() {
+        graph.warm_steps = 0;  // also where nothing is recorded yet: whoever calls this changes what a step allocates
         if (!graph.exec) return;
         ctk_device_sync();
         ctk_graph_destroy(graph.exec);
         graph.exec = nullptr;
-        graph.warm_steps = 0;
         DeviceBlockCache::instance().release_graph();
         SplitBufferCache::instance().release_graph();
         if (graph_owner() == this) graph_owner() = nullptr;
@@ -564,7 +564,6 @@ public:
             graph.x = Tensor(ShapeTag{}, {static_cast<size_t>(batch), in}, DType::kFloat, DeviceType::kCUDA, false);
             graph.labels = Tensor(ShapeTag{}, {static_cast<size_t>(batch)}, DType::kFloat, DeviceType::kCUDA, false);
             graph.batch = batch;
-            graph.warm_steps = 0;
             cuda_check(ctk_device_sync(), "graph input allocation");
         }
         const size_t xb = static_cast<size_t>(batch) * in * sizeof(float), lb = static_cast<size_t>(batch) * sizeof(float);
