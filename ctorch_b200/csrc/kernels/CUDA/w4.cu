@@ -197,8 +197,8 @@ __global__ void __launch_bounds__(W4_THREADS) w4_dequantize_kernel(const uint32_
 // tcgen05 on whole numbers.  A code of 0..15 in a byte IS an e4m3 number: 0..7 are its subnormals, 8..15 its first
 // normals, and both count in steps of 2^-9, so the weight's operand is made by two masks and a shift per eight codes.  x is
 // taken in fixed point: 38 bits below the largest |x| of its row's 128 neighbours, as eight signed digits base 32, and
-// a digit of -16..15 in sign and magnitude is an e4m3 number of the same kind (16 is the last that counts in these steps).  So each (row, digit) is a column of the
-// instruction's B, every product and every sum of a group is a whole number below 2^24 times 2^-18 -- exact in the fp32
+// a digit of -16..16, doubled, in sign and magnitude is an e4m3 number of four significant bits.  So each (row, digit) is a column of the
+// instruction's B, every product and every sum of a group is a whole number below 2^24 times 2^-17 -- exact in the fp32
 // accumulator whatever it does -- and so is the zero point's share, zero * (sum of the digits).  What rounds: x to its 38 bits,
 // eight digits joined in fp32, one fma per group with the scale.
 //
@@ -282,17 +282,19 @@ __device__ __forceinline__ void write_digits(float4 x, int r, int lane, uint8_t*
     top = __reduce_max_sync(0xffffffffu, top);
     int ex = static_cast<int>(top >> 23);  // |v| < 2^(ex - 126)
     const bool bad = ex == 255;
-    ex = max(ex, 37);                      // (that far down x has fewer bits anyway)
-    const float up = __uint_as_float(static_cast<uint32_t>(127 + 164 - ex) << 23);  // |v| 2^(164 - ex) < 2^38
+    // |v| 2^(164 - ex) < 2^38.  The smallest unit is 2^-149, of which every fp32 number is a multiple.
+    ex = max(ex, 15);
+    const int up = 127 + 164 - ex, up0 = min(up, 254);  // in two exact factors: one would overflow for the smallest x
+    const float up_by = __uint_as_float(static_cast<uint32_t>(up0) << 23), up_rest = __uint_as_float(static_cast<uint32_t>(127 + up - up0) << 23);
     uint32_t digits[2][4];                 // four digits of five bits each, 16 too large: the lower ones, the upper ones
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        const float t = bad ? 0.0f : v[e] * up, upper = rintf(t * (1.0f / 1048576.0f));
+        const float t = bad ? 0.0f : v[e] * up_by * up_rest, upper = rintf(t * (1.0f / 1048576.0f));
         const uint32_t low = static_cast<uint32_t>(__float2int_rn(fmaf(upper, -1048576.0f, t)) + 0x84210);  // 16 in each of four digits
         digits[0][e] = low;
         digits[1][e] = static_cast<uint32_t>(static_cast<int>(upper) + 0x84210) + (low >> 20);  // (the rest may be too large for its digits by one)
     }
-    // four bytes of digit d: sign and magnitude; this lane's four k are codes 0..3 (even lanes) or 4..7 of a word
+    // four bytes of digit d: sign and twice the magnitude; this lane's four k are codes 0..3 (even lanes) or 4..7 of a word
     int pair = 0;  // sums over the group of digit 2p and 32 times digit 2p + 1
 #pragma unroll
     for (int d = 0; d < 8; ++d) {
@@ -302,7 +304,8 @@ __device__ __forceinline__ void write_digits(float4 x, int r, int lane, uint8_t*
         for (int e = 0; e < 4; ++e) {
             const int g = static_cast<int>((digits[d / 4][e] >> (5 * (d % 4))) & 31u) - 16;
             sum += g;
-            four |= (g < 0 ? static_cast<uint32_t>(0x80 - g) : static_cast<uint32_t>(g)) << (8 * e);
+            const int mag = abs(g);
+            four |= static_cast<uint32_t>((mag + min(mag, 8)) | ((g >> 24) & 0x80)) << (8 * e);  // (2 mag: up to 16 as it stands, then in steps of 2)
         }
         const uint32_t other = __shfl_xor_sync(0xffffffffu, four, 1);
         const uint32_t first = lane & 1 ? other : four, second = lane & 1 ? four : other;
@@ -312,10 +315,11 @@ __device__ __forceinline__ void write_digits(float4 x, int r, int lane, uint8_t*
 #pragma unroll
         for (int s = 1; s < GROUP / 4; s <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);  // of the group's lanes
         pair = d & 1 ? pair + 32 * sum : sum;
-        if ((d & 1) && lane % (GROUP / 4) == 0) sums[((lane / (GROUP / 4)) * ROWS + r) * 4 + d / 2] = static_cast<float>(pair) * (1.0f / 262144.0f);
+        if ((d & 1) && lane % (GROUP / 4) == 0) sums[((lane / (GROUP / 4)) * ROWS + r) * 4 + d / 2] = static_cast<float>(pair) * (1.0f / 131072.0f);
     }
-    // what one unit of digit 0 stands for, times 2^18
-    if (lane == 0) sums[C::GPP * ROWS * 4 + r] = __uint_as_float(bad ? 0x7FC00000u : static_cast<uint32_t>(127 + ex - 164 + 18) << 23);
+    // x's step: what a unit of the joined digits stands for, 2^(ex - 164) of digit 0 by 2^17 (the accumulator's units) and 2^20 (those
+    // of the upper digits): 2^(ex - 127), no more than the largest |v| and more than half of it
+    if (lane == 0) sums[C::GPP * ROWS * 4 + r] = __uint_as_float(bad ? 0x7FC00000u : static_cast<uint32_t>(ex) << 23);
 }
 template <int GROUP, int ROWS>
 __global__ void __launch_bounds__(128) w4_digits_kernel(const float* __restrict__ x, int64_t ldx, int64_t m, int64_t k, int64_t pieces, uint8_t* __restrict__ image) {
@@ -578,7 +582,10 @@ w4_matmul_kernel(const __grid_constant__ CUtensorMap codes, const MmArgs P) {
                         const uint32_t* q = &d[c & 1][r * 8];
                         auto pair = [&](int e) { return fmaf(__uint_as_float(q[2 * e + 1]), 32.0f, __uint_as_float(q[2 * e])); };  // exact: below 2^20 units
                         const float w0 = fmaf(z, ds[r].x, pair(0)), w1 = fmaf(z, ds[r].y, pair(1)), w2 = fmaf(z, ds[r].z, pair(2)), w3 = fmaf(z, ds[r].w, pair(3));
-                        result[r0 + r] = fmaf(fmaf(fmaf(w3, 1024.0f, w2), 1048576.0f, fmaf(w1, 1024.0f, w0)), up[r], result[r0 + r]);
+                        // (Joined in units of the upper digits, so that up is the size of the group's largest product: it leaves fp32's
+                        // range where that does.  In units of digit 0 it was subnormal below products of 1e-32.  A factor of its own for
+                        // the step costs 2 to 7 %.)
+                        result[r0 + r] = fmaf(fmaf(fmaf(w1, 1024.0f, w0), 1.0f / 1048576.0f, fmaf(w3, 1024.0f, w2)), up[r], result[r0 + r]);
                     }
                 }
                 acc ^= 1;

@@ -448,7 +448,10 @@ ctk_status ctk_w4_dequantize_f32(const uint32_t* packed, const float* scales, co
  * Made for few rows (the weight's bytes are the bound up to about 8 rows); any m is taken.  fp32-level accuracy:
  * x enters rounded to within 2^-38 of the largest |x| among the 128 consecutive k (from a multiple of 128) of its
  * row that hold it, the sums within a group are exact, and the groups' sums are joined in fp32 in an order that
- * depends on the sizes only.  A row of x that holds an infinity or a NaN gives NaN.  x must not overlap y.
+ * depends on the sizes only.  That holds for x of any size, subnormal numbers included, as long as
+ * the largest of those |x| times the scale is a normal fp32 number itself: below 2^-125 a group's sum may be off by
+ * 2^-138 more, from 2^128 on the result is not finite even where the codes are the zero point.  A row of x that
+ * holds an infinity or a NaN gives NaN.  x must not overlap y.
  * x's digits, about 8.2 bytes per element, come from the device's pool in the stream's order where x is not small. */
 ctk_status ctk_w4_matmul_f32(const float* x, int64_t ldx, const uint32_t* packed, const float* scales, const uint8_t* zeros,
                              const float* bias, int relu, float* y, int64_t ldy, int64_t m, int64_t k, int64_t n,
