@@ -629,7 +629,7 @@ w4_matmul_kernel(const __grid_constant__ CUtensorMap codes, const MmArgs P) {
             v = R[r * R_PITCH + c];
         }
         if (P.bias) v += __ldg(P.bias + col_base + c);
-        if (P.relu) v = v > 0.0f ? v : 0.0f;
+        if (P.relu) v = v <= 0.0f ? 0.0f : v;  // (a NaN stays one)
         P.y[(row_base + r) * P.ldy + col_base + c] = v;
     }
     if (split > 1) cluster_sync_all();  // the peers have read this CTA's sums

@@ -451,7 +451,9 @@ ctk_status ctk_w4_dequantize_f32(const uint32_t* packed, const float* scales, co
  * depends on the sizes only.  That holds for x of any size, subnormal numbers included, as long as
  * the largest of those |x| times the scale is a normal fp32 number itself: below 2^-125 a group's sum may be off by
  * 2^-138 more, from 2^128 on the result is not finite even where the codes are the zero point.  A row of x that
- * holds an infinity or a NaN gives NaN.  x must not overlap y.
+ * holds an infinity or a NaN gives NaN, and so do a column with a NaN among its scales and a NaN in the bias: relu lets it
+ * through (ctk_matmul_3xtf32_fused_f32's gives 0 for NaN), since the infinities among them would have stayed visible.
+ * x must not overlap y.
  * x's digits, about 8.2 bytes per element, come from the device's pool in the stream's order where x is not small. */
 ctk_status ctk_w4_matmul_f32(const float* x, int64_t ldx, const uint32_t* packed, const float* scales, const uint8_t* zeros,
                              const float* bias, int relu, float* y, int64_t ldy, int64_t m, int64_t k, int64_t n,

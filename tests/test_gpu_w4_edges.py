@@ -1,4 +1,5 @@
-"""4-bit weights at the ends of fp32's range: the product of very small and very large x and scales.
+"""4-bit weights at the ends of fp32's range: the product of very small and very large x and scales,
+and of what is not finite, under relu too.
 
 Tolerance of the product: that of the ordinary sizes, (group + groups + 40) 2^-23 sum |x| |w|, and near the smallest
 numbers half a step of 2^-149 for each of the at most groups + 10 roundings of the result."""
@@ -64,3 +65,43 @@ def test_products_below_the_smallest_normal_number(cb, m, k, n, group, factor, s
     x = (rng.standard_normal((m, k)) * factor).astype(np.float32)
     got = cb.ops.matmul_w4(cb.to_device(x), w4).numpy()
     assert (np.abs(got - x.astype(np.float64) @ w) <= bound_of(x, w, group) + -(-k // group) * 2.0 ** -138).all()
+
+
+@pytest.mark.parametrize("relu", [False, True])
+@pytest.mark.parametrize("m,k", [(1, 200), (5, 200), (5, 5000), (20, 900)])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+def test_non_finite_x_gives_nan_with_and_without_relu(cb, bad, m, k, relu):
+    rng = np.random.default_rng(6)
+    w4, _ = weight(cb, rng, k, 50, 64, False, 1.0)
+    b = cb.to_device(rng.standard_normal(50).astype(np.float32))
+    x = rng.standard_normal((m, k)).astype(np.float32)
+    clean = cb.ops.matmul_w4(cb.to_device(x), w4, bias=b, relu=relu).numpy()
+    x[m // 2, k // 3] = bad
+    y = cb.ops.matmul_w4(cb.to_device(x), w4, bias=b, relu=relu).numpy()
+    assert np.isnan(y[m // 2]).all()
+    assert np.array_equal(np.delete(y, m // 2, 0), np.delete(clean, m // 2, 0)) and np.isfinite(clean).all()
+
+
+def test_nan_scales_and_bias_show_under_relu(cb):
+    rng = np.random.default_rng(7)
+    w = rng.standard_normal((96, 6)).astype(np.float32)
+    w[40, 2] = np.inf
+    q = cb.ops.w4_quantize(cb.to_device(w), group=32)
+    b = np.ones(6, np.float32)
+    b[4] = np.nan
+    y = cb.ops.matmul_w4(cb.to_device(np.ones((3, 96), np.float32)), q, bias=cb.to_device(b), relu=True).numpy()
+    assert np.isnan(y[:, [2, 4]]).all() and np.isfinite(y[:, [0, 1, 3, 5]]).all() and (y[:, [0, 1, 3, 5]] >= 0).all()
+
+
+def test_a_poisoned_hidden_layer_shows_in_the_prediction(cb):
+    from ctorch_b200 import frontend as F
+    rng = np.random.default_rng(9)
+    dims = [40, 64, 10]
+    params = rng.standard_normal(40 * 64 + 64 + 64 * 10 + 10).astype(np.float32)
+    x = F.Tensor.from_numpy(rng.random((5, 40)).astype(np.float32))
+    for bad in (np.nan, np.inf, -np.inf):
+        poisoned = params.copy()
+        poisoned[7 * 64 + 3] = bad
+        tr = F.MlpTrainer(dims, poisoned, 0.1)
+        tr.quantize_w4(group=32)
+        assert np.isnan(tr.predict_w4(x).numpy()).all()
