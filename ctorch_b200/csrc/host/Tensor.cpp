@@ -904,6 +904,7 @@ void Tensor::muon_update_from_(const float* g_device, Tensor& momentum, const Mu
 
 W4Weight W4Weight::quantize(const Tensor& w, int group, bool symmetric) {
     want_matrix(w, "W4Weight::quantize");
+    want_untracked(w, "W4Weight::quantize");
     if (group != 32 && group != 64 && group != 128) refuse(ErrorType::DIMENSION, "W4Weight::quantize: group must be 32, 64 or 128");
     if (w.numel() == 0) refuse(ErrorType::DIMENSION, "W4Weight::quantize: empty weight");
     W4Weight q;
@@ -940,6 +941,7 @@ Tensor Tensor::linear_w4(const W4Weight& W, const Tensor* bias, bool relu) const
     if (bias) {
         if (bias->device() != DeviceType::kCUDA || bias->dtype() != DType::kFloat) refuse(ErrorType::DEVICE_COMPAT, "linear_w4: float device bias expected");
         if (bias->numel() != W.n() || !bias->is_contiguous()) refuse(ErrorType::DIMENSION, "linear_w4: one bias per column expected");
+        want_untracked(*bias, "linear_w4");
     }
     std::vector<size_t> shape = _shape;
     shape.back() = W.n();

@@ -196,7 +196,8 @@ public:
     void sgd_update_shared_(const Tensor& g, float lr);
 
     // ---- orthogonalised updates and 4-bit weights (no counterpart in the reference) ----
-    // These are not recorded on the tape; a tensor whose gradient the current tape would follow is refused.
+    // These are not recorded on the tape.  What returns a tensor or a 4-bit weight refuses a tensor (a bias too) whose gradient
+    // the current tape would follow; muon_update_ changes a leaf in place, as sgd_update_ does.
     // This 2-D contiguous float device tensor with singular values near 1 (ctk_orthogonalize_f32).
     Tensor orthogonalize(int steps = 5, float eps = 1e-7f) const;
     // One orthogonalised step of this weight matrix, in place, next to sgd_update_: momentum is a tensor of the same shape,

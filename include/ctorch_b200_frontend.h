@@ -94,7 +94,8 @@ int cth_linear(void* x, void* w, void* bias, int relu, void** out);
 int cth_sgd_update(void* param, void* grad, float lr); /* p -= g*lr on the device (mnist/mnist.cpp:80-92) */
 
 /* ---- orthogonalised updates and 4-bit weights (no counterpart in the reference) ----
- * Not recorded on the tape: a tensor that requires grad while a context is current is refused. */
+ * Not recorded on the tape: orthogonalize, w4_quantize and linear_w4 refuse a tensor (x and the bias) that requires grad while a
+ * context is current; muon_update changes a leaf in place, as sgd_update does. */
 int cth_orthogonalize(void* tensor, int steps, float eps, void** out);   /* ctk_orthogonalize_f32 of a 2-D tensor */
 /* One orthogonalised step of a weight matrix [in, out] in place, next to cth_sgd_update; momentum: a tensor of the same
  * shape, updated in place.  scale < 0: sqrt(max(1, out / in)). */
