@@ -437,8 +437,9 @@ ctk_status ctk_orthogonalize_status(int* status);
 size_t ctk_w4_packed_bytes(int64_t k, int64_t n, int group);
 /* Quantises w [k, n] (row pitch ldw).  zeros == NULL: symmetric, scale = max|w| / 7 of the group, code =
  * round(w / scale) + 8.  Otherwise scale = (max(w, 0) - min(w, 0)) / 15, zero = round(-min(w, 0) / scale), code =
- * round(w / scale) + zero clamped to [0, 15].  Scales are rounded to the nearest fp32 number, quotients exactly
- * (ties to even).  A group of zeros gets scale 0; a group with a non-finite weight gets scale NaN. */
+ * round(w / scale) + zero clamped to [0, 15].  (Where a scale is subnormal it can be less than that fraction of the range: the
+ * zero point is clamped to 15 then, and symmetric codes to [1, 15].)  Scales are rounded to the nearest fp32 number, quotients
+ * exactly (ties to even).  A group of zeros gets scale 0; a group with a non-finite weight gets scale NaN. */
 ctk_status ctk_w4_quantize_f32(const float* w, int64_t ldw, int64_t k, int64_t n, int group, uint32_t* packed,
                                float* scales, uint8_t* zeros, void* stream);
 /* The values a 4-bit weight stands for, w [k, n] with row pitch ldw. */
