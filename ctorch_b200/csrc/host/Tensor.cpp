@@ -828,14 +828,20 @@ void Tensor::sgd_update_(const Tensor& g, float lr) {
     sgd_update_from_(g.data<float>(), lr);
 }
 
-void Tensor::sgd_update_from_(const float* g_device, float lr) {
+float* Tensor::shared_data_() {
+    _storage.drop_split();
+    return static_cast<float*>(_storage.raw()) + _storage_offset;
+}
+
+void Tensor::sgd_update_from_(const float* g_device, float lr, bool shared) {
     if (_device != DeviceType::kCUDA || _dtype != DType::kFloat)
         Ctorch_Error::throwException(ErrorPlatform::kGENERAL, ErrorType::DEVICE_COMPAT, "sgd_update_: float device tensor expected");
     // A weight matrix that enters products (its buffer carries a kept hi/lo split) gets the split of
     // its new value from the update kernel itself instead of a separate pass before the next product.
     const bool resplit = _storage.has_split() && _shape.size() == 2 && is_contiguous() && _shape[1] % 4 == 0 && _storage_offset % 4 == 0 &&
                          (reinterpret_cast<uintptr_t>(g_device) & 15u) == 0;
-    float* p = data<float>();  // detaches from sharers, drops the split of the old value
+    // data() detaches from sharers and drops the split of the old value
+    float* p = !shared ? data<float>() : resplit ? static_cast<float*>(_storage.raw()) + _storage_offset : shared_data_();
     if (resplit) {
         const int64_t outer = static_cast<int64_t>(_shape[0]), inner = static_cast<int64_t>(_shape[1]);
         KeptSplit* ks = _storage.kept_split(static_cast<int64_t>(_storage_offset), outer, inner, inner, ctk_matmul_split_bytes(inner, outer));
@@ -844,6 +850,7 @@ void Tensor::sgd_update_from_(const float* g_device, float lr) {
             ks->valid = ctk_matmul_split_tag_for(p, inner, inner);
             return;
         }
+        if (shared) _storage.drop_split();
     }
     cuda_check(ctk_sgd_update_f32(p, g_device, lr, static_cast<int64_t>(numel()), t_stream), "sgd_update_");
 }
@@ -889,13 +896,7 @@ void Tensor::muon_update_from_(const float* g_device, Tensor& momentum, const Mu
     const int64_t rows = extent(*this, 0), cols = extent(*this, 1), ld = cols ? cols : 1;
     const float scale = o.scale >= 0.0f ? o.scale : std::sqrt(std::max(1.0f, static_cast<float>(cols) / static_cast<float>(rows ? rows : 1)));
     float* m = momentum.data<float>();
-    float* p;
-    if (shared) {
-        p = static_cast<float*>(_storage.raw()) + _storage_offset;  // no detach: the sharers are meant to see it
-        _storage.drop_split();                                      // a split of the old values, if any, is stale now
-    } else {
-        p = data<float>();  // detaches from sharers, drops the split of the old value
-    }
+    float* p = shared ? shared_data_() : data<float>();  // (data() detaches from sharers; both drop the split of the old value)
     Tensor ws(ShapeTag{}, {ctk_orthogonalize_workspace_bytes(rows, cols) / sizeof(float) + 1}, DType::kFloat, DeviceType::kCUDA, false);
     cuda_check(ctk_muon_update_f32(p, ld, g_device, ld, m, ld, rows, cols, o.lr, o.momentum, o.nesterov ? 1 : 0, o.weight_decay, scale, o.steps, o.eps,
                                    ws.data<float>(), t_stream),

@@ -188,7 +188,10 @@ public:
     // The same update with the gradient given as a raw device pointer to numel() contiguous floats
     // (16-byte aligned for the form that also rewrites the kept split): gradients that live in a
     // communicator's registered buffer instead of a Tensor.
-    void sgd_update_from_(const float* g_device, float lr);
+    // shared: written through to every tensor that shares this buffer, as sgd_update_shared_.
+    void sgd_update_from_(const float* g_device, float lr, bool shared = false);
+    // The buffer itself for a write that every sharer is meant to see: no detach; the split of the old values, if any, is dropped.
+    float* shared_data_();
     // The same update written THROUGH to every tensor that shares this buffer -- in particular the copy
     // the tape took when the parameter was registered, which the reference's backward keeps reading
     // while the live weights move on (src/AutoDiff.cpp:286-290, :1651).  With this form backward sees

@@ -416,7 +416,7 @@ public:
                     // every rank's shard travels to everyone.  The weights' kept split is dropped by the
                     // write access; the next product that reads them makes it again.
                     const int64_t chunk = slot_len[p] / comm_world, first = comm_rank * chunk;
-                    float* w = t.data<float>();
+                    float* w = fresh_weights ? t.shared_data_() : t.data<float>();
                     cuda_check(ctk_sgd_update_f32(w + first, slot + first, lr, chunk, st), "sharded update");
                     cuda_check(ctk_event_record(event_in(ev_upd, p), st), "record");
                     cuda_check(ctk_stream_wait_event(comm_stream, ev_upd[p]), "wait");
@@ -425,7 +425,7 @@ public:
                     return;
                 }
                 if (muon_param(p)) t.muon_update_from_(slot, muon.momentum[p / 2], muon.options, fresh_weights);
-                else t.sgd_update_from_(slot, lr);
+                else t.sgd_update_from_(slot, lr, fresh_weights);
                 return;
             }
             if (muon_param(p)) {
