@@ -170,7 +170,7 @@ public:
     // Orthogonalised steps for the weight matrices (no counterpart in the reference; off by default).  Biases keep
     // the SGD step with the trainer's lr, and with hidden_only so do the first and the last layer's weights.
     struct Muon {
-        bool on = false, hidden_only = false;
+        bool on = false, hidden_only = false, used = false;
         MuonOptions options;
         std::vector<Tensor> momentum;  // per layer
     } muon;
@@ -180,6 +180,7 @@ public:
             throw std::runtime_error("cth_mlp_set_muon: steps in [1, 64], eps > 0 and momentum in [0, 1) expected");
         release_graph();  // a recorded step holds the old rule
         muon.on = on;
+        muon.used = muon.used || on;
         muon.options = o;
         muon.hidden_only = hidden_only;
         if (on && muon.momentum.empty()) {
@@ -196,10 +197,18 @@ public:
         const size_t l = static_cast<size_t>(p / 2);
         return !muon.hidden_only || (l > 0 && l + 1 < W.size());
     }
+    // Whoever reads the weights learns of a step whose kernels gave up a wait: what it left in them is not an update.
+    void check_muon_waits() {
+        if (!muon.used) return;
+        int status = 0;
+        cuda_check(ctk_orthogonalize_status(&status), "orthogonalised steps: status");
+        if (status) throw std::runtime_error("a bounded wait of an orthogonalised step ran out (status " + std::to_string(status) + "): this trainer's weights are no longer defined");
+    }
     // The momentum of every weight matrix, packed in layer order, for a checkpoint.
     void muon_state(float* out, const float* in) {
         if (!muon.on) throw std::runtime_error("cth_mlp_*_muon_state: switch orthogonalised steps on first");
         finish_exchange();
+        if (out) check_muon_waits();
         cuda_check(ctk_device_sync(), "muon_state sync");
         for (Tensor& m : muon.momentum) {
             if (out) { m.copy_to_host(out, m.numel()); out += m.numel(); }
@@ -212,6 +221,7 @@ public:
     std::vector<Tensor> b4;
     void quantize_w4(int group, bool symmetric) {
         finish_exchange();
+        check_muon_waits();
         AutoDiffContext::Guard guard(nullptr);
         std::vector<W4Weight> q;
         for (const Tensor& w : W) q.push_back(W4Weight::quantize(w, group, symmetric));
@@ -784,6 +794,7 @@ public:
 
     void get_params(float* out) {
         finish_exchange();
+        check_muon_waits();
         for (size_t l = 0; l < W.size(); ++l) {
             W[l].copy_to_host(out, W[l].numel());
             out += W[l].numel();

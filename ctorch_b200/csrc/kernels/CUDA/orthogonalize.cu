@@ -409,7 +409,7 @@ __global__ void __launch_bounds__(THREADS, 1) ns_product_kernel(const __grid_con
             }
             if (!ok) {
                 st_cluster_u32(peer_abort, 1u);
-                for (int i = 0; i < 2048; ++i) __nanosleep(1000);
+                settle();
             }
         }
     } else if (warp == 1) {
@@ -610,8 +610,7 @@ __global__ void __launch_bounds__(MID_THREADS, 1) ns_tile_kernel(const __grid_co
             }
             // (every copy issued has been waited for by the multiplying warp unless a wait ran out: then give the copies in flight
             // a couple of milliseconds to land)
-            if (!ok)
-                for (int i = 0; i < 2048; ++i) __nanosleep(1000);
+            if (!ok) settle();
         }
     } else if (warp == 1) {
         {
@@ -621,8 +620,11 @@ __global__ void __launch_bounds__(MID_THREADS, 1) ns_tile_kernel(const __grid_co
             constexpr uint32_t a_lbo = A_MN ? STAGE_BYTES / 4 : 0u, b_lbo = B_MN ? STAGE_BYTES / 4 : 0u;
             for (int i = 0; i < kb1 - kb0; ++i) {
                 const int st = i % STAGES, acc = i & 1;
-                if (!mbar_wait(tempty_bar(acc), ((i >> 1) & 1) ^ 1u, &abort_flag, &g_ns_status, 0x600 | acc)) break;
-                if (!mbar_wait(full_bar(st), (i / STAGES) & 1, &abort_flag, &g_ns_status, 0x610 | st)) break;
+                if (!mbar_wait(tempty_bar(acc), ((i >> 1) & 1) ^ 1u, &abort_flag, &g_ns_status, 0x600 | acc) ||
+                    !mbar_wait(full_bar(st), (i / STAGES) & 1, &abort_flag, &g_ns_status, 0x610 | st)) {
+                    settle();  // (the loading warp may have issued its last copies and be gone)
+                    break;
+                }
                 fence_after();
                 const uint32_t d = tmem + acc * 128;
                 const uint64_t a = make_desc(smem_base + st * STAGE_BYTES, a_lbo), b = make_desc(smem_base + st * STAGE_BYTES + STAGE_BYTES / 2, b_lbo);
@@ -643,7 +645,10 @@ __global__ void __launch_bounds__(MID_THREADS, 1) ns_tile_kernel(const __grid_co
         const uint32_t t_row = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + c0;
         for (int i = 0; i < kb1 - kb0; ++i) {
             const int acc = i & 1;
-            if (!mbar_wait(tfull_bar(acc), (i >> 1) & 1, &abort_flag, &g_ns_status, 0x700 | acc)) break;
+            if (!mbar_wait(tfull_bar(acc), (i >> 1) & 1, &abort_flag, &g_ns_status, 0x700 | acc)) {
+                settle();
+                break;
+            }
             fence_after();
             uint32_t r[32];
             tmem_ld32(t_row + acc * 128, r);
@@ -1123,6 +1128,7 @@ __global__ void __launch_bounds__(CL_THREADS, 1) ns_cluster_kernel(const Cluster
             *reinterpret_cast<Vec<V>*>(at[k]) = o;
         }
     }
+    if (abort_flag) settle();
     if (ctas > 1) cluster_sync_all();  // no CTA leaves while another may still signal it
     else __syncthreads();
     if (warp == 0) {

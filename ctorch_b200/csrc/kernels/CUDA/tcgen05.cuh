@@ -47,6 +47,13 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
     return false;
 }
 
+// What a role does when its wait has run out: a couple of milliseconds for the copies and products in flight, before their memory is
+// used for anything else, freed or left.
+__device__ __forceinline__ void settle() {
+#pragma unroll 1
+    for (int i = 0; i < 2048; ++i) __nanosleep(1000);
+}
+
 // One lane of a converged warp, chosen so that the compiler knows it is one: instructions that take their operands from
 // uniform registers (tcgen05.mma, tcgen05.commit, TMA copies) are then issued directly, where behind `lane == 0` each is wrapped
 // in a loop over possibly different lanes.  Measured per kind::f8f6f4 instruction of N = 16: 20 clocks (A in tensor memory) and

@@ -602,6 +602,11 @@ w4_matmul_kernel(const __grid_constant__ CUtensorMap codes, const MmArgs P) {
     // ---- the sums of the cluster's CTAs ----
     fence_before();
     __syncthreads();  // no operand is read any more
+    if (abort_flag) {  // a wait has run out: no plausible numbers
+        settle();
+#pragma unroll
+        for (int r = 0; r < C::MINE; ++r) result[r] = __int_as_float(0x7fc00000);
+    }
     fence_after();
     if (warp == W_MMA) tmem_dealloc<1>(tmem, C::TMEM_COLS);
     float* const R = reinterpret_cast<float*>(smem);

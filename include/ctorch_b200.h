@@ -421,7 +421,8 @@ ctk_status ctk_orthogonalize_f32(const float* g, int64_t ldg, float* out, int64_
 ctk_status ctk_muon_update_f32(float* p, int64_t ldp, const float* g, int64_t ldg, float* momentum, int64_t ldm,
                                int64_t rows, int64_t cols, float lr, float mu, int nesterov, float weight_decay,
                                float scale, int steps, float eps, void* workspace, void* stream);
-/* Device status word of these kernels' bounded waits: 0 = none ran out.  Synchronises the device. */
+/* Device status word of these kernels' bounded waits: 0 = none ran out; a call in which one did leaves an undefined result.
+ * Synchronises the device. */
 ctk_status ctk_orthogonalize_status(int* status);
 
 /* ------------------------------------------------------------------------------------------- */
@@ -459,7 +460,8 @@ ctk_status ctk_w4_dequantize_f32(const uint32_t* packed, const float* scales, co
 ctk_status ctk_w4_matmul_f32(const float* x, int64_t ldx, const uint32_t* packed, const float* scales, const uint8_t* zeros,
                              const float* bias, int relu, float* y, int64_t ldy, int64_t m, int64_t k, int64_t n,
                              int group, void* stream);
-/* Device status word of the product's bounded waits: 0 = none ran out.  Synchronises the device. */
+/* Device status word of the product's bounded waits: 0 = none ran out; a call in which one did gives NaN in the columns
+ * that it did not finish.  Synchronises the device. */
 ctk_status ctk_w4_status(int* status);
 
 /* ------------------------------------------------------------------------------------------- */

@@ -190,7 +190,8 @@ int cth_tensor_narrow_rows(void* tensor, int64_t start, int64_t count, void** ou
  * lr is theirs; biases, and with hidden_only the first and the last layer's weights, keep SGD with the trainer's lr.
  * on == 0 returns to SGD and drops the momentum.  Works in the eager, the graph and the data-parallel step except the sharded
  * update (mode 3), which is refused.  May be called between steps of any kind: a recorded graph is released, and the graph step
- * runs eagerly twice before it records the new rule.  get / set_muon_state: the momenta, packed in
+ * runs eagerly twice before it records the new rule.  If a kernel of such a step ever gives up a wait (ctk_orthogonalize_status), reading
+ * the weights (get_params, quantize_w4, get_muon_state) fails from then on.  get / set_muon_state: the momenta, packed in
  * layer order (the sizes of the weights), for a checkpoint. */
 int cth_mlp_set_muon(void* mlp, int on, float lr, float mu, int nesterov, float weight_decay, float scale, int steps,
                      float eps, int hidden_only);
