@@ -6,6 +6,7 @@
 // Also holds MlpTrainer: the training step of the reference's mnist/mnist.cpp:44-92 written against
 // this front end for any layer list, with an optional NCCL gradient all-reduce that overlaps
 // backward (data-parallel replicas; the reference is single-process).
+#include <cmath>
 #include <cstring>
 #include <memory>
 #include <string>
@@ -176,8 +177,8 @@ public:
     } muon;
     void set_muon(bool on, const MuonOptions& o, bool hidden_only) {
         if (on && dp_mode == DP_SHARDED) throw std::runtime_error("cth_mlp_set_muon: a sharded update owns parts of a matrix, an orthogonalised step needs all of it; use another data-parallel mode");
-        if (on && (!(o.steps >= 1 && o.steps <= 64) || !(o.eps > 0.0f) || !(o.momentum >= 0.0f && o.momentum < 1.0f)))
-            throw std::runtime_error("cth_mlp_set_muon: steps in [1, 64], eps > 0 and momentum in [0, 1) expected");
+        if (on && (!(o.steps >= 1 && o.steps <= 64) || !(o.eps > 0.0f && std::isfinite(o.eps)) || !(o.momentum >= 0.0f && o.momentum < 1.0f)))
+            throw std::runtime_error("cth_mlp_set_muon: steps in [1, 64], a finite eps > 0 and momentum in [0, 1) expected");
         release_graph();  // a recorded step holds the old rule
         muon.on = on;
         muon.used = muon.used || on;
