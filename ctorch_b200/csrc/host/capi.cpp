@@ -180,17 +180,19 @@ public:
         if (on && (!(o.steps >= 1 && o.steps <= 64) || !(o.eps > 0.0f && std::isfinite(o.eps)) || !(o.momentum >= 0.0f && o.momentum < 1.0f)))
             throw std::runtime_error("cth_mlp_set_muon: steps in [1, 64], a finite eps > 0 and momentum in [0, 1) expected");
         release_graph();  // a recorded step holds the old rule
+        if (on && muon.momentum.empty()) {
+            std::vector<Tensor> fresh;  // (complete or not at all: there may be no room for it)
+            for (Tensor& w : W) {
+                fresh.emplace_back(ShapeTag{}, w.sizes(), DType::kFloat, DeviceType::kCUDA, true);
+                fresh.back().data<float>();
+            }
+            cuda_check(ctk_device_sync(), "set_muon sync");
+            muon.momentum = std::move(fresh);
+        }
         muon.on = on;
         muon.used = muon.used || on;
         muon.options = o;
         muon.hidden_only = hidden_only;
-        if (on && muon.momentum.empty()) {
-            for (Tensor& w : W) {
-                muon.momentum.emplace_back(ShapeTag{}, w.sizes(), DType::kFloat, DeviceType::kCUDA, true);
-                muon.momentum.back().data<float>();
-            }
-            cuda_check(ctk_device_sync(), "set_muon sync");
-        }
         if (!on) muon.momentum.clear();
     }
     bool muon_param(int p) const {
