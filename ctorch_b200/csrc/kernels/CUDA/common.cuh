@@ -48,6 +48,17 @@ inline bool spans_overlap(const void* a, int64_t rows_a, int64_t cols_a, int64_t
     return shift < first || shift + second > lda;
 }
 
+// Whether the [rows, cols] fp32 array at a, row pitch ld, shares a byte with the `bytes` bytes at b.
+inline bool touches(const void* a, int64_t rows, int64_t cols, int64_t ld, const void* b, size_t bytes) {
+    if (!b || rows <= 0 || cols <= 0 || bytes == 0) return false;
+    const uintptr_t a0 = reinterpret_cast<uintptr_t>(a), b0 = reinterpret_cast<uintptr_t>(b), b1 = b0 + bytes;
+    const uintptr_t pitch = 4 * static_cast<uintptr_t>(ld), row = 4 * static_cast<uintptr_t>(cols);
+    if (a0 >= b1 || b0 >= a0 + (static_cast<uintptr_t>(rows) - 1) * pitch + row) return false;
+    if (b0 <= a0) return true;
+    const uintptr_t r = (b0 - a0) / pitch;  // b starts in this row or in the gap behind it
+    return (b0 - a0) % pitch < row || (r + 1 < static_cast<uintptr_t>(rows) && b1 > a0 + (r + 1) * pitch);
+}
+
 inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s); }
 
 // NVTX range around the host side of an entry point (header-only NVTX: a no-op costing a few

@@ -743,6 +743,12 @@ ctk_status matmul_rows(const MmArgs& P, cudaStream_t st) {
     }
 }
 
+// Whether an fp32 matrix shares memory with a part of the 4-bit weight.
+bool touches_weight(const float* a, int64_t rows, int64_t cols, int64_t ld, const uint32_t* packed, const float* scales, const uint8_t* zeros, int64_t k, int64_t n, int group) {
+    const size_t groups = static_cast<size_t>((k + group - 1) / group) * static_cast<size_t>(n);
+    return touches(a, rows, cols, ld, packed, groups * static_cast<size_t>(group / 2)) || touches(a, rows, cols, ld, scales, groups * 4) || touches(a, rows, cols, ld, zeros, groups);
+}
+
 bool group_ok(int group) { return group == 32 || group == 64 || group == 128; }
 constexpr int64_t kMaxExtent = int64_t(1) << 30;
 
@@ -765,6 +771,7 @@ ctk_status ctk_w4_quantize_f32(const float* w, int64_t ldw, int64_t k, int64_t n
     CTK_REQUIRE(w && packed && scales, "ctk_w4_quantize_f32: null pointer");
     CTK_REQUIRE((reinterpret_cast<uintptr_t>(packed) & 15u) == 0, "ctk_w4_quantize_f32: packed must be 16-byte aligned");
     CTK_REQUIRE(aligned_to(w, 4) && aligned_to(scales, 4), "ctk_w4_quantize_f32: misaligned pointer");
+    CTK_REQUIRE(!touches_weight(w, k, n, ldw, packed, scales, zeros, k, n, group), "ctk_w4_quantize_f32: w overlaps packed, scales or zeros");
     const int64_t groups = (k + group - 1) / group, per_cta = group == 32 ? quantize_parts(32) : 1;
     const int64_t grid = (groups + per_cta - 1) / per_cta * ((n + W4_THREADS - 1) / W4_THREADS);
     if (grid > 0x7FFFFFFF) return fail(CTK_ERR_LIMIT, "ctk_w4_quantize_f32: too many groups");
@@ -787,6 +794,7 @@ ctk_status ctk_w4_dequantize_f32(const uint32_t* packed, const float* scales, co
     CTK_REQUIRE(w && packed && scales, "ctk_w4_dequantize_f32: null pointer");
     CTK_REQUIRE((reinterpret_cast<uintptr_t>(packed) & 15u) == 0, "ctk_w4_dequantize_f32: packed must be 16-byte aligned");
     CTK_REQUIRE(aligned_to(w, 4) && aligned_to(scales, 4), "ctk_w4_dequantize_f32: misaligned pointer");
+    CTK_REQUIRE(!touches_weight(w, k, n, ldw, packed, scales, zeros, k, n, group), "ctk_w4_dequantize_f32: w overlaps packed, scales or zeros");
     const int64_t groups = (k + group - 1) / group, grid = (k + 31) / 32 * ((n + W4_THREADS - 1) / W4_THREADS);
     if (grid > 0x7FFFFFFF) return fail(CTK_ERR_LIMIT, "ctk_w4_dequantize_f32: too large");
     w4_dequantize_kernel<<<static_cast<unsigned>(grid), W4_THREADS, 0, as_stream(stream)>>>(packed, scales, zeros, k, n, group, groups, w, ldw);
@@ -806,6 +814,9 @@ ctk_status ctk_w4_matmul_f32(const float* x, int64_t ldx, const uint32_t* packed
     CTK_REQUIRE((reinterpret_cast<uintptr_t>(packed) & 15u) == 0, "ctk_w4_matmul_f32: packed must be 16-byte aligned");
     CTK_REQUIRE(aligned_to(x, 4) && aligned_to(scales, 4) && aligned_to(bias, 4) && aligned_to(y, 4), "ctk_w4_matmul_f32: misaligned pointer");
     CTK_REQUIRE(!spans_overlap(x, m, k, ldx, y, m, n, ldy), "ctk_w4_matmul_f32: x and y overlap");
+    CTK_REQUIRE(!touches_weight(y, m, n, ldy, packed, scales, zeros, k, n, group), "ctk_w4_matmul_f32: y overlaps packed, scales or zeros");
+    // (one row added to what y holds: each element is read before it is written, and by the same thread)
+    CTK_REQUIRE((m == 1 && bias == y) || !touches(y, m, n, ldy, bias, static_cast<size_t>(n) * 4), "ctk_w4_matmul_f32: y overlaps bias");
     MmArgs P = {};
     P.x = x;
     P.ldx = ldx;

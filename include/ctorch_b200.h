@@ -440,7 +440,8 @@ size_t ctk_w4_packed_bytes(int64_t k, int64_t n, int group);
  * round(w / scale) + 8.  Otherwise scale = (max(w, 0) - min(w, 0)) / 15, zero = round(-min(w, 0) / scale), code =
  * round(w / scale) + zero clamped to [0, 15].  (Where a scale is subnormal it can be less than that fraction of the range: the
  * zero point is clamped to 15 then, and symmetric codes to [1, 15].)  Scales are rounded to the nearest fp32 number, quotients
- * exactly (ties to even).  A group of zeros gets scale 0; a group with a non-finite weight gets scale NaN. */
+ * exactly (ties to even).  A group of zeros gets scale 0; a group with a non-finite weight gets scale NaN.  w must not
+ * overlap the other arrays, here and in ctk_w4_dequantize_f32. */
 ctk_status ctk_w4_quantize_f32(const float* w, int64_t ldw, int64_t k, int64_t n, int group, uint32_t* packed,
                                float* scales, uint8_t* zeros, void* stream);
 /* The values a 4-bit weight stands for, w [k, n] with row pitch ldw. */
@@ -455,7 +456,7 @@ ctk_status ctk_w4_dequantize_f32(const uint32_t* packed, const float* scales, co
  * 2^-138 more, from 2^128 on the result is not finite even where the codes are the zero point.  A row of x that
  * holds an infinity or a NaN gives NaN, and so do a column with a NaN among its scales and a NaN in the bias: relu lets it
  * through (ctk_matmul_3xtf32_fused_f32's gives 0 for NaN), since the infinities among them would have stayed visible.
- * x must not overlap y.
+ * y must overlap neither x nor the weight's arrays, nor bias, except that one row (m = 1) may be added to y itself (bias == y).
  * x's digits, about 8.2 bytes per element, come from the device's pool in the stream's order where x is not small. */
 ctk_status ctk_w4_matmul_f32(const float* x, int64_t ldx, const uint32_t* packed, const float* scales, const uint8_t* zeros,
                              const float* bias, int relu, float* y, int64_t ldy, int64_t m, int64_t k, int64_t n,
