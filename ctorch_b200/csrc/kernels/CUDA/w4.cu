@@ -705,7 +705,7 @@ ctk_status launch_matmul(MmArgs P, int split, cudaStream_t st) {
 // cost START clocks (barriers, first loads, the cluster's sums), a block of 256 k in an SM that is full (two CTAs up to 8 rows,
 // one above) PER_BLOCK; alone on its SM a CTA of few rows is 1.4 times slower per block.  From 16384 x 16384 g128: 31.6 / 36 /
 // 45 / 68 us with 2 / 4 / 8 / 16 rows, 253 us for 64 rows in three passes of 24.  So 64 x 4096 x 4096 takes 16 rows and whole
-// columns (128 CTAs: 21.6 us; 24 rows and a split of 4: 31.8 us; 8 rows: 23.2 us) and 1 x 4096 x 4096 2 rows and a split of 8.
+// columns (128 CTAs: 21.6 us; 24 rows and a split of 4: 31.8 us; 8 rows: 23.2 us) and 1 x 4096 x 4096 2 rows and a split of 4.
 struct Shape {
     int rows, split;
 };
@@ -833,8 +833,9 @@ ctk_status ctk_w4_matmul_f32(const float* x, int64_t ldx, const uint32_t* packed
     P.relu = relu;
     P.quads = P.groups % 4 == 0 && aligned_to(scales, 16) && aligned_to(zeros, 4);
     cudaStream_t st = as_stream(stream);
-    // x's digits take about 8.2 bytes per element of x: many rows go in slabs of 512 MB of them (a multiple of every kernel's rows)
-    const int64_t per_row = P.groups * group * 9 + 1, slab = std::min<int64_t>(65520, std::max<int64_t>(48, (int64_t(512) << 20) / per_row / 48 * 48));
+    // x's digits take 8.3 to 12 bytes per element of x (X_BYTES / (128 ROWS)): many rows go in slabs of at most 512 MB of them (a
+    // multiple of every kernel's rows)
+    const int64_t per_row = P.groups * group * 12 + 1, slab = std::min<int64_t>(65520, std::max<int64_t>(48, (int64_t(512) << 20) / per_row / 48 * 48));
     for (int64_t r = 0; r < m; r += slab) {
         MmArgs Q = P;
         Q.m = m - r < slab ? m - r : slab;

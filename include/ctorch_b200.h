@@ -457,7 +457,8 @@ ctk_status ctk_w4_dequantize_f32(const uint32_t* packed, const float* scales, co
  * holds an infinity or a NaN gives NaN, and so do a column with a NaN among its scales and a NaN in the bias: relu lets it
  * through (ctk_matmul_3xtf32_fused_f32's gives 0 for NaN), since the infinities among them would have stayed visible.
  * y must overlap neither x nor the weight's arrays, nor bias, except that one row (m = 1) may be added to y itself (bias == y).
- * x's digits, about 8.2 bytes per element, come from the device's pool in the stream's order where x is not small. */
+ * x's digits come from the device's pool in the stream's order where x is not small: 8.3 to 12 bytes per element, for a number of
+ * rows rounded up to a multiple of 2 (one row), 4, 8, 16 or 24, 512 MB at a time. */
 ctk_status ctk_w4_matmul_f32(const float* x, int64_t ldx, const uint32_t* packed, const float* scales, const uint8_t* zeros,
                              const float* bias, int relu, float* y, int64_t ldy, int64_t m, int64_t k, int64_t n,
                              int group, void* stream);
